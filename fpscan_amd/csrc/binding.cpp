@@ -20,6 +20,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <cmath>
 #include <string>
 #include <utility>
 
@@ -523,6 +524,158 @@ at::Tensor pscan_softplus(const at::Tensor& z, const at::Tensor& rate, const at:
   return PScanSoftplusFunction::apply(z, rate, tokens, backward_follows({z, rate, tokens}));
 }
 
+// ---- the gated delta rule: q, k (batch, seqlen, key_heads, key_dim), v (batch, seqlen, heads,
+// value_dim), log_decay and beta (batch, seqlen, heads). Views (slices of a fused projection) are
+// taken as they are, where their last axis is contiguous.
+void check_heads(const at::Tensor& t, const at::Tensor& like, const char* name, int64_t dims) {
+  TORCH_CHECK(t.device().is_cuda(), name, " must be a CUDA tensor");
+  const auto st = t.scalar_type();
+  TORCH_CHECK(st == at::kHalf || st == at::kBFloat16 || st == at::kFloat, name,
+              " must be float16 or bfloat16 or float32");
+  TORCH_CHECK(st == like.scalar_type(), name, " must have the dtype of v (", like.scalar_type(),
+              "), got ", st);
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", got ",
+              t.device());
+  TORCH_CHECK(t.dim() == dims, name, " must be a ", dims, "-d (batch, seqlen, heads",
+              dims == 4 ? ", dim" : "", ") tensor, got ", t.dim(), " dims");
+}
+
+// The tensor's strides for the C ABI. An axis of one element has any stride in torch and none here.
+fpscan_heads heads_of(const at::Tensor& t) {
+  return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0,
+          t.size(2) > 1 ? t.stride(2) : 0};
+}
+
+void check_vectors(const at::Tensor& t, const char* name) {
+  const int64_t vec = 16 / (int64_t)t.element_size();
+  const fpscan_heads x = heads_of(t);
+  TORCH_CHECK(t.size(3) <= 1 || t.stride(3) == 1, name, " must have a contiguous last axis");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data) % 16 | x.stride_b % vec | x.stride_t % vec |
+               x.stride_h % vec) == 0, name, ": data and strides must be whole 16-byte vectors (",
+              vec, " elements)");
+}
+
+// Bytes from a tensor's first element to the end of its last, through its strides.
+int64_t span_bytes(const at::Tensor& t) {
+  if (t.numel() == 0) return 0;
+  int64_t n = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+  return n * (int64_t)t.element_size();
+}
+
+bool spans_overlap(const at::Tensor& a, const at::Tensor& b) {
+  const char* pa = static_cast<const char*>(a.data_ptr());
+  const char* pb = static_cast<const char*>(b.data_ptr());
+  const int64_t na = span_bytes(a), nb = span_bytes(b);
+  return na > 0 && nb > 0 && pa < pb + nb && pb < pa + na;
+}
+
+fpscan_delta delta_problem(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                           const at::Tensor& log_decay, const at::Tensor& beta,
+                           const c10::optional<double>& scale) {
+  check_heads(v, v, "v", 4);
+  check_heads(q, v, "q", 4);
+  check_heads(k, v, "k", 4);
+  check_heads(log_decay, v, "log_decay", 3);
+  check_heads(beta, v, "beta", 3);
+  const int64_t B = v.size(0), L = v.size(1), H = v.size(2), Dv = v.size(3);
+  TORCH_CHECK(k.size(0) == B && k.size(1) == L, "k must have the batch and seqlen of v (", B, ", ",
+              L, "), got ", k.sizes());
+  TORCH_CHECK(q.sizes() == k.sizes(), "q must have the shape of k ", k.sizes(), ", got ", q.sizes());
+  const int64_t Hk = k.size(2), Dk = k.size(3);
+  TORCH_CHECK(Hk > 0 ? H % Hk == 0 : H == 0, "v's heads (", H, ") must be a multiple of k's (", Hk,
+              ")");
+  for (const auto& [t, name] : {std::pair<const at::Tensor*, const char*>{&log_decay, "log_decay"},
+                                {&beta, "beta"}})
+    TORCH_CHECK(t->size(0) == B && t->size(1) == L && t->size(2) == H, name, " must have shape (", B,
+                ", ", L, ", ", H, "), got ", t->sizes());
+  TORCH_CHECK(Dk >= 8 && Dk <= FPSCAN_DELTA_MAX_KEY_DIM && Dk % 8 == 0,
+              "q and k: dim must be a multiple of 8, >= 8, <= ", FPSCAN_DELTA_MAX_KEY_DIM, ", got ",
+              Dk);
+  TORCH_CHECK(Dv >= 8 && Dv <= FPSCAN_DELTA_MAX_VALUE_DIM && Dv % 8 == 0,
+              "v: dim must be a multiple of 8, >= 8, <= ", FPSCAN_DELTA_MAX_VALUE_DIM, ", got ", Dv);
+  if (v.numel() > 0) {
+    check_vectors(q, "q");
+    check_vectors(k, "k");
+    check_vectors(v, "v");
+  }
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)Dk);
+  return {B, L, Hk, H, Dk, Dv, dtype_code(v.scalar_type()), (float)s, heads_of(q), heads_of(k),
+          heads_of(v), heads_of(log_decay), heads_of(beta)};
+}
+
+// `out` as a contiguous tensor of v's shape that shares no byte with what the call reads.
+void check_delta_out(const at::Tensor& out, const at::Tensor& v,
+                     std::initializer_list<const at::Tensor*> inputs, const char* op) {
+  TORCH_CHECK(out.is_contiguous(), "out must be contiguous");
+  check_like(out, v, "out", "v");
+  for (const at::Tensor* i : inputs)
+    TORCH_CHECK(!spans_overlap(out, *i), op, ": out must not overlap an input");
+}
+
+void check_state(const at::Tensor& state, const at::Tensor& v, int64_t Dk, int64_t slots,
+                 std::initializer_list<const at::Tensor*> others, const char* op) {
+  TORCH_CHECK(state.device() == v.device(), "state must be on ", v.device(), ", got ",
+              state.device());
+  TORCH_CHECK(state.scalar_type() == at::kFloat, "state must be float32, got ",
+              state.scalar_type());
+  TORCH_CHECK(state.is_contiguous(), "state must be contiguous");
+  TORCH_CHECK(state.dim() == 4 && (slots < 0 || state.size(0) == slots) &&
+                  state.size(1) == v.size(2) && state.size(2) == Dk && state.size(3) == v.size(3),
+              "state must have shape (", slots < 0 ? "slots" : std::to_string(slots), ", ",
+              v.size(2), ", ", Dk, ", ", v.size(3), "), got ", state.sizes());
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0,
+              "state must be 16-byte aligned");
+  TORCH_CHECK(!state.requires_grad() || !at::GradMode::is_enabled(), op, ": state is updated in "
+              "place and carries no gradient; detach it or call this under no_grad");
+  for (const at::Tensor* i : others)
+    TORCH_CHECK(!spans_overlap(state, *i), op, ": state must not overlap another tensor of the call");
+}
+
+at::Tensor gated_delta_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& log_decay, const at::Tensor& beta,
+                               const at::Tensor& out, const c10::optional<double>& scale,
+                               const c10::optional<at::Tensor>& state) {
+  const fpscan_delta p = delta_problem(q, k, v, log_decay, beta, scale);
+  check_delta_out(out, v, {&q, &k, &v, &log_decay, &beta}, "gated_delta_forward");
+  if (state.has_value())
+    check_state(*state, v, p.key_dim, p.batch, {&q, &k, &v, &log_decay, &beta, &out},
+                "gated_delta_forward");
+  if (v.numel() == 0) return out;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(v.device());
+  void* stream = launch_stream(v);
+  const size_t ws_bytes = fpscan_delta_workspace_bytes(&p, FPSCAN_OP_FWD);
+  at::Tensor ws = workspace(ws_bytes, v);
+  check_status(fpscan_delta_fwd(&p, out.data_ptr(), state.has_value() ? state->data_ptr<float>() : nullptr,
+                                ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, stream));
+  return out;
+}
+
+at::Tensor gated_delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& log_decay, const at::Tensor& beta,
+                            const at::Tensor& state, const at::Tensor& out,
+                            const c10::optional<double>& scale,
+                            const c10::optional<at::Tensor>& slots) {
+  const fpscan_delta p = delta_problem(q, k, v, log_decay, beta, scale);
+  check_delta_out(out, v, {&q, &k, &v, &log_decay, &beta}, "gated_delta_step");
+  check_state(state, v, p.key_dim, slots.has_value() ? -1 : p.batch,
+              {&q, &k, &v, &log_decay, &beta, &out}, "gated_delta_step");
+  if (slots.has_value()) {
+    TORCH_CHECK(slots->device() == v.device() && slots->scalar_type() == at::kInt &&
+                    slots->is_contiguous() && slots->dim() == 1 && slots->size(0) == p.batch,
+                "slots must be a contiguous int32 tensor with one entry per sequence (", p.batch,
+                ") on ", v.device());
+    TORCH_CHECK(!spans_overlap(state, *slots) && !spans_overlap(out, *slots),
+                "gated_delta_step: slots must not overlap state or out");
+  }
+  if (v.numel() == 0) return out;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(v.device());
+  check_status(fpscan_delta_step(&p, out.data_ptr(), state.data_ptr<float>(),
+                                 slots.has_value() ? slots->data_ptr<int32_t>() : nullptr,
+                                 state.size(0), launch_stream(v)));
+  return out;
+}
+
 // Look-back waits that gave up on the tensors' device since the library was loaded (waits for
 // the device first).
 uint64_t lookback_overruns(int64_t device) {
@@ -589,6 +742,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "d loss / d rate partial per row", pybind11::arg("z"), pybind11::arg("rate"),
         pybind11::arg("out"), pybind11::arg("grad_out"), pybind11::arg("grad_z"),
         pybind11::arg("grad_tokens"), pybind11::arg("grad_rate_rows"));
+  m.def("gated_delta_forward", &gated_delta_forward,
+        "the gated delta rule over whole sequences, written into out; state is updated in place",
+        pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"),
+        pybind11::arg("beta"), pybind11::arg("out"), pybind11::arg("scale"), pybind11::arg("state"));
+  m.def("gated_delta_step", &gated_delta_step,
+        "the gated delta rule token by token, written into out; state is updated in place",
+        pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"),
+        pybind11::arg("beta"), pybind11::arg("state"), pybind11::arg("out"), pybind11::arg("scale"),
+        pybind11::arg("slots"));
   m.def("dimwise_forward", &dimwise_forward,
         "contraction scan, in place into Bx (HIP, gfx950)", pybind11::arg("Ax"),
         pybind11::arg("Bx"), pybind11::arg("Bh"), pybind11::arg("Wq"), pybind11::arg("Wk"));

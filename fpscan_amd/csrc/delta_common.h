@@ -1,0 +1,153 @@
+// Pieces shared by the kernels of the gated delta rule: products of fp32 values on the bf16 matrix
+// units, and the one layout in which every matrix operand is kept.
+//
+// Products. An fp32 value is written as a sum of bf16 planes, x = p0 + p1 + p2 with p0 = bf16(x),
+// p1 = bf16(x - p0), p2 = bf16(x - p0 - p1): 8 bits of significand each, so two planes hold a value
+// to 2^-17 and three to 2^-25, over fp32's whole range (fp16 planes would not). A product of two
+// values is the sum of the plane products p_i p_j with i + j < kTerms, each exact in the matrix
+// units' fp32 accumulators. bf16 inputs are one plane, fp16 inputs two and fp32 inputs three, all
+// exact. Six bf16 products of 16x16x32 take 96 cycles where the fp32 matrix instructions take 256
+// for the same block.
+//
+// Layout ("frags"). The matrix instruction 16x16x32 wants from lane l = 16 g + i the row i of the
+// left operand (column i of the right) at eight values of the summed index; it returns column i,
+// rows 4 g .. 4 g + 3. A sum does not care for the order of its terms, so the eight values of lane
+// group g are taken to be {4 g + r, 16 + 4 g + r}: then two result tiles are, lane by lane, a right
+// operand of the next product, and a chain of products stays in registers. A matrix in memory (LDS
+// or global) is kept as blocks of 16 rows x 32 columns of 1 KiB, 16 bytes a lane, so that a block is
+// read as an operand by one 16-byte load a lane, and its transpose by two transposing 8-byte loads.
+#ifndef FPSCAN_DELTA_COMMON_H
+#define FPSCAN_DELTA_COMMON_H
+
+#include "scan_common.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+// Planes of an input element type, exact.
+template <class E> struct InputPlanes;
+template <> struct InputPlanes<BF16> { static constexpr int n = 1; };
+template <> struct InputPlanes<F16> { static constexpr int n = 2; };
+template <> struct InputPlanes<F32> { static constexpr int n = 3; };
+
+// x as kPlanes bf16 planes.
+template <int kPlanes>
+__device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[kPlanes]) {
+#pragma unroll
+  for (int i = 0; i < kPlanes; ++i) {
+    p[i] = __builtin_convertvector(x, bf16x8);
+    if (i + 1 < kPlanes) x -= __builtin_convertvector(p[i], f32x8);
+  }
+}
+
+__device__ __forceinline__ f32x8 join(f32x4 a, f32x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// c + a b over 32 values of the summed index, with the plane products i + j < kTerms.
+template <int kTerms, int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+#pragma unroll
+  for (int t = kTerms - 1; t >= 0; --t)  // small products first
+#pragma unroll
+    for (int i = 0; i <= t; ++i)
+      if (i < NA && t - i < NB)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[t - i], c, 0, 0, 0);
+  return c;
+}
+
+// Byte offset of lane (row i of 16, group q of 4 columns) in a 1 KiB block. The bit that moves row
+// i by eight for odd q spreads the transposing loads over all banks: their 16 lanes of a group read
+// four rows at all four q.
+__device__ __forceinline__ int frag_lane(int i, int q) {
+  return ((i ^ ((q & 1) << 3)) + 16 * q) * 16;
+}
+
+// Byte offset of the four columns col .. col + 3 (col a multiple of 4) of `row` in a matrix of
+// 32 * kBlocks columns.
+template <int kBlocks>
+__device__ __forceinline__ int frag_unit(int row, int col) {
+  return ((row >> 4) * kBlocks + (col >> 5)) * 1024 + frag_lane(row & 15, (col >> 2) & 3) +
+         ((col >> 4) & 1) * 8;
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+// One operand from a block: lane (i, g) takes row i.
+__device__ __forceinline__ bf16x8 frag_rows(const char* block, int lane) {
+  return *reinterpret_cast<const bf16x8*>(block + frag_lane(lane & 15, lane >> 4));
+}
+
+// One operand from the transpose: lane (i, g) takes column 16 (ct % 2) + i of blocks `lo` (16 rows)
+// and `hi` (the 16 rows after them), both the ones that hold column 16 ct. LDS only.
+__device__ __forceinline__ bf16x8 frag_cols(const char* lo, const char* hi, int ct, int lane) {
+  const int off = frag_lane(4 * (lane >> 4) + ((lane >> 2) & 3), lane & 3) + (ct & 1) * 8;
+  typedef __attribute__((address_space(3))) s16x4* ldsp;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ldsp)(lo + off));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ldsp)(hi + off));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Block of the lower triangle of a 64 x 64 matrix: rows 16 mt.., columns 32 s.. (s <= mt / 2).
+__device__ __forceinline__ constexpr int tri_block(int mt, int s) {
+  return mt < 2 ? mt : 2 * mt - 2 + s;
+}
+constexpr int kTriBytes = 6 * 1024;  // one plane of such a matrix
+
+// ------------------------------------------------------------------------ typed global memory
+// Eight consecutive elements at byte offset `off` (kNoOffset: zeros), exact.
+template <class E>
+__device__ __forceinline__ void load8(Rsrc r, uint32_t off, bf16x8 (&p)[InputPlanes<E>::n]) {
+  if constexpr (InputPlanes<E>::n == 1) {
+    p[0] = __builtin_bit_cast(bf16x8, bld16<0>(r, off));
+  } else if constexpr (InputPlanes<E>::n == 2) {
+    split(__builtin_convertvector(__builtin_bit_cast(f16x8, bld16<0>(r, off)), f32x8), p);
+  } else {
+    split(join(__builtin_bit_cast(f32x4, bld16<0>(r, off)),
+               __builtin_bit_cast(f32x4, bld16<0>(r, off + 16))), p);
+  }
+}
+
+template <class E>
+__device__ __forceinline__ float load1(Rsrc r, uint32_t off) {
+  if constexpr (E::kSize == 4)
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+  else
+    return E::widen16((unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+}
+
+template <class E>
+__device__ __forceinline__ void store1(Rsrc r, uint32_t off, float x) {
+  if constexpr (InputPlanes<E>::n == 3) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), r, off, 0, 0);
+  } else if constexpr (InputPlanes<E>::n == 2) {
+    const _Float16 h = static_cast<_Float16>(x);
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, h), r, off, 0, 0);
+  } else {
+    const __bf16 h = static_cast<__bf16>(x);
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, h), r, off, 0, 0);
+  }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
+  return x;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+}  // namespace
+
+#endif  // FPSCAN_DELTA_COMMON_H

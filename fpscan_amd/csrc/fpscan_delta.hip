@@ -1,0 +1,778 @@
+// The gated delta rule on MI355X: for every sequence b and head h a (key_dim, value_dim) state S,
+//   S' = exp(g_t) S[t-1];  e_t = v_t - k_t^T S';  S[t] = S' + k_t (beta_t e_t)^T
+//   out_t = scale q_t^T S[t].
+//
+// Chunks of 64 steps. With G the running sum of g in a chunk, Gam_ij = exp(G_i - G_j) and S the
+// state before it, the rows e of all 64 steps solve a unit lower triangular system:
+//   A_ij = Gam_ij k_i.k_j (j < i),  N = A (I + diag(beta) A)^-1,  M_ij = scale Gam_ij q_i.k_j (j <= i)
+//   R = V - exp(G) K S,   E = R - N (beta R),   U = beta E
+//   out = scale exp(G) Q S + M U,   S_next = exp(G_end) S + (exp(G_end - G) K)^T U.
+// N and M need no state: delta_prep makes them for all chunks at once. delta_chunks then walks the
+// chunks of a (sequence, head), with no other dependence than the state. Neither divides by beta or
+// by a decay: beta = 0 and decays of zero (log_decay = -inf: the state starts anew) are exact.
+//
+// Gradients (dO, and dS' of the state after a chunk, walked backwards by delta_chunks_bwd):
+//   dU = M^T dO + exp(G_end - G) K dS',  Y = dU - N^T (beta dU),  dV = beta Y
+//   dS = exp(G_end) dS' + Q^T (scale exp(G) dO) - K^T (exp(G) dV)
+// and then, for every chunk by itself (delta_grads), with P_ij = scale Gam_ij dO_i.U_j (j <= i) and
+// F_ij = -Gam_ij dV_i.U_j (j < i):
+//   dQ = scale exp(G) dO S^T + P K,  dK = exp(G_end - G) U dS'^T - exp(G) dV S^T + P^T Q + F K + F^T K
+//   dbeta_i = Y_i.E_i
+//   dG_i = q_i.dq_i + k_i.dk_i - 2 beta_i dbeta_i,  dg_t = sum_{i >= t} dG_i + <S_next, dS'>.
+#include "../../include/fpscan_hip.h"
+#include "delta_common.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr int kChunk = 64;
+constexpr float kLeastLog = -104.0f;  // exp of it and of all below is 0 in fp32
+
+struct Heads {  // element strides of a (batch, seqlen, heads, dim) tensor
+  const void* p;
+  int64_t b, t, h;
+};
+
+struct DeltaArgs {
+  Heads q, k, v, g, beta, go;
+  char* out;          // contiguous (batch, seqlen, heads, value_dim)
+  float* state;       // contiguous (batch, heads, key_dim, value_dim), or null
+  char *gb, *n, *m;   // per chunk: (G, beta), N, M
+  char *s, *e;        // saved per chunk: S before it, E
+  float *ss, *es;     // and their scales
+  char *ds, *y;       // the same of dS' and Y
+  float *dss, *ys;
+  char *gq, *gk, *gg, *gbeta;
+  const int32_t* slots;
+  int64_t L, chunks, heads_total, nslots;
+  int H, R, Dk, Dv, vblocks;
+  float scale;
+};
+
+// Terms of a product that feeds outputs of the tensors' type: 2^-17 for the half types. Products
+// that feed the state, where that is returned in fp32, take three.
+template <class E> constexpr int out_terms() { return InputPlanes<E>::n == 3 ? 3 : 2; }
+
+// Rows of one head from step t0 on: `rows` rows of `dim` elements, all else reads as zero.
+__device__ __forceinline__ Rsrc head_rsrc(const Heads& x, int64_t b, int64_t h, int64_t t0,
+                                          int rows, int dim, int size) {
+  const int bytes = rows > 0 ? (int)(((rows - 1) * x.t + dim) * size) : 0;
+  return row_rsrc(x.p, b * x.b + h * x.h + t0 * x.t, size, bytes);
+}
+
+// One element of a (batch, seqlen, heads) tensor.
+template <class E>
+__device__ __forceinline__ float element(const Heads& x, int64_t b, int64_t t, int64_t h) {
+  const int64_t at = b * x.b + t * x.t + h * x.h;
+  if constexpr (E::kSize == 4)
+    return static_cast<const float*>(x.p)[at];
+  else
+    return E::widen16(static_cast<const unsigned short*>(x.p)[at]);
+}
+
+// The wave's index in its workgroup, in a scalar register: what follows from it is uniform.
+__device__ __forceinline__ int wave_index() {
+  return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+}
+
+__device__ __forceinline__ int rows_left(int64_t L, int64_t t0) {
+  return (int)(L - t0 < kChunk ? L - t0 : kChunk);
+}
+
+// ------------------------------------------------------------------------------- preparation
+// One workgroup of four waves per (sequence, head, chunk). Wave w makes rows 16 w.. of K K^T and
+// Q K^T; then N = A - A beta N by blocks of 16: the inverses D of the diagonal blocks of
+// I + A beta by substitution, one wave each, and the blocks below them column by column, one wave
+// each, N_IK = D_I (A_IK - sum_{K <= J < I} (A beta)_IJ N_JK), with the fp32 matrix instruction.
+constexpr int kPrepStride = 68;
+
+template <class E, int KD, int kTerms, int kOut>
+__global__ __launch_bounds__(256) void delta_prep(DeltaArgs a) {
+  __shared__ __attribute__((aligned(16))) float A[kChunk][kPrepStride];
+  __shared__ __attribute__((aligned(16))) float M[kChunk][kPrepStride];
+  __shared__ __attribute__((aligned(16))) float D[4][16][20];
+  __shared__ __attribute__((aligned(16))) float ghi[kChunk], glo[kChunk], beta[kChunk];
+  constexpr int NI = InputPlanes<E>::n;
+  const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
+  const int64_t ch = blockIdx.x, bh = ch / a.chunks, t0 = (ch - bh * a.chunks) * kChunk;
+  const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / a.R;
+  const int rows = rows_left(a.L, t0);
+
+  if (w == 0) {
+    const bool in = lane < rows;
+    float g = 0.0f, bt = 0.0f;
+    if (in) {
+      g = element<E>(a.g, b, t0 + lane, h);
+      bt = element<E>(a.beta, b, t0 + lane, h);
+    }
+    g = g < kLeastLog ? kLeastLog : g;  // NaN stays
+    // differences of the running sum have to keep their precision after a decay of zero, whose
+    // -104 all later sums hold: summed in 64 bits, kept as two floats
+    double G = g;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double o = __shfl_up(G, d);
+      G += lane >= d ? o : 0.0;
+    }
+    const float hi = (float)G, lo = (float)(G - hi);
+    ghi[lane] = hi;
+    glo[lane] = lo;
+    beta[lane] = bt;
+    reinterpret_cast<f32x4*>(a.gb)[ch * kChunk + lane] = f32x4{hi, lo, bt, 0.0f};
+  }
+
+  f32x4 kk[4] = {}, qk[4] = {};
+  {
+    const Rsrc rk = head_rsrc(a.k, b, hk, t0, rows, a.Dk, E::kSize);
+    const Rsrc rq = head_rsrc(a.q, b, hk, t0, rows, a.Dk, E::kSize);
+    const int kst = (int)a.k.t * E::kSize, qst = (int)a.q.t * E::kSize;
+    for (int s = 0; s < KD / 32; ++s) {
+      const int d = 32 * s + 8 * lg;
+      const bool in = d < a.Dk;
+      bf16x8 ka[NI], qa[NI];
+      load8<E>(rk, in ? (16 * w + li) * kst + d * E::kSize : kNoOffset, ka);
+      load8<E>(rq, in ? (16 * w + li) * qst + d * E::kSize : kNoOffset, qa);
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+        if (nt <= w) {
+          bf16x8 kb[NI];
+          load8<E>(rk, in ? (16 * nt + li) * kst + d * E::kSize : kNoOffset, kb);
+          kk[nt] = mma<3>(ka, kb, kk[nt]);
+          qk[nt] = mma<3>(qa, kb, qk[nt]);
+        }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < 4; ++nt)
+    if (nt <= (w | 1)) {  // the blocks of 32 columns that reach the diagonal, zeros above it
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * w + 4 * lg + r, j = 16 * nt + li;
+        const float gam = j <= i ? expf((ghi[i] - ghi[j]) + (glo[i] - glo[j])) : 0.0f;
+        A[i][j] = j < i ? gam * kk[nt][r] : 0.0f;
+        M[i][j] = j <= i ? a.scale * (gam * qk[nt][r]) : 0.0f;
+      }
+    }
+  __syncthreads();
+
+  {  // D[w] = the inverse of I + (A beta)[w][w], lane by column
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == li ? 1.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) v = fmaf(-(A[16 * w + i][16 * w + j] * beta[16 * w + j]), x[j], v);
+      x[i] = v;
+    }
+    if (lg == 0)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) D[w][i][li] = x[i];
+  }
+  __syncthreads();
+  f32x4 n[4];
+#pragma unroll
+  for (int I = 0; I < 4; ++I)
+    if (I >= w) {
+      f32x4 x, y = {};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = A[16 * I + 4 * lg + r][16 * w + li];
+#pragma unroll
+      for (int J = 0; J < I; ++J)
+        if (J >= w) {
+          const f32x4 m = *reinterpret_cast<const f32x4*>(&A[16 * I + li][16 * J + 4 * lg]) *
+                          *reinterpret_cast<const f32x4*>(&beta[16 * J + 4 * lg]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(-m[r], n[J][r], x, 0, 0, 0);
+        }
+      const f32x4 m = *reinterpret_cast<const f32x4*>(&D[I][li][4 * lg]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(m[r], x[r], y, 0, 0, 0);
+      n[I] = y;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int I = 0; I < 4; ++I)
+    if (I >= w)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) A[16 * I + 4 * lg + r][16 * w + li] = n[I][r];
+  __syncthreads();
+
+  // out in 16-byte pieces, a block of 16 x 32 per wave and turn
+  for (int f = w; f < 6; f += 4) {
+    const int mt = f < 2 ? f : 1 + f / 2, s = f < 2 ? 0 : f & 1;
+    const int i = 16 * mt + li, j = 32 * s + 4 * lg, at = f * 1024 + frag_lane(li, lg);
+    bf16x8 pn[kTerms], pm[kOut];
+    split(join(*reinterpret_cast<const f32x4*>(&A[i][j]),
+               *reinterpret_cast<const f32x4*>(&A[i][j + 16])), pn);
+    split(join(*reinterpret_cast<const f32x4*>(&M[i][j]),
+               *reinterpret_cast<const f32x4*>(&M[i][j + 16])), pm);
+#pragma unroll
+    for (int p = 0; p < kTerms; ++p)
+      *reinterpret_cast<bf16x8*>(a.n + (ch * kTerms + p) * kTriBytes + at) = pn[p];
+#pragma unroll
+    for (int p = 0; p < kOut; ++p)
+      *reinterpret_cast<bf16x8*>(a.m + (ch * kOut + p) * kTriBytes + at) = pm[p];
+  }
+}
+
+// --------------------------------------------------------------- what a forward keeps per chunk
+// Blocks of 16 columns (one wave's) as frags of the transpose: a lane's eight values of a result
+// pair are 16 bytes. For bf16 tensors they are kept in fp16, scaled by a power of two so that the
+// block's largest is in [2^14, 2^15): 2^-12 of it at half the bytes of fp32, where the outputs that
+// come of them are rounded to 2^-9. fp16 and fp32 tensors keep fp32.
+template <class E>
+constexpr int kept_size() { return InputPlanes<E>::n == 1 ? 2 : 4; }
+
+__device__ __forceinline__ float block_scale(float most) {
+  const int e = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^e
+  const int up = 15 - e > 126 ? 126 : 15 - e;
+  return __uint_as_float((unsigned)(up + 127) << 23);
+}
+
+template <class E, int kPairs>
+__device__ __forceinline__ void keep(char* to, float* scale, const f32x4 (&x)[2 * kPairs], int lane) {
+  if constexpr (kept_size<E>() == 2) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * kPairs; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x[i][r]));
+    const float up = block_scale(wave_max(most));
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      reinterpret_cast<f16x8*>(to)[i * 64 + lane] =
+          __builtin_convertvector(join(x[2 * i], x[2 * i + 1]) * up, f16x8);
+    if (lane == 0) *scale = 1.0f / up;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      reinterpret_cast<f32x8*>(to)[i * 64 + lane] = join(x[2 * i], x[2 * i + 1]);
+  }
+}
+
+// ---------------------------------------------------------------------------- walks over chunks
+// What the walks read of a chunk, in LDS: K and Q as frags, N and M, and per step exp(G),
+// exp(G_end - G) and beta.
+template <class E, int KD, int kTerms, int kOut>
+struct ChunkLds {
+  static constexpr int NI = InputPlanes<E>::n;
+  static constexpr int kBlocks = KD / 32;
+  static constexpr int kPlane = kChunk * KD * 2;
+  static constexpr int k = 0, q = k + NI * kPlane, n = q + NI * kPlane, m = n + kTerms * kTriBytes,
+                       gam = m + kOut * kTriBytes, end = gam + 4 * kChunk, beta = end + 4 * kChunk,
+                       size = beta + 4 * kChunk;
+};
+
+template <class E, int KD, int kTerms, int kOut>
+__device__ __forceinline__ void stage(char* lds, const DeltaArgs& a, int64_t ch, int64_t b, int64_t hk,
+                                      int64_t t0) {
+  using C = ChunkLds<E, KD, kTerms, kOut>;
+  constexpr int NI = C::NI, G8 = KD / 8;
+  const int tid = threadIdx.x, nt = blockDim.x, rows = rows_left(a.L, t0);
+  const Rsrc rk = head_rsrc(a.k, b, hk, t0, rows, a.Dk, E::kSize);
+  const Rsrc rq = head_rsrc(a.q, b, hk, t0, rows, a.Dk, E::kSize);
+  for (int i = tid; i < kChunk * G8; i += nt) {
+    const int t = i / G8, d = (i % G8) * 8;
+    bf16x8 pk[NI], pq[NI];
+    load8<E>(rk, d < a.Dk ? (t * (int)a.k.t + d) * E::kSize : kNoOffset, pk);
+    load8<E>(rq, d < a.Dk ? (t * (int)a.q.t + d) * E::kSize : kNoOffset, pq);
+    const int u0 = frag_unit<C::kBlocks>(t, d), u1 = frag_unit<C::kBlocks>(t, d + 4);
+#pragma unroll
+    for (int p = 0; p < NI; ++p) {
+      const u32x4 vk = __builtin_bit_cast(u32x4, pk[p]), vq = __builtin_bit_cast(u32x4, pq[p]);
+      *reinterpret_cast<u32x2*>(lds + C::k + p * C::kPlane + u0) = u32x2{vk[0], vk[1]};
+      *reinterpret_cast<u32x2*>(lds + C::k + p * C::kPlane + u1) = u32x2{vk[2], vk[3]};
+      *reinterpret_cast<u32x2*>(lds + C::q + p * C::kPlane + u0) = u32x2{vq[0], vq[1]};
+      *reinterpret_cast<u32x2*>(lds + C::q + p * C::kPlane + u1) = u32x2{vq[2], vq[3]};
+    }
+  }
+  for (int i = tid; i < kTerms * kTriBytes / 16; i += nt)
+    reinterpret_cast<u32x4*>(lds + C::n)[i] =
+        reinterpret_cast<const u32x4*>(a.n + ch * kTerms * kTriBytes)[i];
+  for (int i = tid; i < kOut * kTriBytes / 16; i += nt)
+    reinterpret_cast<u32x4*>(lds + C::m)[i] =
+        reinterpret_cast<const u32x4*>(a.m + ch * kOut * kTriBytes)[i];
+  if (tid < kChunk) {
+    const f32x4* gb = reinterpret_cast<const f32x4*>(a.gb) + ch * kChunk;
+    const f32x4 x = gb[tid], l = gb[kChunk - 1];
+    reinterpret_cast<float*>(lds + C::gam)[tid] = expf(x[0]) * (1.0f + x[1]);
+    reinterpret_cast<float*>(lds + C::end)[tid] = expf((l[0] - x[0]) + (l[1] - x[1]));
+    reinterpret_cast<float*>(lds + C::beta)[tid] = x[2];
+  }
+}
+
+template <int NP>
+__device__ __forceinline__ void rows_of(const char* block, int plane_bytes, int lane,
+                                        bf16x8 (&p)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) p[i] = frag_rows(block + i * plane_bytes, lane);
+}
+
+template <int NP>
+__device__ __forceinline__ void cols_of(const char* lo, const char* hi, int plane_bytes, int ct,
+                                        int lane, bf16x8 (&p)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) p[i] = frag_cols(lo + i * plane_bytes, hi + i * plane_bytes, ct, lane);
+}
+
+// Forward. A wave owns 16 columns of the state (all key rows, in registers, lane by column), so the
+// chain of a chunk, K S -> E -> S, passes from product to product without leaving the wave: a
+// workgroup's waves share the left operands in LDS and meet only to exchange those.
+template <class E, int KD, int kTerms, bool kSave>
+__global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a) {
+  constexpr int kOut = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
+  using C = ChunkLds<E, KD, kTerms, kOut>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // the workgroups of one head, which read the same K, Q, N and M, on one XCD
+  const int64_t id = blockIdx.x, bh = id / (8 * a.vblocks) * 8 + id % 8;
+  const int vb = (int)(id / 8 % a.vblocks);
+  if (bh >= a.heads_total) return;
+  const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / a.R;
+  const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
+  const int tile = vb * (blockDim.x >> 6) + w, col = tile * 16 + li;
+  const bool in = col < a.Dv;
+  const int tiles = (a.Dv + 15) >> 4;
+  const int vst = (int)a.v.t * E::kSize, ost = a.H * a.Dv * E::kSize;
+
+  f32x4 S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * t + 4 * lg + r;
+      S[t][r] = a.state && in && row < a.Dk ? a.state[(bh * a.Dk + row) * a.Dv + col] : 0.0f;
+    }
+
+  for (int64_t c = 0; c < a.chunks; ++c) {
+    const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
+    const int rows = rows_left(a.L, t0);
+    const Rsrc rv = head_rsrc(a.v, b, h, t0, rows, a.Dv, E::kSize);
+    f32x4 x[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x[mt][r] = load1<E>(rv, in ? (16 * mt + 4 * lg + r) * vst + col * E::kSize : kNoOffset);
+    __syncthreads();
+    stage<E, KD, kTerms, kOut>(lds, a, ch, b, hk, t0);
+    __syncthreads();
+    if (kSave && tile < tiles)
+      keep<E, KT / 2>(a.s + (ch * tiles + tile) * KD * 16 * kept_size<E>(), a.ss + ch * tiles + tile,
+                      S, lane);
+
+    f32x4 ks[4] = {}, o[4] = {};
+#pragma unroll
+    for (int s = 0; s < KD / 32; ++s) {
+      bf16x8 sp[kTerms];
+      split(join(S[2 * s], S[2 * s + 1]), sp);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        bf16x8 f[NI];
+        const int at = (mt * C::kBlocks + s) * 1024;
+        rows_of(lds + C::k + at, C::kPlane, lane, f);
+        ks[mt] = mma<kTerms>(f, sp, ks[mt]);
+        rows_of(lds + C::q + at, C::kPlane, lane, f);
+        o[mt] = mma<kOut>(f, sp, o[mt]);
+      }
+    }
+    // x: V -> R -> E; u: beta R -> U
+    f32x4 gam[4], u[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      gam[mt] = *reinterpret_cast<const f32x4*>(lds + C::gam + (16 * mt + 4 * lg) * 4);
+      x[mt] -= gam[mt] * ks[mt];
+      u[mt] = *reinterpret_cast<const f32x4*>(lds + C::beta + (16 * mt + 4 * lg) * 4) * x[mt];
+    }
+    bf16x8 up[2][kTerms];
+    split(join(u[0], u[1]), up[0]);
+    split(join(u[2], u[3]), up[1]);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 y = {};
+#pragma unroll
+      for (int s = 0; s <= mt / 2; ++s) {
+        bf16x8 f[kTerms];
+        rows_of(lds + C::n + tri_block(mt, s) * 1024, kTriBytes, lane, f);
+        y = mma<kTerms>(f, up[s], y);
+      }
+      x[mt] -= y;
+      u[mt] = *reinterpret_cast<const f32x4*>(lds + C::beta + (16 * mt + 4 * lg) * 4) * x[mt];
+    }
+    if (kSave && tile < tiles)
+      keep<E, 2>(a.e + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.es + ch * tiles + tile, x,
+                 lane);
+    {
+      bf16x8 uo[2][kOut];
+      split(join(u[0], u[1]), uo[0]);
+      split(join(u[2], u[3]), uo[1]);
+      const Rsrc ro = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
+                               ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        f32x4 y = o[mt] * (gam[mt] * a.scale);
+#pragma unroll
+        for (int s = 0; s <= mt / 2; ++s) {
+          bf16x8 f[kOut];
+          rows_of(lds + C::m + tri_block(mt, s) * 1024, kTriBytes, lane, f);
+          y = mma<kOut>(f, uo[s], y);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store1<E>(ro, in ? (16 * mt + 4 * lg + r) * ost + col * E::kSize : kNoOffset, y[r]);
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+      u[mt] *= *reinterpret_cast<const f32x4*>(lds + C::end + (16 * mt + 4 * lg) * 4);
+    split(join(u[0], u[1]), up[0]);
+    split(join(u[2], u[3]), up[1]);
+    const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      S[t] *= last;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 f[NI];
+        const char* at = lds + C::k + (2 * s * C::kBlocks + t / 2) * 1024;
+        cols_of(at, at + C::kBlocks * 1024, C::kPlane, t, lane, f);
+        S[t] = mma<kTerms>(f, up[s], S[t]);
+      }
+    }
+  }
+  if (a.state && in)
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * t + 4 * lg + r;
+        if (row < a.Dk) a.state[(bh * a.Dk + row) * a.Dv + col] = S[t][r];
+      }
+}
+
+// ------------------------------------------------------------------------------ token by token
+// The recurrence itself in fp32, for one to a few tokens: a wave holds 32 columns of a state (lane:
+// four columns, KD / 8 consecutive rows), and one reduction over the eight row groups gives k^T S',
+// q^T S' and q.k; then out = scale (q^T S' + (q.k) u). Bound by reading and writing the state.
+template <class E, int KD>
+__global__ __launch_bounds__(256) void delta_steps(DeltaArgs a) {
+  constexpr int NR = KD / 8, NI = InputPlanes<E>::n;
+  const int lane = threadIdx.x & 63, cl = lane & 7, rg = lane >> 3;
+  const int64_t wid = (int64_t)blockIdx.x * 4 + wave_index(), bh = wid / a.vblocks;
+  if (bh >= a.heads_total) return;
+  const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / a.R;
+  const int col = (int)(wid - bh * a.vblocks) * 32 + cl * 4;
+  const bool in = col < a.Dv;
+  int64_t slot = b;
+  if (a.slots) slot = a.slots[b];
+  const bool live = slot >= 0 && slot < a.nslots;
+  float* st = a.state + ((slot * a.H + h) * a.Dk + rg * NR) * a.Dv + col;
+
+  f32x4 S[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    S[i] = live && in && rg * NR + i < a.Dk ? *reinterpret_cast<const f32x4*>(st + i * a.Dv)
+                                            : f32x4{};
+  for (int64_t t = 0; t < a.L; ++t) {
+    const Rsrc rk = head_rsrc(a.k, b, hk, t, 1, a.Dk, E::kSize);
+    const Rsrc rq = head_rsrc(a.q, b, hk, t, 1, a.Dk, E::kSize);
+    const Rsrc rv = head_rsrc(a.v, b, h, t, 1, a.Dv, E::kSize);
+    float k[NR], q[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i += 8) {
+      bf16x8 p[NI];
+      const int d = rg * NR + i;
+      load8<E>(rk, d < a.Dk ? d * E::kSize : kNoOffset, p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        k[i + j] = (float)p[0][j];
+#pragma unroll
+        for (int n = 1; n < NI; ++n) k[i + j] += (float)p[n][j];
+      }
+      load8<E>(rq, d < a.Dk ? d * E::kSize : kNoOffset, p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        q[i + j] = (float)p[0][j];
+#pragma unroll
+        for (int n = 1; n < NI; ++n) q[i + j] += (float)p[n][j];
+      }
+    }
+    const float alpha = expf(element<E>(a.g, b, t, h)), beta = element<E>(a.beta, b, t, h);
+    f32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = load1<E>(rv, in ? (col + j) * E::kSize : kNoOffset);
+
+    f32x4 ks = {}, qs = {};
+    float qk = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      S[i] *= alpha;
+      ks += k[i] * S[i];
+      qs += q[i] * S[i];
+      qk = fmaf(q[i], k[i], qk);
+    }
+#pragma unroll
+    for (int m = 8; m < 64; m <<= 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ks[j] += __shfl_xor(ks[j], m);
+        qs[j] += __shfl_xor(qs[j], m);
+      }
+      qk += __shfl_xor(qk, m);
+    }
+    const f32x4 u = beta * (v - ks);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) S[i] += k[i] * u;
+    const f32x4 o = live ? a.scale * (qs + qk * u) : f32x4{};
+    if (rg == 0 && in) {
+      const Rsrc ro = row_rsrc(a.out, ((b * a.L + t) * a.H + h) * a.Dv, E::kSize, a.Dv * E::kSize);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store1<E>(ro, (col + j) * E::kSize, o[j]);
+    }
+  }
+  if (live && in)
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+      if (rg * NR + i < a.Dk) *reinterpret_cast<f32x4*>(st + i * a.Dv) = S[i];
+}
+
+// ------------------------------------------------------------------------------------ host side
+size_t size_of(int dtype) { return dtype == FPSCAN_DTYPE_F32 ? 4 : 2; }
+
+bool known(int dtype) {
+  return dtype == FPSCAN_DTYPE_F32 || dtype == FPSCAN_DTYPE_F16 || dtype == FPSCAN_DTYPE_BF16;
+}
+
+bool empty(const fpscan_delta* p) { return p->batch == 0 || p->seqlen == 0 || p->heads == 0; }
+
+// A tensor's strides: whole 16-byte vectors, and a chunk's rows within a buffer range.
+int check_heads(const fpscan_heads& x, int64_t batch, int64_t seqlen, int64_t heads, int64_t dim,
+                int size, bool vectors) {
+  if (x.data == nullptr) return FPSCAN_ERR_NULL;
+  if (x.stride_b < 0 || x.stride_t < 0 || x.stride_h < 0) return FPSCAN_ERR_SHAPE;
+  const int64_t most = (int64_t)1 << 47;
+  if (x.stride_t > ((int64_t)1 << 31) / kChunk / size - dim || x.stride_h > most / size ||
+      x.stride_b > most / size)
+    return FPSCAN_ERR_SHAPE;
+  // 128-bit: the product of a count and a stride may pass 64
+  const __int128 span = (__int128)(batch - 1) * x.stride_b + (__int128)(seqlen - 1) * x.stride_t +
+                        (__int128)(heads - 1) * x.stride_h + dim;
+  if (span * size >= ((__int128)1 << 48)) return FPSCAN_ERR_SHAPE;
+  if (vectors) {
+    const int64_t v = 16 / size;
+    if ((uintptr_t)x.data % 16 || x.stride_b % v || x.stride_t % v || x.stride_h % v)
+      return FPSCAN_ERR_ALIGN;
+  } else if ((uintptr_t)x.data % size) {
+    return FPSCAN_ERR_ALIGN;
+  }
+  return FPSCAN_OK;
+}
+
+// Sizes alone: what the workspaces depend on.
+int check_sizes(const fpscan_delta* p) {
+  if (p == nullptr) return FPSCAN_ERR_NULL;
+  if (!known(p->dtype)) return FPSCAN_ERR_DTYPE;
+  if (p->batch < 0 || p->seqlen < 0 || p->heads < 0 || p->key_heads < 0) return FPSCAN_ERR_SHAPE;
+  if (p->key_dim < 8 || p->key_dim > FPSCAN_DELTA_MAX_KEY_DIM || p->key_dim % 8 || p->value_dim < 8 ||
+      p->value_dim > FPSCAN_DELTA_MAX_VALUE_DIM || p->value_dim % 8)
+    return FPSCAN_ERR_SHAPE;
+  if (empty(p)) return FPSCAN_OK;
+  if (p->key_heads < 1 || p->heads % p->key_heads) return FPSCAN_ERR_SHAPE;
+  const int64_t most = (int64_t)1 << 31;
+  if (p->heads >= 1 << 16 || p->batch >= most || p->seqlen >= most * kChunk) return FPSCAN_ERR_SHAPE;
+  // rows of a chunk of the contiguous outputs within a buffer range
+  if (p->heads * p->value_dim * (int64_t)size_of(p->dtype) > ((int64_t)1 << 31) / kChunk - 4096)
+    return FPSCAN_ERR_SHAPE;
+  const __int128 groups = (__int128)p->batch * p->heads * ((p->seqlen + kChunk - 1) / kChunk);
+  if (groups >= most || (__int128)p->batch * p->heads * ((p->value_dim + 31) / 32) >= most)
+    return FPSCAN_ERR_SHAPE;
+  const __int128 span = (__int128)p->batch * p->seqlen * p->heads * p->value_dim;
+  if (span * size_of(p->dtype) >= ((__int128)1 << 48)) return FPSCAN_ERR_SHAPE;
+  return FPSCAN_OK;
+}
+
+int check_inputs(const fpscan_delta* p) {
+  int st = check_sizes(p);
+  if (st != FPSCAN_OK || empty(p)) return st;
+  const int size = (int)size_of(p->dtype);
+  if ((st = check_heads(p->q, p->batch, p->seqlen, p->key_heads, p->key_dim, size, true)) ||
+      (st = check_heads(p->k, p->batch, p->seqlen, p->key_heads, p->key_dim, size, true)) ||
+      (st = check_heads(p->v, p->batch, p->seqlen, p->heads, p->value_dim, size, true)) ||
+      (st = check_heads(p->log_decay, p->batch, p->seqlen, p->heads, 1, size, false)) ||
+      (st = check_heads(p->beta, p->batch, p->seqlen, p->heads, 1, size, false)))
+    return st;
+  return FPSCAN_OK;
+}
+
+Heads heads_of(const fpscan_heads& x) { return Heads{x.data, x.stride_b, x.stride_t, x.stride_h}; }
+
+DeltaArgs args_of(const fpscan_delta* p) {
+  DeltaArgs a = {};
+  a.q = heads_of(p->q);
+  a.k = heads_of(p->k);
+  a.v = heads_of(p->v);
+  a.g = heads_of(p->log_decay);
+  a.beta = heads_of(p->beta);
+  a.L = p->seqlen;
+  a.chunks = (p->seqlen + kChunk - 1) / kChunk;
+  a.heads_total = p->batch * p->heads;
+  a.H = (int)p->heads;
+  a.R = (int)(p->heads / p->key_heads);
+  a.Dk = (int)p->key_dim;
+  a.Dv = (int)p->value_dim;
+  a.scale = p->scale;
+  return a;
+}
+
+int padded_key_dim(const fpscan_delta* p) { return p->key_dim <= 64 ? 64 : 128; }
+
+// Terms by type and use, as the kernels take them.
+int terms_out(const fpscan_delta* p) { return p->dtype == FPSCAN_DTYPE_F32 ? 3 : 2; }
+int terms_state(const fpscan_delta* p, bool keeps_state) { return keeps_state ? 3 : terms_out(p); }
+
+// Parts of a workspace, each a whole number of 256 bytes.
+struct Carver {
+  char* base;
+  size_t used = 0;
+  char* take(size_t bytes) {
+    char* at = base ? base + used : nullptr;
+    used += (bytes + 255) & ~(size_t)255;
+    return at;
+  }
+};
+
+// G, beta, N and M of every chunk.
+void carve_prep(Carver& w, DeltaArgs& a, const fpscan_delta* p, bool keeps_state) {
+  const size_t n = (size_t)(a.heads_total * a.chunks);
+  a.gb = w.take(n * kChunk * 16);
+  a.n = w.take(n * terms_state(p, keeps_state) * kTriBytes);
+  a.m = w.take(n * terms_out(p) * kTriBytes);
+}
+
+// What a forward keeps for the gradients; the states and E, of 16 value columns a block.
+void carve_saved(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
+  const size_t blocks = (size_t)(a.heads_total * a.chunks) * ((a.Dv + 15) / 16);
+  const size_t each = p->dtype == FPSCAN_DTYPE_BF16 ? 2 : 4;
+  carve_prep(w, a, p, false);
+  a.s = w.take(blocks * padded_key_dim(p) * 16 * each);
+  a.e = w.take(blocks * kChunk * 16 * each);
+  a.ss = reinterpret_cast<float*>(w.take(blocks * 4));
+  a.es = reinterpret_cast<float*>(w.take(blocks * 4));
+}
+
+template <class F>
+int by_type(int dtype, int kd, F&& f) {
+  if (kd == 64) {
+    if (dtype == FPSCAN_DTYPE_F32) return f(F32{}, std::integral_constant<int, 64>{});
+    if (dtype == FPSCAN_DTYPE_F16) return f(F16{}, std::integral_constant<int, 64>{});
+    return f(BF16{}, std::integral_constant<int, 64>{});
+  }
+  if (dtype == FPSCAN_DTYPE_F32) return f(F32{}, std::integral_constant<int, 128>{});
+  if (dtype == FPSCAN_DTYPE_F16) return f(F16{}, std::integral_constant<int, 128>{});
+  return f(BF16{}, std::integral_constant<int, 128>{});
+}
+
+int launched() { return hipGetLastError() == hipSuccess ? FPSCAN_OK : FPSCAN_ERR_LAUNCH; }
+
+// LDS above 64 KiB has to be allowed per kernel (and device).
+template <class K>
+int allow_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess
+             ? FPSCAN_OK : FPSCAN_ERR_LAUNCH;
+}
+
+// Waves of a walk's workgroup, each with 16 value columns, and the grid: groups of eight heads.
+int walk_waves(const DeltaArgs& a) { return a.Dv >= 64 ? 4 : (a.Dv + 15) / 16; }
+unsigned walk_grid(DeltaArgs& a, int waves) {
+  a.vblocks = (a.Dv + 16 * waves - 1) / (16 * waves);
+  return (unsigned)((a.heads_total + 7) / 8 * 8 * a.vblocks);
+}
+
+template <class E, int KD, int kTerms, bool kSave>
+int walk_forward(DeltaArgs& a, hipStream_t stream) {
+  constexpr int kOut = out_terms<E>(), lds = ChunkLds<E, KD, kTerms, kOut>::size;
+  delta_prep<E, KD, kTerms, kOut><<<(unsigned)(a.heads_total * a.chunks), 256, 0, stream>>>(a);
+  int st = launched();
+  if (st != FPSCAN_OK) return st;
+  if ((st = allow_lds(delta_chunks<E, KD, kTerms, kSave>, lds)) != FPSCAN_OK) return st;
+  const int waves = walk_waves(a);
+  const unsigned grid = walk_grid(a, waves);
+  delta_chunks<E, KD, kTerms, kSave><<<grid, 64 * waves, lds, stream>>>(a);
+  return launched();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fpscan_delta_workspace_bytes(const fpscan_delta* p, int op) {
+  if (check_sizes(p) != FPSCAN_OK || empty(p)) return 0;
+  DeltaArgs a = args_of(p);
+  Carver w{nullptr};
+  if (op == FPSCAN_OP_FWD)
+    carve_prep(w, a, p, true);
+  else if (op == FPSCAN_OP_SAVED)
+    carve_saved(w, a, p);
+  return w.used;
+}
+
+int fpscan_delta_fwd(const fpscan_delta* p, void* out, float* state, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int st = check_inputs(p);
+  if (st != FPSCAN_OK || empty(p)) return st;
+  if (out == nullptr || workspace == nullptr) return FPSCAN_ERR_NULL;
+  if ((uintptr_t)out % 16 || (uintptr_t)state % 16 || (uintptr_t)workspace % 16) return FPSCAN_ERR_ALIGN;
+  if (workspace_bytes < fpscan_delta_workspace_bytes(p, FPSCAN_OP_FWD)) return FPSCAN_ERR_WORKSPACE;
+  DeltaArgs a = args_of(p);
+  a.out = static_cast<char*>(out);
+  a.state = state;
+  Carver w{static_cast<char*>(workspace)};
+  carve_prep(w, a, p, state != nullptr);
+  return by_type(p->dtype, padded_key_dim(p), [&](auto e, auto kd) {
+    using E = decltype(e);
+    return state ? walk_forward<E, kd.value, 3, false>(a, (hipStream_t)stream)
+                 : walk_forward<E, kd.value, out_terms<E>(), false>(a, (hipStream_t)stream);
+  });
+}
+
+int fpscan_delta_fwd_saved(const fpscan_delta* p, void* out, void* saved, size_t saved_bytes,
+                           void* stream) {
+  int st = check_inputs(p);
+  if (st != FPSCAN_OK || empty(p)) return st;
+  if (out == nullptr || saved == nullptr) return FPSCAN_ERR_NULL;
+  if ((uintptr_t)out % 16 || (uintptr_t)saved % 16) return FPSCAN_ERR_ALIGN;
+  if (saved_bytes < fpscan_delta_workspace_bytes(p, FPSCAN_OP_SAVED)) return FPSCAN_ERR_WORKSPACE;
+  DeltaArgs a = args_of(p);
+  a.out = static_cast<char*>(out);
+  Carver w{static_cast<char*>(saved)};
+  carve_saved(w, a, p);
+  return by_type(p->dtype, padded_key_dim(p), [&](auto e, auto kd) {
+    using E = decltype(e);
+    return walk_forward<E, kd.value, out_terms<E>(), true>(a, (hipStream_t)stream);
+  });
+}
+
+int fpscan_delta_step(const fpscan_delta* p, void* out, float* state, const int32_t* slots,
+                      int64_t nslots, void* stream) {
+  int st = check_inputs(p);
+  if (st != FPSCAN_OK || empty(p)) return st;
+  if (out == nullptr || state == nullptr) return FPSCAN_ERR_NULL;
+  if ((uintptr_t)out % 16 || (uintptr_t)state % 16 || (uintptr_t)slots % 4) return FPSCAN_ERR_ALIGN;
+  if (nslots < 0 || (slots == nullptr && nslots < p->batch)) return FPSCAN_ERR_SHAPE;
+  DeltaArgs a = args_of(p);
+  a.out = static_cast<char*>(out);
+  a.state = state;
+  a.slots = slots;
+  a.nslots = nslots;
+  a.vblocks = (a.Dv + 31) / 32;
+  const unsigned grid = (unsigned)((a.heads_total * a.vblocks + 3) / 4);
+  return by_type(p->dtype, padded_key_dim(p), [&](auto e, auto kd) {
+    delta_steps<decltype(e), kd.value><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    return launched();
+  });
+}
+
+}  // extern "C"

@@ -308,3 +308,57 @@ def set_tiling(mode: int = 0) -> None:
     segments; dimwise's row kernel), 2 tiled (persistent grid with look-back) whenever the
     shape allows."""
     _load_extension().set_tiling(int(mode))
+
+
+# ---------------------------------------------------------------------------------------
+# The gated delta rule: the recurrence with a matrix state per head. No reference counterpart.
+# ---------------------------------------------------------------------------------------
+def gated_delta_forward(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    log_decay: torch.Tensor,
+    beta: torch.Tensor,
+    scale: Optional[float] = None,
+    state: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """out[t] = scale * q[t]^T S[t] with, per sequence and head, S' = exp(log_decay[t]) S[t-1] and
+    S[t] = S' + k[t] (beta[t] (v[t] - k[t]^T S'))^T.
+
+    q, k: (batch, seqlen, key_heads, key_dim), each key head shared by heads / key_heads value
+    heads; v: (batch, seqlen, heads, value_dim); log_decay, beta: (batch, seqlen, heads); all of
+    one dtype (fp32/fp16/bf16). Views are taken as they are if the last axis of q, k and v is
+    contiguous and their strides are whole 16-byte vectors. Any seqlen; key_dim a multiple of 8 up
+    to 128, value_dim a multiple of 8. ``scale`` defaults to key_dim ** -0.5.
+
+    ``state``: float32 (batch, heads, key_dim, value_dim), the states before the first step,
+    replaced by those after the last (a prompt, or the next part of one); without it they start
+    from zero and are not kept. log_decay = -inf starts a state anew (a document's first token in
+    a packed sequence); log_decay = beta = 0 leaves it as it is (padding). Runs without autograd;
+    see ``gated_delta``."""
+    ext = _load_extension()
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    return ext.gated_delta_forward(q, k, v, log_decay, beta, out, scale, state)
+
+
+def gated_delta_step(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    log_decay: torch.Tensor,
+    beta: torch.Tensor,
+    state: torch.Tensor,
+    scale: Optional[float] = None,
+    slots: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``gated_delta_forward`` token by token, for decoding: seqlen of one to a few tokens. With
+    ``slots`` (int32, one per sequence), ``state`` is a pool (slots, heads, key_dim, value_dim) and
+    sequence b works on state[slots[b]]; an entry outside the pool (-1) marks a sequence that is
+    not there: its outputs are zero and no state changes. No two entries may be the same slot."""
+    ext = _load_extension()
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    return ext.gated_delta_step(q, k, v, log_decay, beta, state, out, scale, slots)

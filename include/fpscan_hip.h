@@ -298,6 +298,65 @@ size_t fpscan_dimwise_workspace_bytes(int64_t batch, int64_t dim, int64_t seqlen
  * without the chunk (dimwise_scan_final.cu:133, :189). */
 int fpscan_dimwise_groups(int64_t seqlen);
 
+/* ------------------------------------------------------------------------------------------
+ * The gated delta rule: a linear recurrence with a (key_dim, value_dim) state S per sequence and
+ * head,
+ *   S' = exp(log_decay[t]) S[t-1];  u = beta[t] (v[t] - k[t]^T S');  S[t] = S' + k[t] u^T
+ *   out[t] = scale q[t]^T S[t].
+ * q, k: (batch, seqlen, key_heads, key_dim), each key head shared by heads / key_heads consecutive
+ * value heads; v, out: (batch, seqlen, heads, value_dim); log_decay, beta: (batch, seqlen, heads).
+ * All of one element type; states are fp32. Any seqlen; key_dim a multiple of 8 up to 128,
+ * value_dim a multiple of 8 up to 4096. A log_decay of -inf starts the state anew, exactly (a new
+ * document in a packed sequence); log_decay = beta = 0 leaves it as it is. Values beyond fp32's
+ * range or NaN in one step reach the outputs of its 64-step chunk and of all later ones of its
+ * head. No reference counterpart (the reference's states are one number per channel). */
+#define FPSCAN_DELTA_MAX_KEY_DIM 128
+#define FPSCAN_DELTA_MAX_VALUE_DIM 4096
+
+/* A (batch, seqlen, heads, dim) tensor whose last axis is contiguous, strides in elements (of q, k
+ * and v whole 16-byte vectors; log_decay and beta have no last axis and any strides). 64 rows
+ * (stride_t) span less than 2 GiB. */
+typedef struct fpscan_heads {
+  const void* data;
+  int64_t stride_b, stride_t, stride_h;
+} fpscan_heads;
+
+typedef struct fpscan_delta {
+  int64_t batch, seqlen, key_heads, heads, key_dim, value_dim;
+  int dtype;
+  float scale;
+  fpscan_heads q, k, v, log_decay, beta;
+} fpscan_delta;
+
+/* Operation code of fpscan_delta_workspace_bytes for fpscan_delta_fwd_saved's `saved`. */
+#define FPSCAN_OP_SAVED 2
+
+/* Device memory in bytes (16-byte aligned, not used by another call in flight) of a call with these
+ * sizes: FPSCAN_OP_FWD of fpscan_delta_fwd, FPSCAN_OP_SAVED of fpscan_delta_fwd_saved's `saved`,
+ * FPSCAN_OP_BWD of fpscan_delta_bwd. Reads no pointer or stride of `problem`. 0: sizes that the
+ * calls refuse, or nothing to do. */
+size_t fpscan_delta_workspace_bytes(const fpscan_delta* problem, int op);
+
+/* The rule over whole sequences, in chunks of 64 steps on the matrix units. `out`: contiguous,
+ * written in full. `state`: NULL (from zero, not kept), or (batch, heads, key_dim, value_dim)
+ * contiguous, the states before the first step, replaced by those after the last. Products are of
+ * bf16 planes: outputs come of operands held to 2^-17 (half types) or 2^-25 (fp32), states to
+ * 2^-25. Outputs must not overlap inputs. */
+int fpscan_delta_fwd(const fpscan_delta* problem, void* out, float* state, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The forward of a training step, from states of zero: the same outputs as fpscan_delta_fwd without
+ * a state, and in `saved` what fpscan_delta_bwd reads. */
+int fpscan_delta_fwd_saved(const fpscan_delta* problem, void* out, void* saved, size_t saved_bytes,
+                           void* stream);
+
+/* The rule token by token in fp32, for one to a few tokens a sequence (decoding). Sequence b's state
+ * is state[slots[b]] of `nslots` states (heads, key_dim, value_dim), or state[b] where slots is NULL,
+ * and is replaced. A slot outside 0 .. nslots - 1 marks a sequence that is not there: its outputs are
+ * zero and no state changes. Two sequences must not name the same slot. */
+int fpscan_delta_step(const fpscan_delta* problem, void* out, float* state, const int32_t* slots,
+                      int64_t nslots, void* stream);
+
 /* Static description of a status code (never NULL). The reference's equivalent is the
  * TORCH_CHECK message text (full_scan.h:7-9). */
 const char* fpscan_strerror(int status);
