@@ -10,7 +10,8 @@ kernels), and ``lookback_overruns`` / ``check_lookback`` (the tiled paths' count
 waits that gave up, whose outputs are NaN).
 """
 from .ops import (PScan, PScanChannelLast, PScanSoftplus, check_lookback, dimwise_forward,
-                  dimwise_groups, gated_delta_forward, gated_delta_step, lookback_overruns, pscan, pscan_channel_last, pscan_softplus,
+                  dimwise_groups, gated_delta, gated_delta_forward, gated_delta_step,
+                  lookback_overruns, pscan, pscan_channel_last, pscan_softplus,
                   scan_backward,
                   scan_backward_channel_last, scan_backward_softplus, scan_forward,
                   scan_forward_channel_last, scan_forward_softplus)
@@ -18,6 +19,6 @@ from .ops import (PScan, PScanChannelLast, PScanSoftplus, check_lookback, dimwis
 __all__ = ["pscan", "scan_forward", "scan_backward", "PScan", "pscan_channel_last",
            "scan_forward_channel_last", "scan_backward_channel_last", "PScanChannelLast",
            "dimwise_forward", "dimwise_groups", "pscan_softplus", "scan_forward_softplus",
-           "scan_backward_softplus", "PScanSoftplus", "gated_delta_forward", "gated_delta_step",
+           "scan_backward_softplus", "PScanSoftplus", "gated_delta", "gated_delta_forward", "gated_delta_step",
            "lookback_overruns", "check_lookback"]
 __version__ = "0.2.0"

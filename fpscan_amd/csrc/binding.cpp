@@ -553,6 +553,8 @@ void check_vectors(const at::Tensor& t, const char* name) {
   TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data) % 16 | x.stride_b % vec | x.stride_t % vec |
                x.stride_h % vec) == 0, name, ": data and strides must be whole 16-byte vectors (",
               vec, " elements)");
+  TORCH_CHECK(t.size(1) <= 1 || x.stride_t >= t.size(3), name, ": steps must not overlap (seqlen "
+              "stride ", x.stride_t, " below dim ", t.size(3), ")");
 }
 
 // Bytes from a tensor's first element to the end of its last, through its strides.
@@ -651,6 +653,73 @@ at::Tensor gated_delta_forward(const at::Tensor& q, const at::Tensor& k, const a
   return out;
 }
 
+// grad_out as the kernels take it: its own strides where they are whole vectors and its steps apart
+// (a gradient of a sum is one value for all), else a copy.
+at::Tensor readable(const at::Tensor& t) {
+  const int64_t vec = 16 / (int64_t)t.element_size();
+  bool ok = (t.size(3) <= 1 || t.stride(3) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d < 3; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) % vec == 0);
+  ok = ok && (t.size(1) <= 1 || t.stride(1) >= t.size(3));
+  return ok ? t : t.contiguous();
+}
+
+// The gated delta rule as an autograd function in C++ (see PScanFunction). What the backward needs of
+// the forward is one buffer beside the inputs: N and M, and the state and the errors E of every
+// chunk.
+struct GatedDeltaFunction : public torch::autograd::Function<GatedDeltaFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                            const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
+                            const at::Tensor& beta, const c10::optional<double>& scale) {
+    const fpscan_delta p = delta_problem(q, k, v, log_decay, beta, scale);
+    at::Tensor out = at::empty(v.sizes(), v.options());
+    at::Tensor saved = at::empty({0}, v.options().dtype(at::kByte));
+    if (v.numel() > 0) {
+      c10::hip::HIPGuardMasqueradingAsCUDA guard(v.device());
+      void* stream = launch_stream(v);
+      const size_t bytes = fpscan_delta_workspace_bytes(&p, FPSCAN_OP_SAVED);
+      saved = at::empty({(int64_t)bytes}, v.options().dtype(at::kByte));
+      check_status(fpscan_delta_fwd_saved(&p, out.data_ptr(), saved.data_ptr(), bytes, stream));
+    }
+    ctx->save_for_backward({q, k, v, log_decay, beta, saved});
+    ctx->saved_data["scale"] = (double)p.scale;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const at::Tensor &q = t[0], &k = t[1], &v = t[2], &saved = t[5];
+    const fpscan_delta p = delta_problem(q, k, v, t[3], t[4], ctx->saved_data["scale"].toDouble());
+    at::Tensor g[5];
+    for (int i = 0; i < 5; ++i) g[i] = at::empty(t[i].sizes(), t[i].options());
+    if (v.numel() > 0) {
+      const at::Tensor grad_out = readable(grads[0]);
+      check_heads(grad_out, v, "grad_out", 4);
+      TORCH_CHECK(grad_out.sizes() == v.sizes(), "grad_out must have the shape of v ", v.sizes(),
+                  ", got ", grad_out.sizes());
+      c10::hip::HIPGuardMasqueradingAsCUDA guard(v.device());
+      void* stream = launch_stream(v);
+      const fpscan_heads go = heads_of(grad_out);
+      const size_t bytes = fpscan_delta_workspace_bytes(&p, FPSCAN_OP_BWD);
+      at::Tensor ws = workspace(bytes, v);
+      check_status(fpscan_delta_bwd(&p, &go, saved.data_ptr(), (size_t)saved.numel(), g[0].data_ptr(),
+                                    g[1].data_ptr(), g[2].data_ptr(), g[3].data_ptr(),
+                                    g[4].data_ptr(), ws.data_ptr(), bytes, stream));
+    }
+    return {g[0], g[1], g[2], g[3], g[4], at::Tensor()};
+  }
+};
+
+at::Tensor gated_delta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                       const at::Tensor& log_decay, const at::Tensor& beta,
+                       const c10::optional<double>& scale) {
+  if (!backward_follows({q, k, v, log_decay, beta})) {
+    check_heads(v, v, "v", 4);
+    return gated_delta_forward(q, k, v, log_decay, beta, at::empty(v.sizes(), v.options()), scale,
+                               c10::nullopt);
+  }
+  return GatedDeltaFunction::apply(q, k, v, log_decay, beta, scale);
+}
+
 at::Tensor gated_delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const at::Tensor& log_decay, const at::Tensor& beta,
                             const at::Tensor& state, const at::Tensor& out,
@@ -742,6 +811,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "d loss / d rate partial per row", pybind11::arg("z"), pybind11::arg("rate"),
         pybind11::arg("out"), pybind11::arg("grad_out"), pybind11::arg("grad_z"),
         pybind11::arg("grad_tokens"), pybind11::arg("grad_rate_rows"));
+  m.def("gated_delta", &gated_delta, "differentiable gated delta rule from states of zero",
+        pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"),
+        pybind11::arg("beta"), pybind11::arg("scale"));
   m.def("gated_delta_forward", &gated_delta_forward,
         "the gated delta rule over whole sequences, written into out; state is updated in place",
         pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"),

@@ -26,6 +26,7 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -43,6 +44,15 @@ __device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[kPlanes]) {
   for (int i = 0; i < kPlanes; ++i) {
     p[i] = __builtin_convertvector(x, bf16x8);
     if (i + 1 < kPlanes) x -= __builtin_convertvector(p[i], f32x8);
+  }
+}
+
+template <int kPlanes>
+__device__ __forceinline__ void split(f32x4 x, bf16x4 (&p)[kPlanes]) {
+#pragma unroll
+  for (int i = 0; i < kPlanes; ++i) {
+    p[i] = __builtin_convertvector(x, bf16x4);
+    if (i + 1 < kPlanes) x -= __builtin_convertvector(p[i], f32x4);
   }
 }
 
@@ -115,6 +125,24 @@ __device__ __forceinline__ void load8(Rsrc r, uint32_t off, bf16x8 (&p)[InputPla
   }
 }
 
+// Four consecutive elements at each of two byte offsets, as one operand.
+template <class E>
+__device__ __forceinline__ void load4x2(Rsrc r, uint32_t o0, uint32_t o1,
+                                        bf16x8 (&p)[InputPlanes<E>::n]) {
+  if constexpr (E::kSize == 2) {
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o0, 0, 0));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o1, 0, 0));
+    const u32x4 v = __builtin_shufflevector(a, b, 0, 1, 2, 3);
+    if constexpr (InputPlanes<E>::n == 1)
+      p[0] = __builtin_bit_cast(bf16x8, v);
+    else
+      split(__builtin_convertvector(__builtin_bit_cast(f16x8, v), f32x8), p);
+  } else {
+    split(join(__builtin_bit_cast(f32x4, bld16<0>(r, o0)),
+               __builtin_bit_cast(f32x4, bld16<0>(r, o1))), p);
+  }
+}
+
 template <class E>
 __device__ __forceinline__ float load1(Rsrc r, uint32_t off) {
   if constexpr (E::kSize == 4)
@@ -145,6 +173,13 @@ __device__ __forceinline__ float wave_max(float x) {
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+// The sum over the 16 lanes of a lane group.
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) x += __shfl_xor(x, m);
   return x;
 }
 

@@ -266,29 +266,37 @@ struct ChunkLds {
                        size = beta + 4 * kChunk;
 };
 
-template <class E, int KD, int kTerms, int kOut>
-__device__ __forceinline__ void stage(char* lds, const DeltaArgs& a, int64_t ch, int64_t b, int64_t hk,
-                                      int64_t t0) {
-  using C = ChunkLds<E, KD, kTerms, kOut>;
-  constexpr int NI = C::NI, G8 = KD / 8;
-  const int tid = threadIdx.x, nt = blockDim.x, rows = rows_left(a.L, t0);
+// K and Q of a chunk as frags, plane after plane.
+template <class E, int KD>
+__device__ __forceinline__ void stage_keys(char* k, char* q, const DeltaArgs& a, int64_t b, int64_t hk,
+                                           int64_t t0) {
+  constexpr int NI = InputPlanes<E>::n, G8 = KD / 8, kBlocks = KD / 32, kPlane = kChunk * KD * 2;
+  const int rows = rows_left(a.L, t0);
   const Rsrc rk = head_rsrc(a.k, b, hk, t0, rows, a.Dk, E::kSize);
   const Rsrc rq = head_rsrc(a.q, b, hk, t0, rows, a.Dk, E::kSize);
-  for (int i = tid; i < kChunk * G8; i += nt) {
+  for (int i = threadIdx.x; i < kChunk * G8; i += blockDim.x) {
     const int t = i / G8, d = (i % G8) * 8;
     bf16x8 pk[NI], pq[NI];
     load8<E>(rk, d < a.Dk ? (t * (int)a.k.t + d) * E::kSize : kNoOffset, pk);
     load8<E>(rq, d < a.Dk ? (t * (int)a.q.t + d) * E::kSize : kNoOffset, pq);
-    const int u0 = frag_unit<C::kBlocks>(t, d), u1 = frag_unit<C::kBlocks>(t, d + 4);
+    const int u0 = frag_unit<kBlocks>(t, d), u1 = frag_unit<kBlocks>(t, d + 4);
 #pragma unroll
     for (int p = 0; p < NI; ++p) {
       const u32x4 vk = __builtin_bit_cast(u32x4, pk[p]), vq = __builtin_bit_cast(u32x4, pq[p]);
-      *reinterpret_cast<u32x2*>(lds + C::k + p * C::kPlane + u0) = u32x2{vk[0], vk[1]};
-      *reinterpret_cast<u32x2*>(lds + C::k + p * C::kPlane + u1) = u32x2{vk[2], vk[3]};
-      *reinterpret_cast<u32x2*>(lds + C::q + p * C::kPlane + u0) = u32x2{vq[0], vq[1]};
-      *reinterpret_cast<u32x2*>(lds + C::q + p * C::kPlane + u1) = u32x2{vq[2], vq[3]};
+      *reinterpret_cast<u32x2*>(k + p * kPlane + u0) = u32x2{vk[0], vk[1]};
+      *reinterpret_cast<u32x2*>(k + p * kPlane + u1) = u32x2{vk[2], vk[3]};
+      *reinterpret_cast<u32x2*>(q + p * kPlane + u0) = u32x2{vq[0], vq[1]};
+      *reinterpret_cast<u32x2*>(q + p * kPlane + u1) = u32x2{vq[2], vq[3]};
     }
   }
+}
+
+template <class E, int KD, int kTerms, int kOut>
+__device__ __forceinline__ void stage(char* lds, const DeltaArgs& a, int64_t ch, int64_t b, int64_t hk,
+                                      int64_t t0) {
+  using C = ChunkLds<E, KD, kTerms, kOut>;
+  const int tid = threadIdx.x, nt = blockDim.x;
+  stage_keys<E, KD>(lds + C::k, lds + C::q, a, b, hk, t0);
   for (int i = tid; i < kTerms * kTriBytes / 16; i += nt)
     reinterpret_cast<u32x4*>(lds + C::n)[i] =
         reinterpret_cast<const u32x4*>(a.n + ch * kTerms * kTriBytes)[i];
@@ -452,6 +460,407 @@ __global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a) {
       }
 }
 
+// Backward walk, the same way: a wave owns 16 columns of dS' and gives dV, and for the gradients of q
+// and k the dS' and Y of every chunk.
+template <class E, int KD>
+__global__ __launch_bounds__(256) void delta_chunks_bwd(DeltaArgs a) {
+  constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
+  using C = ChunkLds<E, KD, kT, kT>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int64_t id = blockIdx.x, bh = id / (8 * a.vblocks) * 8 + id % 8;
+  const int vb = (int)(id / 8 % a.vblocks);
+  if (bh >= a.heads_total) return;
+  const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / a.R;
+  const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
+  const int tile = vb * (blockDim.x >> 6) + w, col = tile * 16 + li;
+  const bool in = col < a.Dv;
+  const int tiles = (a.Dv + 15) >> 4;
+  const int gst = (int)a.go.t * E::kSize, ost = a.H * a.Dv * E::kSize;
+
+  f32x4 dS[KT] = {};
+  for (int64_t c = a.chunks - 1; c >= 0; --c) {
+    const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
+    const int rows = rows_left(a.L, t0);
+    const Rsrc rg = head_rsrc(a.go, b, h, t0, rows, a.Dv, E::kSize);
+    f32x4 x[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x[mt][r] = load1<E>(rg, in ? (16 * mt + 4 * lg + r) * gst + col * E::kSize : kNoOffset);
+    __syncthreads();
+    stage<E, KD, kT, kT>(lds, a, ch, b, hk, t0);
+    __syncthreads();
+    if (tile < tiles)
+      keep<E, KT / 2>(a.ds + (ch * tiles + tile) * KD * 16 * kept_size<E>(), a.dss + ch * tiles + tile,
+                      dS, lane);
+
+    f32x4 u[4] = {}, beta[4];
+#pragma unroll
+    for (int s = 0; s < KD / 32; ++s) {
+      bf16x8 sp[kT];
+      split(join(dS[2 * s], dS[2 * s + 1]), sp);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        bf16x8 f[NI];
+        rows_of(lds + C::k + (mt * C::kBlocks + s) * 1024, C::kPlane, lane, f);
+        u[mt] = mma<kT>(f, sp, u[mt]);
+      }
+    }
+    {
+      bf16x8 xp[2][NI];
+      split(join(x[0], x[1]), xp[0]);
+      split(join(x[2], x[3]), xp[1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        u[mt] *= *reinterpret_cast<const f32x4*>(lds + C::end + (16 * mt + 4 * lg) * 4);
+        beta[mt] = *reinterpret_cast<const f32x4*>(lds + C::beta + (16 * mt + 4 * lg) * 4);
+#pragma unroll
+        for (int s = mt / 2; s < 2; ++s) {
+          bf16x8 f[kT];
+          cols_of(lds + C::m + tri_block(2 * s, mt / 2) * 1024,
+                  lds + C::m + tri_block(2 * s + 1, mt / 2) * 1024, kTriBytes, mt, lane, f);
+          u[mt] = mma<kT>(f, xp[s], u[mt]);
+        }
+      }
+    }
+    bf16x8 up[2][kT];
+    split(join(beta[0] * u[0], beta[1] * u[1]), up[0]);
+    split(join(beta[2] * u[2], beta[3] * u[3]), up[1]);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 y = {};
+#pragma unroll
+      for (int s = mt / 2; s < 2; ++s) {
+        bf16x8 f[kT];
+        cols_of(lds + C::n + tri_block(2 * s, mt / 2) * 1024,
+                lds + C::n + tri_block(2 * s + 1, mt / 2) * 1024, kTriBytes, mt, lane, f);
+        y = mma<kT>(f, up[s], y);
+      }
+      u[mt] -= y;
+    }
+    if (tile < tiles)
+      keep<E, 2>(a.y + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.ys + ch * tiles + tile, u,
+                 lane);
+    const Rsrc ro = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
+                             ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      u[mt] *= beta[mt];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        store1<E>(ro, in ? (16 * mt + 4 * lg + r) * ost + col * E::kSize : kNoOffset, u[mt][r]);
+      const f32x4 gam = *reinterpret_cast<const f32x4*>(lds + C::gam + (16 * mt + 4 * lg) * 4);
+      u[mt] *= -gam;
+      x[mt] *= gam * a.scale;
+    }
+    split(join(u[0], u[1]), up[0]);
+    split(join(u[2], u[3]), up[1]);
+    bf16x8 xp[2][kT];
+    split(join(x[0], x[1]), xp[0]);
+    split(join(x[2], x[3]), xp[1]);
+    const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      dS[t] *= last;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 f[NI];
+        const int at = (2 * s * C::kBlocks + t / 2) * 1024;
+        cols_of(lds + C::k + at, lds + C::k + at + C::kBlocks * 1024, C::kPlane, t, lane, f);
+        dS[t] = mma<kT>(f, up[s], dS[t]);
+        cols_of(lds + C::q + at, lds + C::q + at + C::kBlocks * 1024, C::kPlane, t, lane, f);
+        dS[t] = mma<kT>(f, xp[s], dS[t]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------- gradients of q, k, g, beta
+// One workgroup of four waves per (sequence, key head, chunk), over the value heads that share the
+// key head; wave w makes KD / 4 key columns of dQ and dK. First the sums over the value columns, 32
+// at a time: dO S^T, dV S^T, U dS'^T (for its key columns) and dO U^T, dV U^T (rows 16 w..); then the
+// sums over steps, with P and F by way of LDS.
+template <class E, int KD>
+struct GradLds {
+  static constexpr int NI = InputPlanes<E>::n, kT = out_terms<E>();
+  static constexpr int kState = 32 * KD * 2, kSteps = 32 * kChunk * 2;  // one plane, 32 value columns
+  static constexpr int s = 0, ds = s + kT * kState, u = ds + kT * kState, dv = u + kT * kSteps,
+                       first = dv + kT * kSteps;
+  static constexpr int kKeys = kChunk * KD * 2, kSquare = kChunk * kChunk * 2;
+  static constexpr int k = 0, q = k + NI * kKeys, p = q + NI * kKeys, f = p + kT * kSquare,
+                       second = f + kT * kSquare;
+  static constexpr int rows = first > second ? first : second;  // per step: floats
+  static constexpr int kRow = 4 * kChunk;
+  static constexpr int hi = rows, lo = hi + kRow, beta = lo + kRow, gam = beta + kRow,
+                       end = gam + kRow, dbeta = end + kRow, dg = dbeta + 2 * kRow,
+                       sums = dg + 4 * kRow, size = sums + 64;
+};
+
+// Eight kept values of block `block`, piece `at`.
+template <class E>
+__device__ __forceinline__ f32x8 kept(const char* from, const float* scale, int64_t block, int pieces,
+                                      int at) {
+  if constexpr (kept_size<E>() == 2)
+    return __builtin_convertvector(reinterpret_cast<const f16x8*>(from)[block * pieces + at], f32x8) *
+           scale[block];
+  else
+    return reinterpret_cast<const f32x8*>(from)[block * pieces + at];
+}
+
+// x's planes as one piece of frags.
+template <int NP>
+__device__ __forceinline__ void put(char* to, int plane_bytes, f32x8 x) {
+  bf16x8 p[NP];
+  split(x, p);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(to + i * plane_bytes) = p[i];
+}
+
+// The value at (row, col) of staged keys.
+template <int NI>
+__device__ __forceinline__ float key_at(const char* keys, int unit, int r, int plane_bytes) {
+  float x = 0.0f;
+#pragma unroll
+  for (int p = NI - 1; p >= 0; --p)
+    x += (float)reinterpret_cast<const __bf16*>(keys + p * plane_bytes + unit)[r];
+  return x;
+}
+
+template <class E, int KD, bool kShared>
+__global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
+  using C = GradLds<E, KD>;
+  constexpr int kT = C::kT, NI = C::NI, NT = KD / 64, kBlocks = KD / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
+  const int64_t group = blockIdx.x / a.chunks, c = blockIdx.x - group * a.chunks, t0 = c * kChunk;
+  const int Hk = a.H / a.R;
+  const int64_t b = group / Hk, hk = group - b * Hk;
+  const int rows = rows_left(a.L, t0), tiles = (a.Dv + 15) >> 4;
+  float* const row_hi = reinterpret_cast<float*>(lds + C::hi);
+  float* const row_lo = reinterpret_cast<float*>(lds + C::lo);
+  float* const row_beta = reinterpret_cast<float*>(lds + C::beta);
+  float* const row_gam = reinterpret_cast<float*>(lds + C::gam);
+  float* const row_end = reinterpret_cast<float*>(lds + C::end);
+  float* const part_dbeta = reinterpret_cast<float*>(lds + C::dbeta);  // [2][64]
+  float* const part_dg = reinterpret_cast<float*>(lds + C::dg);        // [4][64]
+  float* const sums = reinterpret_cast<float*>(lds + C::sums);         // [4] <S, dS'>, [4] rest
+  const int gst = (int)a.go.t * E::kSize;
+
+  f32x4 dq[4][NT] = {}, dk[4][NT] = {};  // over the value heads
+  for (int j = 0; j < a.R; ++j) {
+    const int64_t h = hk * a.R + j, bh = b * a.H + h, ch = bh * a.chunks + c;
+    const Rsrc rg = head_rsrc(a.go, b, h, t0, rows, a.Dv, E::kSize);
+    __syncthreads();  // the last head's rows are read
+    if (tid < kChunk) {
+      const f32x4* gb = reinterpret_cast<const f32x4*>(a.gb) + ch * kChunk;
+      const f32x4 x = gb[tid], l = gb[kChunk - 1];
+      row_hi[tid] = x[0];
+      row_lo[tid] = x[1];
+      row_beta[tid] = x[2];
+      row_gam[tid] = expf(x[0]) * (1.0f + x[1]);
+      row_end[tid] = expf((l[0] - x[0]) + (l[1] - x[1]));
+    }
+    f32x4 os[4][NT] = {}, vs[4][NT] = {}, us[4][NT] = {}, ou[4] = {}, vu[4] = {};
+    f32x8 db = {};
+    float sds = 0.0f;
+    for (int vb = 0; vb < (a.Dv + 31) / 32; ++vb) {
+      __syncthreads();  // rows are there, or the block before is read
+      for (int i = tid; i < 2 * kBlocks * 64; i += 256) {
+        const int vt = i / (kBlocks * 64), at = i % (kBlocks * 64), tile = 2 * vb + vt;
+        f32x8 x = {}, y = {};
+        if (tile < tiles) {
+          x = kept<E>(a.s, a.ss, ch * tiles + tile, kBlocks * 64, at);
+          y = kept<E>(a.ds, a.dss, ch * tiles + tile, kBlocks * 64, at);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) sds = fmaf(x[r], y[r], sds);
+        const int to = (i >> 6) * 1024 + frag_lane(i & 15, (i >> 4) & 3);
+        put<kT>(lds + C::s + to, C::kState, x);
+        put<kT>(lds + C::ds + to, C::kState, y);
+      }
+      {
+        const int vt = tid >> 7, s = w & 1, tile = 2 * vb + vt;
+        f32x8 x = {}, y = {};
+        if (tile < tiles) {
+          x = kept<E>(a.e, a.es, ch * tiles + tile, 128, s * 64 + lane);
+          y = kept<E>(a.y, a.ys, ch * tiles + tile, 128, s * 64 + lane);
+        }
+        const f32x8 beta = join(*reinterpret_cast<const f32x4*>(row_beta + 32 * s + 4 * lg),
+                                *reinterpret_cast<const f32x4*>(row_beta + 32 * s + 16 + 4 * lg));
+        db += x * y;
+        const int to = (2 * vt + s) * 1024 + frag_lane(li, lg);
+        put<kT>(lds + C::u + to, C::kSteps, x * beta);
+        put<kT>(lds + C::dv + to, C::kSteps, y * beta);
+      }
+      __syncthreads();
+      bf16x8 sp[NT][kT], dsp[NT][kT], ow[NI], vw[kT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int ct = w * NT + n, at = ct / 2 * 1024;
+        cols_of(lds + C::s + at, lds + C::s + at + kBlocks * 1024, C::kState, ct, lane, sp[n]);
+        cols_of(lds + C::ds + at, lds + C::ds + at + kBlocks * 1024, C::kState, ct, lane, dsp[n]);
+      }
+      const int d0 = 32 * vb + 4 * lg;
+      load4x2<E>(rg, d0 < a.Dv ? (16 * w + li) * gst + d0 * E::kSize : kNoOffset,
+                 d0 + 16 < a.Dv ? (16 * w + li) * gst + (d0 + 16) * E::kSize : kNoOffset, ow);
+      cols_of(lds + C::dv + w / 2 * 1024, lds + C::dv + (2 + w / 2) * 1024, C::kSteps, w, lane, vw);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        bf16x8 op[NI], vp[kT], upl[kT];
+        load4x2<E>(rg, d0 < a.Dv ? (16 * mt + li) * gst + d0 * E::kSize : kNoOffset,
+                   d0 + 16 < a.Dv ? (16 * mt + li) * gst + (d0 + 16) * E::kSize : kNoOffset, op);
+        cols_of(lds + C::dv + mt / 2 * 1024, lds + C::dv + (2 + mt / 2) * 1024, C::kSteps, mt, lane, vp);
+        cols_of(lds + C::u + mt / 2 * 1024, lds + C::u + (2 + mt / 2) * 1024, C::kSteps, mt, lane, upl);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          os[mt][n] = mma<kT>(op, sp[n], os[mt][n]);
+          vs[mt][n] = mma<kT>(vp, sp[n], vs[mt][n]);
+          us[mt][n] = mma<kT>(upl, dsp[n], us[mt][n]);
+        }
+        if (mt <= w) {
+          ou[mt] = mma<kT>(ow, upl, ou[mt]);
+          vu[mt] = mma<kT>(vw, upl, vu[mt]);
+        }
+      }
+    }
+    __syncthreads();
+    stage_keys<E, KD>(lds + C::k, lds + C::q, a, b, hk, t0);
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+      if (nt <= (w | 1)) {
+        f32x4 p, f;
+        const int jj = 16 * nt + li, i0 = 16 * w + 4 * lg;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = i0 + r;
+          const float gam =
+              jj <= i ? expf((row_hi[i] - row_hi[jj]) + (row_lo[i] - row_lo[jj])) : 0.0f;
+          p[r] = jj <= i ? a.scale * (gam * ou[nt][r]) : 0.0f;
+          f[r] = jj < i ? -(gam * vu[nt][r]) : 0.0f;
+        }
+        bf16x4 pp[kT], fp[kT];
+        split(p, pp);
+        split(f, fp);
+        const int to = frag_unit<2>(jj, i0);
+#pragma unroll
+        for (int x = 0; x < kT; ++x) {
+          *reinterpret_cast<bf16x4*>(lds + C::p + x * C::kSquare + to) = pp[x];
+          *reinterpret_cast<bf16x4*>(lds + C::f + x * C::kSquare + to) = fp[x];
+        }
+      }
+    // dbeta: over the 16 value columns of a lane group, then the two tiles
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float x = group_sum(db[r]);
+      if (li == 0) part_dbeta[(tid >> 7) * kChunk + 32 * (w & 1) + (r >> 2) * 16 + 4 * lg + (r & 3)] = x;
+    }
+    __syncthreads();
+    float rest = 0.0f;
+    f32x4 dG[4] = {};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int ct = w * NT + n;
+      bf16x8 kp[2][NI], qp[2][NI];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int at = (2 * s * kBlocks + ct / 2) * 1024;
+        cols_of(lds + C::k + at, lds + C::k + at + kBlocks * 1024, C::kKeys, ct, lane, kp[s]);
+        cols_of(lds + C::q + at, lds + C::q + at + kBlocks * 1024, C::kKeys, ct, lane, qp[s]);
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const f32x4 gam = *reinterpret_cast<const f32x4*>(row_gam + 16 * mt + 4 * lg);
+        const f32x4 write = us[mt][n] * *reinterpret_cast<const f32x4*>(row_end + 16 * mt + 4 * lg);
+        f32x4 x = os[mt][n] * (gam * a.scale), y = write - vs[mt][n] * gam;
+        bf16x8 f[kT];
+#pragma unroll
+        for (int s = 0; s <= mt / 2; ++s) {
+          const int at = (4 * s + mt / 2) * 1024;  // P^T and F^T: rows 32 s.., columns 16 mt..
+          cols_of(lds + C::p + at, lds + C::p + at + 2048, C::kSquare, mt, lane, f);
+          x = mma<kT>(f, kp[s], x);
+          cols_of(lds + C::f + at, lds + C::f + at + 2048, C::kSquare, mt, lane, f);
+          y = mma<kT>(f, kp[s], y);
+        }
+#pragma unroll
+        for (int s = mt / 2; s < 2; ++s) {
+          const int at = (2 * mt + s) * 1024;
+          rows_of(lds + C::p + at, C::kSquare, lane, f);
+          y = mma<kT>(f, qp[s], y);
+          rows_of(lds + C::f + at, C::kSquare, lane, f);
+          y = mma<kT>(f, kp[s], y);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int col = 16 * ct + (li & ~3), unit = frag_unit<kBlocks>(16 * mt + 4 * lg + r, col);
+          const float kv = key_at<NI>(lds + C::k, unit, li & 3, C::kKeys);
+          const float qv = key_at<NI>(lds + C::q, unit, li & 3, C::kKeys);
+          dG[mt][r] += qv * x[r] + kv * y[r];
+          rest = fmaf(kv, write[r], rest);
+        }
+        if constexpr (kShared) {
+          dq[mt][n] += x;
+          dk[mt][n] += y;
+        } else {
+          dq[mt][n] = x;
+          dk[mt][n] = y;
+        }
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = group_sum(dG[mt][r]);
+        if (li == 0) part_dg[w * kChunk + 16 * mt + 4 * lg + r] = x;
+      }
+    const float sum_s = wave_sum(sds), sum_r = wave_sum(rest);
+    if (lane == 0) {
+      sums[w] = sum_s;
+      sums[4 + w] = sum_r;
+    }
+    __syncthreads();
+    if (w == 0) {
+      const float dbeta = part_dbeta[lane] + part_dbeta[kChunk + lane];
+      float x = part_dg[lane] + part_dg[kChunk + lane] + part_dg[2 * kChunk + lane] +
+                part_dg[3 * kChunk + lane] - 2.0f * row_beta[lane] * dbeta;
+      // sums over the steps from this one on
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const float o = __shfl_down(x, d);
+        x += lane + d < 64 ? o : 0.0f;
+      }
+      x += row_gam[kChunk - 1] * (sums[0] + sums[1] + sums[2] + sums[3]) +
+           (sums[4] + sums[5] + sums[6] + sums[7]);
+      if (lane < rows) {
+        // the first step decays a state of zero; a decay of zero passes nothing on
+        if (t0 + lane == 0 || element<E>(a.g, b, t0 + lane, h) < kLeastLog) x = 0.0f;
+        store1<E>(row_rsrc(a.gg, (b * a.L + t0) * a.H + h, E::kSize, (63 * a.H + 1) * E::kSize),
+                  lane * a.H * E::kSize, x);
+        store1<E>(row_rsrc(a.gbeta, (b * a.L + t0) * a.H + h, E::kSize, (63 * a.H + 1) * E::kSize),
+                  lane * a.H * E::kSize, dbeta);
+      }
+    }
+  }
+  const int st = Hk * a.Dk * E::kSize;
+  const int64_t base = ((b * a.L + t0) * Hk + hk) * a.Dk;
+  const int bytes = (rows - 1) * st + a.Dk * E::kSize;
+  const Rsrc oq = row_rsrc(a.gq, base, E::kSize, bytes), ok = row_rsrc(a.gk, base, E::kSize, bytes);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = (w * NT + n) * 16 + li;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t off =
+            col < a.Dk ? (16 * mt + 4 * lg + r) * st + col * E::kSize : kNoOffset;
+        store1<E>(oq, off, dq[mt][n][r]);
+        store1<E>(ok, off, dk[mt][n][r]);
+      }
+  }
+}
+
 // ------------------------------------------------------------------------------ token by token
 // The recurrence itself in fp32, for one to a few tokens: a wave holds 32 columns of a state (lane:
 // four columns, KD / 8 consecutive rows), and one reduction over the eight row groups gives k^T S',
@@ -553,6 +962,8 @@ int check_heads(const fpscan_heads& x, int64_t batch, int64_t seqlen, int64_t he
   if (x.data == nullptr) return FPSCAN_ERR_NULL;
   if (x.stride_b < 0 || x.stride_t < 0 || x.stride_h < 0) return FPSCAN_ERR_SHAPE;
   const int64_t most = (int64_t)1 << 47;
+  // steps apart: the kernels let the range of a chunk's rows end its reads
+  if (seqlen > 1 && x.stride_t < dim) return FPSCAN_ERR_SHAPE;
   if (x.stride_t > ((int64_t)1 << 31) / kChunk / size - dim || x.stride_h > most / size ||
       x.stride_b > most / size)
     return FPSCAN_ERR_SHAPE;
@@ -600,21 +1011,23 @@ int check_inputs(const fpscan_delta* p) {
   if ((st = check_heads(p->q, p->batch, p->seqlen, p->key_heads, p->key_dim, size, true)) ||
       (st = check_heads(p->k, p->batch, p->seqlen, p->key_heads, p->key_dim, size, true)) ||
       (st = check_heads(p->v, p->batch, p->seqlen, p->heads, p->value_dim, size, true)) ||
-      (st = check_heads(p->log_decay, p->batch, p->seqlen, p->heads, 1, size, false)) ||
-      (st = check_heads(p->beta, p->batch, p->seqlen, p->heads, 1, size, false)))
+      (st = check_heads(p->log_decay, p->batch, p->seqlen, p->heads, 0, size, false)) ||
+      (st = check_heads(p->beta, p->batch, p->seqlen, p->heads, 0, size, false)))
     return st;
   return FPSCAN_OK;
 }
 
-Heads heads_of(const fpscan_heads& x) { return Heads{x.data, x.stride_b, x.stride_t, x.stride_h}; }
+Heads heads_of(const fpscan_heads& x, int64_t seqlen, int64_t dim) {
+  return Heads{x.data, x.stride_b, seqlen > 1 ? x.stride_t : dim, x.stride_h};
+}
 
 DeltaArgs args_of(const fpscan_delta* p) {
   DeltaArgs a = {};
-  a.q = heads_of(p->q);
-  a.k = heads_of(p->k);
-  a.v = heads_of(p->v);
-  a.g = heads_of(p->log_decay);
-  a.beta = heads_of(p->beta);
+  a.q = heads_of(p->q, p->seqlen, p->key_dim);
+  a.k = heads_of(p->k, p->seqlen, p->key_dim);
+  a.v = heads_of(p->v, p->seqlen, p->value_dim);
+  a.g = heads_of(p->log_decay, p->seqlen, 1);
+  a.beta = heads_of(p->beta, p->seqlen, 1);
   a.L = p->seqlen;
   a.chunks = (p->seqlen + kChunk - 1) / kChunk;
   a.heads_total = p->batch * p->heads;
@@ -662,6 +1075,16 @@ void carve_saved(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
   a.es = reinterpret_cast<float*>(w.take(blocks * 4));
 }
 
+// What the walk backwards leaves for the gradients of q and k.
+void carve_bwd(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
+  const size_t blocks = (size_t)(a.heads_total * a.chunks) * ((a.Dv + 15) / 16);
+  const size_t each = p->dtype == FPSCAN_DTYPE_BF16 ? 2 : 4;
+  a.ds = w.take(blocks * padded_key_dim(p) * 16 * each);
+  a.y = w.take(blocks * kChunk * 16 * each);
+  a.dss = reinterpret_cast<float*>(w.take(blocks * 4));
+  a.ys = reinterpret_cast<float*>(w.take(blocks * 4));
+}
+
 template <class F>
 int by_type(int dtype, int kd, F&& f) {
   if (kd == 64) {
@@ -704,6 +1127,21 @@ int walk_forward(DeltaArgs& a, hipStream_t stream) {
   return launched();
 }
 
+template <class E, int KD>
+int backward(DeltaArgs& a, hipStream_t stream) {
+  constexpr int kT = out_terms<E>(), lds = ChunkLds<E, KD, kT, kT>::size, glds = GradLds<E, KD>::size;
+  int st = allow_lds(delta_chunks_bwd<E, KD>, lds);
+  if (st != FPSCAN_OK) return st;
+  const int waves = walk_waves(a);
+  const unsigned grid = walk_grid(a, waves);
+  delta_chunks_bwd<E, KD><<<grid, 64 * waves, lds, stream>>>(a);
+  if ((st = launched()) != FPSCAN_OK) return st;
+  const auto kernel = a.R > 1 ? delta_grads<E, KD, true> : delta_grads<E, KD, false>;
+  if ((st = allow_lds(kernel, glds)) != FPSCAN_OK) return st;
+  kernel<<<(unsigned)(a.heads_total / a.R * a.chunks), 256, glds, stream>>>(a);
+  return launched();
+}
+
 }  // namespace
 
 extern "C" {
@@ -716,6 +1154,8 @@ size_t fpscan_delta_workspace_bytes(const fpscan_delta* p, int op) {
     carve_prep(w, a, p, true);
   else if (op == FPSCAN_OP_SAVED)
     carve_saved(w, a, p);
+  else if (op == FPSCAN_OP_BWD)
+    carve_bwd(w, a, p);
   return w.used;
 }
 
@@ -752,6 +1192,40 @@ int fpscan_delta_fwd_saved(const fpscan_delta* p, void* out, void* saved, size_t
   return by_type(p->dtype, padded_key_dim(p), [&](auto e, auto kd) {
     using E = decltype(e);
     return walk_forward<E, kd.value, out_terms<E>(), true>(a, (hipStream_t)stream);
+  });
+}
+
+int fpscan_delta_bwd(const fpscan_delta* p, const fpscan_heads* grad_out, const void* saved,
+                     size_t saved_bytes, void* grad_q, void* grad_k, void* grad_v,
+                     void* grad_log_decay, void* grad_beta, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  int st = check_inputs(p);
+  if (st != FPSCAN_OK || empty(p)) return st;
+  if (!grad_out || !saved || !grad_q || !grad_k || !grad_v || !grad_log_decay || !grad_beta ||
+      !workspace)
+    return FPSCAN_ERR_NULL;
+  const int size = (int)size_of(p->dtype);
+  if ((st = check_heads(*grad_out, p->batch, p->seqlen, p->heads, p->value_dim, size, true)))
+    return st;
+  if (((uintptr_t)saved | (uintptr_t)workspace | (uintptr_t)grad_q | (uintptr_t)grad_k |
+       (uintptr_t)grad_v) % 16 || ((uintptr_t)grad_log_decay | (uintptr_t)grad_beta) % size)
+    return FPSCAN_ERR_ALIGN;
+  if (saved_bytes < fpscan_delta_workspace_bytes(p, FPSCAN_OP_SAVED) ||
+      workspace_bytes < fpscan_delta_workspace_bytes(p, FPSCAN_OP_BWD))
+    return FPSCAN_ERR_WORKSPACE;
+  DeltaArgs a = args_of(p);
+  a.go = heads_of(*grad_out, p->seqlen, p->value_dim);
+  a.out = static_cast<char*>(grad_v);
+  a.gq = static_cast<char*>(grad_q);
+  a.gk = static_cast<char*>(grad_k);
+  a.gg = static_cast<char*>(grad_log_decay);
+  a.gbeta = static_cast<char*>(grad_beta);
+  Carver kept{const_cast<char*>(static_cast<const char*>(saved))};
+  carve_saved(kept, a, p);
+  Carver w{static_cast<char*>(workspace)};
+  carve_bwd(w, a, p);
+  return by_type(p->dtype, padded_key_dim(p), [&](auto e, auto kd) {
+    return backward<decltype(e), kd.value>(a, (hipStream_t)stream);
   });
 }
 

@@ -343,6 +343,22 @@ def gated_delta_forward(
     return ext.gated_delta_forward(q, k, v, log_decay, beta, out, scale, state)
 
 
+def gated_delta(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    log_decay: torch.Tensor,
+    beta: torch.Tensor,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """Differentiable ``gated_delta_forward`` from states of zero: gradients for q, k, v, log_decay
+    and beta, run by the extension's C++ autograd function (see ``pscan``). Where autograd records
+    the call, the forward keeps for the backward, beside its inputs, the state and the errors of
+    every 64-step chunk: 2 (bf16) or 4 bytes for each of (1 + key_dim / 64) value_dim values a step
+    and head, and 24 KiB (36 KiB in fp32) of chunk matrices."""
+    return _load_extension().gated_delta(q, k, v, log_decay, beta, scale)
+
+
 def gated_delta_step(
     q: torch.Tensor,
     k: torch.Tensor,

@@ -314,8 +314,8 @@ int fpscan_dimwise_groups(int64_t seqlen);
 #define FPSCAN_DELTA_MAX_VALUE_DIM 4096
 
 /* A (batch, seqlen, heads, dim) tensor whose last axis is contiguous, strides in elements (of q, k
- * and v whole 16-byte vectors; log_decay and beta have no last axis and any strides). 64 rows
- * (stride_t) span less than 2 GiB. */
+ * and v whole 16-byte vectors, stride_t at least dim; log_decay and beta have no last axis and any
+ * strides). 64 rows (stride_t) span less than 2 GiB. Batch and heads may have strides of 0. */
 typedef struct fpscan_heads {
   const void* data;
   int64_t stride_b, stride_t, stride_h;
@@ -349,6 +349,15 @@ int fpscan_delta_fwd(const fpscan_delta* problem, void* out, float* state, void*
  * a state, and in `saved` what fpscan_delta_bwd reads. */
 int fpscan_delta_fwd_saved(const fpscan_delta* problem, void* out, void* saved, size_t saved_bytes,
                            void* stream);
+
+/* Gradients of fpscan_delta_fwd_saved's call on the same problem, whose `saved` it reads (and does
+ * not change): all five contiguous, in the shapes and the type of q, k, v, log_decay and beta, written
+ * in full; those of q and k are summed over the value heads that share a key head, in a fixed order.
+ * Where exp(log_decay) is 0 in fp32 its gradient is 0. Outputs must not overlap inputs. */
+int fpscan_delta_bwd(const fpscan_delta* problem, const fpscan_heads* grad_out, const void* saved,
+                     size_t saved_bytes, void* grad_q, void* grad_k, void* grad_v,
+                     void* grad_log_decay, void* grad_beta, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 /* The rule token by token in fp32, for one to a few tokens a sequence (decoding). Sequence b's state
  * is state[slots[b]] of `nslots` states (heads, key_dim, value_dim), or state[b] where slots is NULL,
