@@ -11,7 +11,7 @@ waits that gave up, whose outputs are NaN).
 """
 from .ops import (PScan, PScanChannelLast, PScanSoftplus, check_lookback, dimwise_forward,
                   dimwise_groups, gated_delta, gated_delta_forward, gated_delta_step,
-                  lookback_overruns, pscan, pscan_channel_last, pscan_softplus,
+                  group_norm_channel_last, lookback_overruns, pscan, pscan_channel_last, pscan_softplus,
                   scan_backward,
                   scan_backward_channel_last, scan_backward_softplus, scan_forward,
                   scan_forward_channel_last, scan_forward_softplus)
@@ -20,5 +20,6 @@ __all__ = ["pscan", "scan_forward", "scan_backward", "PScan", "pscan_channel_las
            "scan_forward_channel_last", "scan_backward_channel_last", "PScanChannelLast",
            "dimwise_forward", "dimwise_groups", "pscan_softplus", "scan_forward_softplus",
            "scan_backward_softplus", "PScanSoftplus", "gated_delta", "gated_delta_forward", "gated_delta_step",
+           "group_norm_channel_last",
            "lookback_overruns", "check_lookback"]
 __version__ = "0.2.0"

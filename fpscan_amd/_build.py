@@ -54,7 +54,7 @@ def _atomic_out(path):
 
 
 HIP_SOURCES = ("fpscan_scan.hip", "fpscan_scan_cl.hip", "fpscan_dimwise.hip", "fpscan_delta.hip",
-               "fpscan_probe.hip")
+               "fpscan_norm.hip", "fpscan_probe.hip")
 
 
 def build_hip_library() -> str:

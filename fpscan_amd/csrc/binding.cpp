@@ -745,6 +745,113 @@ at::Tensor gated_delta_step(const at::Tensor& q, const at::Tensor& k, const at::
   return out;
 }
 
+// ---- group norm with an activation, channels last: x (batch, seqlen, dim) contiguous, weight and
+// bias fp32 with one value per channel, gate like x
+fpscan_norm norm_problem(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                         const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& gate,
+                         int64_t activation, double eps) {
+  check_input_cl(x, "x");
+  const int64_t D = x.size(2);
+  TORCH_CHECK(groups >= 1 && D % groups == 0, "groups must divide dim (", D, "), got ", groups);
+  TORCH_CHECK(D * (int64_t)x.element_size() <= FPSCAN_NORM_MAX_ROW_BYTES, "x: dim must be at most ",
+              FPSCAN_NORM_MAX_ROW_BYTES / (int64_t)x.element_size(), " for ", x.scalar_type(), ", got ", D);
+  TORCH_CHECK(activation == FPSCAN_ACT_NONE || activation == FPSCAN_ACT_SILU, "unknown activation");
+  TORCH_CHECK(eps >= 0, "eps must not be negative, got ", eps);
+  for (const auto& [t, name] : {std::pair<const c10::optional<at::Tensor>*, const char*>{&weight, "weight"},
+                                {&bias, "bias"}}) {
+    if (!t->has_value()) continue;
+    const at::Tensor& w = **t;
+    TORCH_CHECK(w.device() == x.device(), name, " must be on ", x.device(), ", got ", w.device());
+    TORCH_CHECK(w.scalar_type() == at::kFloat, name, " must be float32, got ", w.scalar_type());
+    TORCH_CHECK(w.is_contiguous() && w.dim() == 1 && w.size(0) == D, name, " must be a contiguous "
+                "float32 tensor with one value per channel (", D, "), got ", w.sizes());
+  }
+  if (gate.has_value()) {
+    check_input_cl(*gate, "gate");
+    check_like(*gate, x, "gate", "x");
+  }
+  return {x.size(0), x.size(1), D, groups, dtype_code(x.scalar_type()), (int)activation, (float)eps};
+}
+
+const float* float_data(const c10::optional<at::Tensor>& t) {
+  return t.has_value() ? t->data_ptr<float>() : nullptr;
+}
+const void* any_data(const c10::optional<at::Tensor>& t) {
+  return t.has_value() ? t->data_ptr() : nullptr;
+}
+
+at::Tensor run_norm(const fpscan_norm& p, const at::Tensor& x, const c10::optional<at::Tensor>& weight,
+                    const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& gate,
+                    float* stats) {
+  at::Tensor out = at::empty_like(x);
+  if (x.numel() == 0) return out;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  void* stream = launch_stream(x);
+  const size_t bytes = fpscan_norm_workspace_bytes(&p, FPSCAN_OP_FWD);
+  at::Tensor ws = workspace(bytes, x);
+  check_status(fpscan_norm_fwd(&p, x.data_ptr(), float_data(weight), float_data(bias), any_data(gate),
+                               out.data_ptr(), stats, bytes ? ws.data_ptr() : nullptr, bytes, stream));
+  return out;
+}
+
+struct GroupNormFunction : public torch::autograd::Function<GroupNormFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, int64_t groups,
+                            const c10::optional<at::Tensor>& weight,
+                            const c10::optional<at::Tensor>& bias,
+                            const c10::optional<at::Tensor>& gate, int64_t activation, double eps) {
+    const fpscan_norm p = norm_problem(x, groups, weight, bias, gate, activation, eps);
+    at::Tensor stats = at::empty({2, p.batch, p.groups}, x.options().dtype(at::kFloat));
+    at::Tensor out = run_norm(p, x, weight, bias, gate, stats.data_ptr<float>());
+    auto or_empty = [](const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); };
+    ctx->save_for_backward({x, or_empty(weight), or_empty(bias), or_empty(gate), stats});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["eps"] = eps;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const at::Tensor& x = t[0];
+    c10::optional<at::Tensor> given[3];
+    for (int i = 0; i < 3; ++i)
+      if (t[i + 1].defined()) given[i] = t[i + 1];
+    const auto& [weight, bias, gate] = given;
+    const fpscan_norm p =
+        norm_problem(x, ctx->saved_data["groups"].toInt(), weight, bias, gate,
+                     ctx->saved_data["activation"].toInt(), ctx->saved_data["eps"].toDouble());
+    const bool empty = x.numel() == 0;  // then the parameters' gradients are sums of nothing
+    auto like = [empty](const c10::optional<at::Tensor>& o) {
+      return !o.has_value() ? at::Tensor() : empty ? at::zeros_like(*o) : at::empty_like(*o);
+    };
+    at::Tensor gx = at::empty_like(x), gw = like(weight), gb = like(bias), gg = like(gate);
+    if (!empty) {
+      const at::Tensor go = grads[0].contiguous();
+      check_like(go, x, "grad_out", "x");
+      c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+      void* stream = launch_stream(x);
+      const size_t bytes = fpscan_norm_workspace_bytes(&p, FPSCAN_OP_BWD);
+      at::Tensor ws = workspace(bytes, x);
+      check_status(fpscan_norm_bwd(&p, x.data_ptr(), float_data(weight), float_data(bias),
+                                   any_data(gate), t[4].data_ptr<float>(), go.data_ptr(), gx.data_ptr(),
+                                   gg.defined() ? gg.data_ptr() : nullptr,
+                                   gw.defined() ? gw.data_ptr<float>() : nullptr,
+                                   gb.defined() ? gb.data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
+                                   stream));
+    }
+    return {gx, at::Tensor(), gw, gb, gg, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor group_norm_cl(const at::Tensor& x, int64_t groups, const c10::optional<at::Tensor>& weight,
+                         const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& gate,
+                         int64_t activation, double eps) {
+  if (!backward_follows({x, weight.value_or(x), bias.value_or(x), gate.value_or(x)}))
+    return run_norm(norm_problem(x, groups, weight, bias, gate, activation, eps), x, weight, bias, gate,
+                    nullptr);
+  return GroupNormFunction::apply(x, groups, weight, bias, gate, activation, eps);
+}
+
 // Look-back waits that gave up on the tensors' device since the library was loaded (waits for
 // the device first).
 uint64_t lookback_overruns(int64_t device) {
@@ -823,6 +930,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("log_decay"),
         pybind11::arg("beta"), pybind11::arg("state"), pybind11::arg("out"), pybind11::arg("scale"),
         pybind11::arg("slots"));
+  m.def("group_norm_cl", &group_norm_cl,
+        "differentiable channel-last group norm with an activation (0 none, 1 silu) or an activated gate",
+        pybind11::arg("x"), pybind11::arg("groups"), pybind11::arg("weight"), pybind11::arg("bias"),
+        pybind11::arg("gate"), pybind11::arg("activation"), pybind11::arg("eps"));
   m.def("dimwise_forward", &dimwise_forward,
         "contraction scan, in place into Bx (HIP, gfx950)", pybind11::arg("Ax"),
         pybind11::arg("Bx"), pybind11::arg("Bh"), pybind11::arg("Wq"), pybind11::arg("Wk"));

@@ -1,0 +1,666 @@
+// Group norm of (batch, seqlen, dim) tensors with an activation, forward and backward:
+//   h = (x - mean) rstd, over each (sequence, group of dim / groups channels);  y = h w + b
+//   out = act(y), or y act(gate) where a gate is given;  act: identity or SiLU, z / (1 + exp(-z)).
+// Backward, with dy the gradient at y:
+//   dx = rstd (w dy - m1 - h m2), m1 and m2 the means of w dy and w dy h over the group;
+//   dw = sum dy h, db = sum dy, dgate = dout y act'(gate).
+//
+// A thread owns 16 bytes of channels and walks rows, so that per-channel values stay in registers
+// and a row is read in order. With seqlen 1 (token by token) a row's statistics are taken while it
+// is in registers: every tensor is read and written once. Otherwise a first pass over chunks of rows
+// takes the sums, a small kernel joins the chunks, and a second pass applies them. All statistics are
+// fp32, all sums in a fixed order. The variance is of differences from a mean: a thread's values from
+// the first of them, which is one of the summed, so that at most log2 of their count is lost of 24
+// bits, then between means (M2 = sum M2_i + n_i (mean_i - mean)^2).
+#include "../../include/fpscan_hip.h"
+#include "delta_common.h"
+
+#include <type_traits>
+
+namespace {
+
+struct NormArgs {
+  const char *x, *gate, *go;
+  const float *weight, *bias;
+  char *out, *gx, *ggate;
+  float *mean, *rstd;   // per (sequence, group)
+  float* part;          // per chunk of rows: forward (mean, M2) per group; backward sum dy, sum dy h
+  float* channels;      // backward, per sequence: sum dy, sum dy h per channel
+  int64_t batch, seqlen, chunk_rows, chunks;
+  int dim, groups, width, vecs, rows, lanes;  // rows: of a workgroup at a time
+  float eps;
+};
+
+template <class E>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (E::kSize == 4)
+    return 1.0f / (1.0f + expf(-z));
+  else  // a few 2^-23, where the outputs are rounded to 2^-9 or 2^-12
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+}
+
+template <class E>
+__device__ __forceinline__ void load_vec(const char* p, float (&f)[E::V]) {
+  E::unpack(*reinterpret_cast<const u32x4*>(p), f);
+}
+
+template <class E>
+__device__ __forceinline__ void store_vec(char* p, const float (&f)[E::V]) {
+  *reinterpret_cast<u32x4*>(p) = E::pack(f);
+}
+
+// A thread's place: row `row` of the workgroup's rows and the 16-byte vector of it that begins with
+// channel `c`; threads past the last row have none.
+struct Place {
+  int row, c;
+  bool in;
+};
+template <class E>
+__device__ __forceinline__ Place place(const NormArgs& a) {
+  const int row = (int)threadIdx.x / a.vecs, vec = (int)threadIdx.x - row * a.vecs;
+  return {row, vec * E::V, row < a.rows};
+}
+
+// Weights and biases of a thread's channels; 1 and 0 where there are none.
+template <int V>
+__device__ __forceinline__ void params(const NormArgs& a, const Place& p, float (&w)[V], float (&b)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = a.weight && p.in ? a.weight[p.c + i] : 1.0f;
+    b[i] = a.bias && p.in ? a.bias[p.c + i] : 0.0f;
+  }
+}
+
+template <class E, bool kAct, bool kGate>
+__device__ __forceinline__ float activate(float y, float gate) {
+  const float z = kGate ? gate : y;
+  const float act = kAct ? z * sigmoid<E>(z) : z;
+  return kGate ? y * act : act;
+}
+
+// The gradient at y, and the gate's.
+template <class E, bool kAct, bool kGate>
+__device__ __forceinline__ float slope(float y, float gate, float go, float& ggate) {
+  const float z = kGate ? gate : y;
+  float act = z, d = 1.0f;
+  if constexpr (kAct) {
+    const float s = sigmoid<E>(z);
+    act = z * s;
+    d = s * fmaf(z, 1.0f - s, 1.0f);
+  }
+  if constexpr (!kGate) return go * d;
+  ggate = go * y * d;
+  return go * act;
+}
+
+// out[row * groups + g] = the sum of buf[row * dim + c] over the channels of group g, for `rows` rows;
+// `per` consecutive threads (a power of two up to the wave) share a sum.
+__device__ __forceinline__ void group_sums(const NormArgs& a, const float* buf, float* out, int rows,
+                                           int per) {
+  const int lane = (int)threadIdx.x & (per - 1);
+  for (int i = (int)threadIdx.x / per; i < rows * a.groups; i += (int)blockDim.x / per) {
+    const int row = i / a.groups, g = i - row * a.groups;
+    const float* const from = buf + row * a.dim + g * a.width;
+    float s = 0.0f;
+    for (int c = lane; c < a.width; c += per) s += from[c];
+    for (int m = per >> 1; m > 0; m >>= 1) s += __shfl_xor(s, m);
+    if (lane == 0) out[i] = s;
+  }
+}
+
+// The sum of a thread's channels over their groups in its row, back per channel. kAligned: groups are
+// `lanes` whole vectors, a power of two up to the wave, and the lanes that hold one add up among
+// themselves. Otherwise through LDS: rows * (dim + groups) floats.
+template <int V, bool kAligned>
+__device__ __forceinline__ void row_sums(const NormArgs& a, const Place& p, float* lds,
+                                         const float (&x)[V], float (&s)[V]) {
+  if constexpr (kAligned) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t += x[i];
+    for (int m = a.lanes >> 1; m > 0; m >>= 1) t += __shfl_xor(t, m);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = t;
+  } else {
+    float* const sums = lds + a.rows * a.dim;
+    if (p.in)
+#pragma unroll
+      for (int i = 0; i < V; ++i) lds[p.row * a.dim + p.c + i] = x[i];
+    __syncthreads();
+    group_sums(a, lds, sums, a.rows, a.lanes);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = p.in ? sums[p.row * a.groups + (p.c + i) / a.width] : 0.0f;
+  }
+}
+
+// A thread's per-channel values, summed over the workgroup's rows: to[c] (through lds, rows * dim).
+template <int V>
+__device__ __forceinline__ void column_sums(const NormArgs& a, const Place& p, float* lds,
+                                            const float (&x)[V], float* to) {
+  __syncthreads();
+  if (p.in)
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[p.row * a.dim + p.c + i] = x[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.dim; c += blockDim.x) {
+    float s = lds[c];
+    for (int r = 1; r < a.rows; ++r) s += lds[r * a.dim + c];
+    to[c] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------ token by token
+template <class E, bool kAct, bool kGate, bool kAligned>
+__global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
+  constexpr int V = E::V;
+  extern __shared__ float lds[];
+  const Place p = place<E>(a);
+  float w[V], b[V];
+  params(a, p, w, b);
+  const float inv = 1.0f / (float)a.width;
+  for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
+    const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
+    const bool in = p.in && r < a.batch;
+    float x[V] = {}, z[V] = {}, s[V], q[V];
+    if (in) load_vec<E>(a.x + at, x);
+    if (kGate && in) load_vec<E>(a.gate + at, z);
+    row_sums<V, kAligned>(a, p, lds, x, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[i] *= inv;
+      if (a.mean && in && (p.c + i) % a.width == 0) a.mean[r * a.groups + (p.c + i) / a.width] = s[i];
+      x[i] -= s[i];
+      q[i] = x[i] * x[i];
+    }
+    row_sums<V, kAligned>(a, p, lds, q, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[i] = 1.0f / sqrtf(fmaf(s[i], inv, a.eps));
+      if (a.mean && in && (p.c + i) % a.width == 0) a.rstd[r * a.groups + (p.c + i) / a.width] = s[i];
+      x[i] = activate<E, kAct, kGate>(fmaf(x[i] * s[i], w[i], b[i]), z[i]);
+    }
+    if (in) store_vec<E>(a.out + at, x);
+  }
+}
+
+template <class E, bool kAct, bool kGate, bool kAligned>
+__global__ __launch_bounds__(1024) void norm_tokens_bwd(NormArgs a) {
+  constexpr int V = E::V;
+  extern __shared__ float lds[];
+  const Place p = place<E>(a);
+  float w[V], b[V], gw[V] = {}, gb[V] = {};
+  params(a, p, w, b);
+  const float inv = 1.0f / (float)a.width;
+  for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
+    const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
+    const bool in = p.in && r < a.batch;
+    float x[V] = {}, z[V] = {}, go[V] = {}, rs[V] = {}, s1[V], s2[V];
+    if (in) {
+      load_vec<E>(a.x + at, x);
+      load_vec<E>(a.go + at, go);
+      if (kGate) load_vec<E>(a.gate + at, z);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (in) {
+        const int64_t g = r * a.groups + (p.c + i) / a.width;
+        rs[i] = a.rstd[g];
+        x[i] = (x[i] - a.mean[g]) * rs[i];
+      }
+      go[i] = slope<E, kAct, kGate>(fmaf(x[i], w[i], b[i]), z[i], go[i], z[i]);
+      gb[i] += go[i];
+      gw[i] = fmaf(go[i], x[i], gw[i]);
+      go[i] *= w[i];
+      s2[i] = go[i] * x[i];
+    }
+    row_sums<V, kAligned>(a, p, lds, go, s1);
+    row_sums<V, kAligned>(a, p, lds, s2, s2);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = rs[i] * (go[i] - s1[i] * inv - x[i] * (s2[i] * inv));
+    if (in) {
+      store_vec<E>(a.gx + at, x);
+      if (kGate) store_vec<E>(a.ggate + at, z);
+    }
+  }
+  float* const part = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+  column_sums(a, p, lds, gb, part);
+  column_sums(a, p, lds, gw, part + a.dim);
+}
+
+// ------------------------------------------------------------------------- over whole sequences
+// The chunk of rows of a workgroup.
+struct Chunk {
+  int64_t b, first, rows;
+};
+__device__ __forceinline__ Chunk chunk_of(const NormArgs& a) {
+  const int64_t b = blockIdx.x / a.chunks, first = (blockIdx.x - b * a.chunks) * a.chunk_rows;
+  const int64_t left = a.seqlen - first;
+  return {b, first, left < a.chunk_rows ? left : a.chunk_rows};
+}
+
+template <class E>
+__global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
+  constexpr int V = E::V;
+  extern __shared__ float lds[];
+  float* const sums = lds + a.rows * a.dim;  // [rows][groups]
+  const Place p = place<E>(a);
+  const Chunk k = chunk_of(a);
+  const char* at = a.x + ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
+  const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
+  float x0[V] = {}, s[V] = {}, q[V] = {}, n = 0.0f;
+  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+    float x[V];
+    load_vec<E>(at, x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (n == 0.0f) x0[i] = x[i];
+      const float d = x[i] - x0[i];
+      s[i] += d;
+      q[i] = fmaf(d, d, q[i]);
+    }
+    n += 1.0f;
+  }
+  const float inv = n > 0.0f ? 1.0f / n : 0.0f;
+  if (p.in)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      q[i] = fmaf(-s[i] * inv, s[i], q[i]);
+      x0[i] = fmaf(s[i], inv, x0[i]);  // the mean of the thread's values of the channel
+      lds[p.row * a.dim + p.c + i] = n * x0[i];
+    }
+  const float all = 1.0f / ((float)k.rows * (float)a.width);
+  float* const part = a.part + (int64_t)blockIdx.x * 2 * a.groups;
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    __syncthreads();
+    group_sums(a, lds, sums, a.rows, a.lanes);
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+      float t = sums[g];
+      for (int r = 1; r < a.rows; ++r) t += sums[r * a.groups + g];
+      part[turn * a.groups + g] = turn == 0 ? t * all : t;
+      if (turn == 0) sums[g] = t * all;
+    }
+    __syncthreads();
+    if (turn == 0 && p.in)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = x0[i] - sums[(p.c + i) / a.width];
+        lds[p.row * a.dim + p.c + i] = fmaf(n * d, d, q[i]);
+      }
+  }
+}
+
+// The chunks of a sequence joined: a wave per (sequence, group), lanes over chunks.
+__global__ __launch_bounds__(256) void norm_join(NormArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (i >= a.batch * a.groups) return;
+  const int64_t b = i / a.groups;
+  const float* const part = a.part + (b * a.chunks * 2) * a.groups + (i - b * a.groups);
+  const float full = (float)a.chunk_rows * (float)a.width;
+  const float last = (float)(a.seqlen - (a.chunks - 1) * a.chunk_rows) * (float)a.width;
+  const float inv = 1.0f / ((float)a.seqlen * (float)a.width);
+  float s = 0.0f;
+  for (int64_t k = lane; k < a.chunks; k += 64)
+    s = fmaf(k + 1 < a.chunks ? full : last, part[k * 2 * a.groups], s);
+  const float mean = wave_sum(s) * inv;
+  float q = 0.0f;
+  for (int64_t k = lane; k < a.chunks; k += 64) {
+    const float d = part[k * 2 * a.groups] - mean;
+    q += fmaf((k + 1 < a.chunks ? full : last) * d, d, part[(k * 2 + 1) * a.groups]);
+  }
+  q = wave_sum(q);
+  if (lane == 0) {
+    a.mean[i] = mean;
+    a.rstd[i] = 1.0f / sqrtf(fmaf(q, inv, a.eps));
+  }
+}
+
+// Means and reciprocal deviations of a thread's channels.
+template <int V>
+__device__ __forceinline__ void statistics(const NormArgs& a, const Place& p, int64_t b, float (&mu)[V],
+                                           float (&rs)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int64_t g = b * a.groups + (p.in ? (p.c + i) / a.width : 0);
+    mu[i] = a.mean[g];
+    rs[i] = a.rstd[g];
+  }
+}
+
+template <class E, bool kAct, bool kGate>
+__global__ __launch_bounds__(1024) void norm_apply(NormArgs a) {
+  constexpr int V = E::V;
+  const Place p = place<E>(a);
+  const Chunk k = chunk_of(a);
+  float w[V], b[V], mu[V], rs[V];
+  params(a, p, w, b);
+  statistics(a, p, k.b, mu, rs);
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] *= rs[i];
+  int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
+  const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
+  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+    float x[V], z[V] = {};
+    load_vec<E>(a.x + at, x);
+    if (kGate) load_vec<E>(a.gate + at, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      x[i] = activate<E, kAct, kGate>(fmaf(x[i] - mu[i], w[i], b[i]), z[i]);
+    store_vec<E>(a.out + at, x);
+  }
+}
+
+// Per chunk and channel: sum dy, sum dy h.
+template <class E, bool kAct, bool kGate>
+__global__ __launch_bounds__(1024) void norm_sums_bwd(NormArgs a) {
+  constexpr int V = E::V;
+  extern __shared__ float lds[];
+  const Place p = place<E>(a);
+  const Chunk k = chunk_of(a);
+  float w[V], b[V], mu[V], rs[V], gw[V] = {}, gb[V] = {};
+  params(a, p, w, b);
+  statistics(a, p, k.b, mu, rs);
+  int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
+  const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
+  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+    float x[V], go[V], z[V] = {};
+    load_vec<E>(a.x + at, x);
+    load_vec<E>(a.go + at, go);
+    if (kGate) load_vec<E>(a.gate + at, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float h = (x[i] - mu[i]) * rs[i];
+      const float dy = slope<E, kAct, kGate>(fmaf(h, w[i], b[i]), z[i], go[i], z[i]);
+      gb[i] += dy;
+      gw[i] = fmaf(dy, h, gw[i]);
+    }
+  }
+  float* const part = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+  column_sums(a, p, lds, gb, part);
+  column_sums(a, p, lds, gw, part + a.dim);
+}
+
+template <class E, bool kAct, bool kGate>
+__global__ __launch_bounds__(1024) void norm_apply_bwd(NormArgs a) {
+  constexpr int V = E::V;
+  extern __shared__ float lds[];
+  const Place p = place<E>(a);
+  const Chunk k = chunk_of(a);
+  // the means over the sequence's groups of w dy and w dy h
+  float* const sums = lds + 2 * a.dim;
+  for (int c = threadIdx.x; c < a.dim; c += blockDim.x) {
+    const float wc = a.weight ? a.weight[c] : 1.0f;
+    lds[c] = wc * a.channels[k.b * 2 * a.dim + c];
+    lds[a.dim + c] = wc * a.channels[(k.b * 2 + 1) * a.dim + c];
+  }
+  __syncthreads();
+  group_sums(a, lds, sums, 2, a.lanes);
+  __syncthreads();
+  float w[V], b[V], mu[V], rs[V], m1[V], m2[V];
+  params(a, p, w, b);
+  statistics(a, p, k.b, mu, rs);
+  const float inv = 1.0f / ((float)a.seqlen * (float)a.width);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int g = p.in ? (p.c + i) / a.width : 0;
+    m1[i] = sums[g] * inv;
+    m2[i] = sums[a.groups + g] * inv;
+  }
+  int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
+  const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
+  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+    float x[V], go[V], z[V] = {};
+    load_vec<E>(a.x + at, x);
+    load_vec<E>(a.go + at, go);
+    if (kGate) load_vec<E>(a.gate + at, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float h = (x[i] - mu[i]) * rs[i];
+      const float dy = slope<E, kAct, kGate>(fmaf(h, w[i], b[i]), z[i], go[i], z[i]);
+      x[i] = rs[i] * (dy * w[i] - m1[i] - h * m2[i]);
+    }
+    store_vec<E>(a.gx + at, x);
+    if (kGate) store_vec<E>(a.ggate + at, z);
+  }
+}
+
+// Sums over the rows of slabs of a (slabs, rows, cols) array: 64 columns a workgroup, 16 threads each.
+// The first `split` columns go to `a`, the others to `b` (either may be null), slab after slab.
+__global__ __launch_bounds__(1024) void norm_columns(const float* from, int64_t rows, int cols, int split,
+                                                     float* to_a, float* to_b, int blocks) {
+  __shared__ float lds[16][64];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int64_t slab = blockIdx.x / blocks;
+  const int c = (int)(blockIdx.x - slab * blocks) * 64 + x;
+  float s = 0.0f;
+  if (c < cols)
+    for (int64_t r = y; r < rows; r += 16) s += from[(slab * rows + r) * cols + c];
+  lds[y][x] = s;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+    for (int i = 1; i < 16; ++i) s += lds[i][x];
+    if (c < split) {
+      if (to_a) to_a[slab * split + c] = s;
+    } else if (to_b) {
+      to_b[slab * (cols - split) + c - split] = s;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ host side
+struct Launch {
+  NormArgs a;
+  int threads, blocks;  // blocks: of the token kernels
+  bool tokens, aligned;
+  size_t lds;
+};
+
+int check(const fpscan_norm* p) {
+  if (p == nullptr) return FPSCAN_ERR_NULL;
+  if (p->dtype != FPSCAN_DTYPE_F32 && p->dtype != FPSCAN_DTYPE_F16 && p->dtype != FPSCAN_DTYPE_BF16)
+    return FPSCAN_ERR_DTYPE;
+  const int size = p->dtype == FPSCAN_DTYPE_F32 ? 4 : 2;
+  if (p->batch < 0 || p->seqlen < 0 || p->dim < 0 || p->groups < 1 || p->dim % p->groups ||
+      p->dim % (16 / size) || p->dim > FPSCAN_NORM_MAX_ROW_BYTES / size || p->activation < 0 ||
+      p->activation > 1)
+    return FPSCAN_ERR_SHAPE;
+  if ((__int128)p->batch * p->seqlen * p->dim * size >= ((__int128)1 << 48)) return FPSCAN_ERR_SHAPE;
+  return FPSCAN_OK;
+}
+
+bool nothing(const fpscan_norm* p) { return p->batch == 0 || p->seqlen == 0 || p->dim == 0; }
+
+int power_of_two_below(int n) {
+  int p = 1;
+  while (2 * p <= n && 2 * p <= 64) p *= 2;
+  return p;
+}
+
+Launch launch_of(const fpscan_norm* p) {
+  Launch l = {};
+  NormArgs& a = l.a;
+  const int size = p->dtype == FPSCAN_DTYPE_F32 ? 4 : 2, V = 16 / size;
+  a.batch = p->batch;
+  a.seqlen = p->seqlen;
+  a.dim = (int)p->dim;
+  a.groups = (int)p->groups;
+  a.width = a.dim / a.groups;
+  a.vecs = a.dim / V;
+  a.eps = p->eps;
+  l.threads = a.vecs <= 256 ? 256 : a.vecs <= 512 ? 512 : 1024;
+  a.rows = l.threads / a.vecs;
+  l.tokens = p->seqlen == 1;
+  const int gv = a.width / V;
+  l.aligned = l.tokens && a.width % V == 0 && gv <= 64 && (gv & (gv - 1)) == 0;
+  a.lanes = l.aligned ? gv : power_of_two_below(l.threads / a.groups < 1 ? 1 : l.threads / a.groups);
+  l.lds = (size_t)a.rows * (a.dim + a.groups) * sizeof(float);
+  if (l.lds < 2 * (size_t)(a.dim + a.groups) * sizeof(float)) l.lds = 2 * (size_t)(a.dim + a.groups) * sizeof(float);
+  // token kernels: a workgroup takes rows in turn, so that the parameters' gradients are summed in
+  // registers first
+  const int64_t turns = (a.batch + a.rows - 1) / a.rows;
+  l.blocks = (int)(turns < 2048 ? turns : 2048);
+  // chunks: some thousand workgroups, 8 to 128 rows a thread
+  int64_t want = 2048 / a.batch;
+  if (want < 1) want = 1;
+  int64_t each = (a.seqlen + want - 1) / want;
+  each = (each + a.rows - 1) / a.rows;
+  each = each < 8 ? 8 : each > 128 ? 128 : each;
+  a.chunk_rows = each * a.rows;
+  a.chunks = (a.seqlen + a.chunk_rows - 1) / a.chunk_rows;
+  return l;
+}
+
+char* take(char*& at, size_t bytes) {
+  char* p = at;
+  at += (bytes + 255) & ~(size_t)255;
+  return p;
+}
+
+size_t carve(char* base, Launch& l, bool backward, bool own_stats) {
+  char* at = base;
+  NormArgs& a = l.a;
+  if (backward) {
+    const int64_t parts = l.tokens ? l.blocks : a.batch * a.chunks;
+    a.part = reinterpret_cast<float*>(take(at, (size_t)parts * 2 * a.dim * 4));
+    if (!l.tokens) a.channels = reinterpret_cast<float*>(take(at, (size_t)a.batch * 2 * a.dim * 4));
+  } else if (!l.tokens) {
+    a.part = reinterpret_cast<float*>(take(at, (size_t)a.batch * a.chunks * 2 * a.groups * 4));
+    if (own_stats) {
+      a.mean = reinterpret_cast<float*>(take(at, (size_t)a.batch * a.groups * 4));
+      a.rstd = reinterpret_cast<float*>(take(at, (size_t)a.batch * a.groups * 4));
+    }
+  }
+  return (size_t)(at - base);
+}
+
+int launched() { return hipGetLastError() == hipSuccess ? FPSCAN_OK : FPSCAN_ERR_LAUNCH; }
+
+template <class F>
+int by_kind(const fpscan_norm* p, bool gate, F&& f) {
+  auto kinds = [&](auto e) {
+    if (p->activation == FPSCAN_ACT_SILU)
+      return gate ? f(e, std::true_type{}, std::true_type{}) : f(e, std::true_type{}, std::false_type{});
+    return gate ? f(e, std::false_type{}, std::true_type{}) : f(e, std::false_type{}, std::false_type{});
+  };
+  if (p->dtype == FPSCAN_DTYPE_F32) return kinds(F32{});
+  if (p->dtype == FPSCAN_DTYPE_F16) return kinds(F16{});
+  return kinds(BF16{});
+}
+
+template <class K>
+int launch(K kernel, const Launch& l, int64_t blocks, hipStream_t stream) {
+  if (l.lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)l.lds) != hipSuccess)
+    return FPSCAN_ERR_LAUNCH;
+  kernel<<<(unsigned)blocks, l.threads, l.lds, stream>>>(l.a);
+  return launched();
+}
+
+int columns(const float* from, int64_t slabs, int64_t rows, int dim, float* to_a, float* to_b, int split,
+            hipStream_t stream) {
+  const int blocks = (2 * dim + 63) / 64;
+  norm_columns<<<(unsigned)(slabs * blocks), 1024, 0, stream>>>(from, rows, 2 * dim, split, to_a, to_b,
+                                                               blocks);
+  return launched();
+}
+
+bool aligned16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % 16) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fpscan_norm_workspace_bytes(const fpscan_norm* p, int op) {
+  if (check(p) != FPSCAN_OK || nothing(p)) return 0;
+  Launch l = launch_of(p);
+  return carve(nullptr, l, op == FPSCAN_OP_BWD, true);
+}
+
+int fpscan_norm_fwd(const fpscan_norm* p, const void* x, const float* weight, const float* bias,
+                    const void* gate, void* out, float* stats, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  int st = check(p);
+  if (st != FPSCAN_OK || nothing(p)) return st;
+  if (!x || !out) return FPSCAN_ERR_NULL;
+  if (!aligned16({x, gate, out, workspace}) || ((uintptr_t)weight | (uintptr_t)bias | (uintptr_t)stats) % 4)
+    return FPSCAN_ERR_ALIGN;
+  Launch l = launch_of(p);
+  if ((!l.tokens && l.a.batch * l.a.chunks >= (int64_t)1 << 31)) return FPSCAN_ERR_SHAPE;
+  if (workspace_bytes < fpscan_norm_workspace_bytes(p, FPSCAN_OP_FWD)) return FPSCAN_ERR_WORKSPACE;
+  carve(static_cast<char*>(workspace), l, false, stats == nullptr);
+  NormArgs& a = l.a;
+  a.x = static_cast<const char*>(x);
+  a.gate = static_cast<const char*>(gate);
+  a.weight = weight;
+  a.bias = bias;
+  a.out = static_cast<char*>(out);
+  if (stats) {
+    a.mean = stats;
+    a.rstd = stats + a.batch * a.groups;
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  return by_kind(p, gate != nullptr, [&](auto e, auto act, auto gated) {
+    using E = decltype(e);
+    if (l.tokens)
+      return l.aligned ? launch(norm_tokens<E, act.value, gated.value, true>, l, l.blocks, s)
+                       : launch(norm_tokens<E, act.value, gated.value, false>, l, l.blocks, s);
+    int st = launch(norm_stats<E>, l, a.batch * a.chunks, s);
+    if (st != FPSCAN_OK) return st;
+    norm_join<<<(unsigned)((a.batch * a.groups + 3) / 4), 256, 0, s>>>(a);
+    if ((st = launched()) != FPSCAN_OK) return st;
+    return launch(norm_apply<E, act.value, gated.value>, l, a.batch * a.chunks, s);
+  });
+}
+
+int fpscan_norm_bwd(const fpscan_norm* p, const void* x, const float* weight, const float* bias,
+                    const void* gate, const float* stats, const void* grad_out, void* grad_x,
+                    void* grad_gate, float* grad_weight, float* grad_bias, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  int st = check(p);
+  if (st != FPSCAN_OK) return st;
+  const hipStream_t s = (hipStream_t)stream;
+  if (nothing(p)) return FPSCAN_OK;
+  if (!x || !stats || !grad_out || !grad_x || !workspace || (gate && !grad_gate)) return FPSCAN_ERR_NULL;
+  if (!aligned16({x, gate, grad_out, grad_x, grad_gate, workspace}) ||
+      ((uintptr_t)weight | (uintptr_t)bias | (uintptr_t)stats | (uintptr_t)grad_weight |
+       (uintptr_t)grad_bias) % 4)
+    return FPSCAN_ERR_ALIGN;
+  Launch l = launch_of(p);
+  if ((!l.tokens && l.a.batch * l.a.chunks >= (int64_t)1 << 31)) return FPSCAN_ERR_SHAPE;
+  if (workspace_bytes < fpscan_norm_workspace_bytes(p, FPSCAN_OP_BWD)) return FPSCAN_ERR_WORKSPACE;
+  carve(static_cast<char*>(workspace), l, true, false);
+  NormArgs& a = l.a;
+  a.x = static_cast<const char*>(x);
+  a.gate = static_cast<const char*>(gate);
+  a.go = static_cast<const char*>(grad_out);
+  a.weight = weight;
+  a.bias = bias;
+  a.gx = static_cast<char*>(grad_x);
+  a.ggate = static_cast<char*>(grad_gate);
+  a.mean = const_cast<float*>(stats);
+  a.rstd = a.mean + a.batch * a.groups;
+  st = by_kind(p, gate != nullptr, [&](auto e, auto act, auto gated) {
+    using E = decltype(e);
+    if (l.tokens)
+      return l.aligned ? launch(norm_tokens_bwd<E, act.value, gated.value, true>, l, l.blocks, s)
+                       : launch(norm_tokens_bwd<E, act.value, gated.value, false>, l, l.blocks, s);
+    int st = launch(norm_sums_bwd<E, act.value, gated.value>, l, a.batch * a.chunks, s);
+    if (st != FPSCAN_OK) return st;
+    if ((st = columns(a.part, a.batch, a.chunks, a.dim, a.channels, nullptr, 2 * a.dim, s)) != FPSCAN_OK)
+      return st;
+    return launch(norm_apply_bwd<E, act.value, gated.value>, l, a.batch * a.chunks, s);
+  });
+  if (st != FPSCAN_OK || (!grad_weight && !grad_bias)) return st;
+  return l.tokens ? columns(a.part, 1, l.blocks, a.dim, grad_bias, grad_weight, a.dim, s)
+                  : columns(a.channels, 1, a.batch, a.dim, grad_bias, grad_weight, a.dim, s);
+}
+
+}  // extern "C"

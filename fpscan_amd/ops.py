@@ -378,3 +378,29 @@ def gated_delta_step(
     if out is None:
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     return ext.gated_delta_step(q, k, v, log_decay, beta, state, out, scale, slots)
+
+
+# ---------------------------------------------------------------------------------------
+# Group norm with an activation, channels last: (batch, seqlen, dim). No reference counterpart.
+# ---------------------------------------------------------------------------------------
+_ACTIVATIONS = {None: 0, "none": 0, "silu": 1}
+
+
+def group_norm_channel_last(
+    x: torch.Tensor,
+    groups: int,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    gate: Optional[torch.Tensor] = None,
+    activation: Optional[str] = "silu",
+    eps: float = 1e-5,
+) -> torch.Tensor:
+    """Differentiable act(y), or y * act(gate) where a gate is given, with y the group norm of x:
+    each sequence's groups of dim / groups channels brought to mean 0 and variance 1 over all its
+    steps, times weight, plus bias. x and gate: (batch, seqlen, dim) contiguous fp32/fp16/bf16, dim a
+    multiple of 16/itemsize; weight, bias: float32, one value per channel. activation: "silu" or
+    None. For a norm token by token (of a layer's heads, say) call it on x.view(-1, 1, dim)."""
+    if activation not in _ACTIVATIONS:
+        raise RuntimeError(f'activation must be "silu" or None, got {activation!r}')
+    return _load_extension().group_norm_cl(x, int(groups), weight, bias, gate,
+                                           _ACTIVATIONS[activation], float(eps))

@@ -366,6 +366,41 @@ int fpscan_delta_bwd(const fpscan_delta* problem, const fpscan_heads* grad_out, 
 int fpscan_delta_step(const fpscan_delta* problem, void* out, float* state, const int32_t* slots,
                       int64_t nslots, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Group norm of (batch, seqlen, dim) contiguous tensors (channels last) with an activation:
+ *   y = (x - mean) / sqrt(variance + eps) weight + bias, mean and variance over each sequence and
+ *       group of dim / groups channels;  out = act(y), or y act(gate) where a gate is given.
+ * With seqlen 1 every token has statistics of its own (the norm of a layer's heads). x, gate and out
+ * share `dtype`; weight and bias: fp32, dim values, or NULL (1 and 0). Statistics and sums are fp32.
+ * dim: a multiple of 16 / itemsize elements, rows up to 16 KiB. No reference counterpart. */
+#define FPSCAN_ACT_NONE 0
+#define FPSCAN_ACT_SILU 1 /* z / (1 + exp(-z)) */
+#define FPSCAN_NORM_MAX_ROW_BYTES 16384
+
+typedef struct fpscan_norm {
+  int64_t batch, seqlen, dim, groups;
+  int dtype, activation;
+  float eps;
+} fpscan_norm;
+
+/* Workspace in bytes (16-byte aligned, not used by another call in flight) of fpscan_norm_fwd
+ * (FPSCAN_OP_FWD) or fpscan_norm_bwd (FPSCAN_OP_BWD); 0: none is needed, or the sizes are refused. */
+size_t fpscan_norm_workspace_bytes(const fpscan_norm* problem, int op);
+
+/* `stats`: NULL, or 2 * batch * groups floats that receive the means and then the reciprocal
+ * deviations, which the backward reads. `out` may be x or gate itself, not overlap them partly. */
+int fpscan_norm_fwd(const fpscan_norm* problem, const void* x, const float* weight, const float* bias,
+                    const void* gate, void* out, float* stats, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* Gradients given the forward's inputs and stats. grad_gate: where a gate is given; grad_weight and
+ * grad_bias (fp32, dim values) may be NULL. Outputs must not overlap inputs or each other. With an
+ * empty batch or seqlen nothing is written. */
+int fpscan_norm_bwd(const fpscan_norm* problem, const void* x, const float* weight, const float* bias,
+                    const void* gate, const float* stats, const void* grad_out, void* grad_x,
+                    void* grad_gate, float* grad_weight, float* grad_bias, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* Static description of a status code (never NULL). The reference's equivalent is the
  * TORCH_CHECK message text (full_scan.h:7-9). */
 const char* fpscan_strerror(int status);
