@@ -162,21 +162,31 @@ __global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
   for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
     const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
     const bool in = p.in && r < a.batch;
-    float x[V] = {}, z[V] = {}, s[V], q[V];
+    float x[V] = {}, z[V] = {}, s[V], q[V], off[V];
     if (in) load_vec<E>(a.x + at, x);
     if (kGate && in) load_vec<E>(a.gate + at, z);
+    row_sums<V, kAligned>(a, p, lds, x, s);
+    float mu[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      mu[i] = s[i] * inv;
+      x[i] -= mu[i];
+      q[i] = x[i] * x[i];
+    }
+    // the sum's own rounding, where means are far from 0, is the mean of the differences
     row_sums<V, kAligned>(a, p, lds, x, s);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       s[i] *= inv;
-      if (a.mean && in && (p.c + i) % a.width == 0) a.mean[r * a.groups + (p.c + i) / a.width] = s[i];
+      mu[i] += s[i];
       x[i] -= s[i];
-      q[i] = x[i] * x[i];
+      off[i] = s[i];
+      if (a.mean && in && (p.c + i) % a.width == 0) a.mean[r * a.groups + (p.c + i) / a.width] = mu[i];
     }
     row_sums<V, kAligned>(a, p, lds, q, s);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      s[i] = 1.0f / sqrtf(fmaf(s[i], inv, a.eps));
+      s[i] = 1.0f / sqrtf(fmaf(-off[i], off[i], s[i] * inv) + a.eps);
       if (a.mean && in && (p.c + i) % a.width == 0) a.rstd[r * a.groups + (p.c + i) / a.width] = s[i];
       x[i] = activate<E, kAct, kGate>(fmaf(x[i] * s[i], w[i], b[i]), z[i]);
     }
@@ -262,11 +272,18 @@ __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
     n += 1.0f;
   }
   const float inv = n > 0.0f ? 1.0f / n : 0.0f;
+  // means are taken from the group's first value, so that sums of means far from 0 lose nothing
+  float* const base = sums + a.rows * a.groups;
+  if (p.in && p.row == 0)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if ((p.c + i) % a.width == 0) base[(p.c + i) / a.width] = x0[i];
+  __syncthreads();
   if (p.in)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       q[i] = fmaf(-s[i] * inv, s[i], q[i]);
-      x0[i] = fmaf(s[i], inv, x0[i]);  // the mean of the thread's values of the channel
+      x0[i] = fmaf(s[i], inv, x0[i] - base[(p.c + i) / a.width]);  // of the thread's values
       lds[p.row * a.dim + p.c + i] = n * x0[i];
     }
   const float all = 1.0f / ((float)k.rows * (float)a.width);
@@ -279,7 +296,7 @@ __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
     for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
       float t = sums[g];
       for (int r = 1; r < a.rows; ++r) t += sums[r * a.groups + g];
-      part[turn * a.groups + g] = turn == 0 ? t * all : t;
+      part[turn * a.groups + g] = turn == 0 ? fmaf(t, all, base[g]) : t;
       if (turn == 0) sums[g] = t * all;
     }
     __syncthreads();
@@ -302,10 +319,11 @@ __global__ __launch_bounds__(256) void norm_join(NormArgs a) {
   const float full = (float)a.chunk_rows * (float)a.width;
   const float last = (float)(a.seqlen - (a.chunks - 1) * a.chunk_rows) * (float)a.width;
   const float inv = 1.0f / ((float)a.seqlen * (float)a.width);
+  const float base = part[0];  // as in norm_stats
   float s = 0.0f;
   for (int64_t k = lane; k < a.chunks; k += 64)
-    s = fmaf(k + 1 < a.chunks ? full : last, part[k * 2 * a.groups], s);
-  const float mean = wave_sum(s) * inv;
+    s = fmaf(k + 1 < a.chunks ? full : last, part[k * 2 * a.groups] - base, s);
+  const float mean = fmaf(wave_sum(s), inv, base);
   float q = 0.0f;
   for (int64_t k = lane; k < a.chunks; k += 64) {
     const float d = part[k * 2 * a.groups] - mean;
@@ -496,8 +514,9 @@ Launch launch_of(const fpscan_norm* p) {
   const int gv = a.width / V;
   l.aligned = l.tokens && a.width % V == 0 && gv <= 64 && (gv & (gv - 1)) == 0;
   a.lanes = l.aligned ? gv : power_of_two_below(l.threads / a.groups < 1 ? 1 : l.threads / a.groups);
-  l.lds = (size_t)a.rows * (a.dim + a.groups) * sizeof(float);
-  if (l.lds < 2 * (size_t)(a.dim + a.groups) * sizeof(float)) l.lds = 2 * (size_t)(a.dim + a.groups) * sizeof(float);
+  // rows of channels and of group sums, and the groups' first values; two such rows at least
+  l.lds = ((size_t)a.rows * (a.dim + a.groups) + a.groups) * sizeof(float);
+  if (a.rows == 1) l.lds = 2 * (size_t)(a.dim + a.groups) * sizeof(float);
   // token kernels: a workgroup takes rows in turn, so that the parameters' gradients are summed in
   // registers first
   const int64_t turns = (a.batch + a.rows - 1) / a.rows;
