@@ -11,11 +11,14 @@
 //
 // Layout ("frags"). The matrix instruction 16x16x32 wants from lane l = 16 g + i the row i of the
 // left operand (column i of the right) at eight values of the summed index; it returns column i,
-// rows 4 g .. 4 g + 3. A sum does not care for the order of its terms, so the eight values of lane
-// group g are taken to be {4 g + r, 16 + 4 g + r}: then two result tiles are, lane by lane, a right
-// operand of the next product, and a chain of products stays in registers. A matrix in memory (LDS
-// or global) is kept as blocks of 16 rows x 32 columns of 1 KiB, 16 bytes a lane, so that a block is
-// read as an operand by one 16-byte load a lane, and its transpose by two transposing 8-byte loads.
+// rows 4 g .. 4 g + 3 of a tile. A sum does not care for the order of its terms, so the eight values
+// of lane group g are those that it holds of a pair of result tiles: such a pair is then, lane by
+// lane, a right operand of the next product, and a chain of products stays in registers. A matrix in
+// memory (LDS or global) is kept as blocks of 16 rows x 32 columns of 1 KiB, 16 bytes a lane, so that
+// a block is read as an operand by one 16-byte load a lane, and its transpose by two transposing
+// 8-byte loads. Which columns a lane group's eight values are is free: for steps, {4 g + r, 16 + 4 g +
+// r}, so that a tile is 16 consecutive steps; for key columns, 8 g + r, so that 16 bytes of a row of
+// keys go to one place (a tile's columns are then those of key_col).
 #ifndef FPSCAN_DELTA_COMMON_H
 #define FPSCAN_DELTA_COMMON_H
 
@@ -72,11 +75,35 @@ __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB
   return c;
 }
 
+// The same for kTiles left operands, tile by tile within a plane product, so that no product waits
+// for the one before it.
+template <int kTerms, int kTiles, int NA, int NB>
+__device__ __forceinline__ void mma_tiles(const bf16x8 (&a)[kTiles][NA], const bf16x8 (&b)[NB],
+                                          f32x4* c) {
+#pragma unroll
+  for (int t = kTerms - 1; t >= 0; --t)
+#pragma unroll
+    for (int i = 0; i <= t; ++i)
+      if (i < NA && t - i < NB)
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+          c[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][i], b[t - i], c[j], 0, 0, 0);
+}
+
+// Keeps the order of loads and products as written: a wave alone on its SIMD has nothing but its own
+// products to cover the latency of its loads, and the compiler would put each load before its use.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // Byte offset of lane (row i of 16, group q of 4 columns) in a 1 KiB block. The bit that moves row
 // i by eight for odd q spreads the transposing loads over all banks: their 16 lanes of a group read
 // four rows at all four q.
 __device__ __forceinline__ int frag_lane(int i, int q) {
   return ((i ^ ((q & 1) << 3)) + 16 * q) * 16;
+}
+
+// The key column of row (or column) x of tile t.
+__device__ __forceinline__ int key_col(int t, int x) {
+  return 32 * (t >> 1) + 8 * (x >> 2) + 4 * (t & 1) + (x & 3);
 }
 
 // Byte offset of the four columns col .. col + 3 (col a multiple of 4) of `row` in a matrix of
@@ -94,8 +121,8 @@ __device__ __forceinline__ bf16x8 frag_rows(const char* block, int lane) {
   return *reinterpret_cast<const bf16x8*>(block + frag_lane(lane & 15, lane >> 4));
 }
 
-// One operand from the transpose: lane (i, g) takes column 16 (ct % 2) + i of blocks `lo` (16 rows)
-// and `hi` (the 16 rows after them), both the ones that hold column 16 ct. LDS only.
+// One operand from the transpose: lane (i, g) takes column i of tile ct, of blocks `lo` (16 rows) and
+// `hi` (the 16 rows after them), both the ones that hold tile ct. LDS only.
 __device__ __forceinline__ bf16x8 frag_cols(const char* lo, const char* hi, int ct, int lane) {
   const int off = frag_lane(4 * (lane >> 4) + ((lane >> 2) & 3), lane & 3) + (ct & 1) * 8;
   typedef __attribute__((address_space(3))) s16x4* ldsp;
@@ -125,30 +152,20 @@ __device__ __forceinline__ void load8(Rsrc r, uint32_t off, bf16x8 (&p)[InputPla
   }
 }
 
-// Four consecutive elements at each of two byte offsets, as one operand.
+// One element as it is, and its value: a load that is used much later is converted there.
 template <class E>
-__device__ __forceinline__ void load4x2(Rsrc r, uint32_t o0, uint32_t o1,
-                                        bf16x8 (&p)[InputPlanes<E>::n]) {
-  if constexpr (E::kSize == 2) {
-    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o0, 0, 0));
-    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o1, 0, 0));
-    const u32x4 v = __builtin_shufflevector(a, b, 0, 1, 2, 3);
-    if constexpr (InputPlanes<E>::n == 1)
-      p[0] = __builtin_bit_cast(bf16x8, v);
-    else
-      split(__builtin_convertvector(__builtin_bit_cast(f16x8, v), f32x8), p);
-  } else {
-    split(join(__builtin_bit_cast(f32x4, bld16<0>(r, o0)),
-               __builtin_bit_cast(f32x4, bld16<0>(r, o1))), p);
-  }
-}
-
-template <class E>
-__device__ __forceinline__ float load1(Rsrc r, uint32_t off) {
+__device__ __forceinline__ unsigned load1_raw(Rsrc r, uint32_t off) {
   if constexpr (E::kSize == 4)
-    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
   else
-    return E::widen16((unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+    return (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+}
+template <class E>
+__device__ __forceinline__ float value_of(unsigned raw) {
+  if constexpr (E::kSize == 4)
+    return __uint_as_float(raw);
+  else
+    return E::widen16((unsigned short)raw);
 }
 
 template <class E>
@@ -164,10 +181,15 @@ __device__ __forceinline__ void store1(Rsrc r, uint32_t off, float x) {
   }
 }
 
+// The largest of values >= 0 over the wave, in a scalar register (DPP, no LDS).
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
+  x = fmaxf(x, dpp_any<kRowShr1>(x));
+  x = fmaxf(x, dpp_any<kRowShr2>(x));
+  x = fmaxf(x, dpp_any<kRowShr4>(x));
+  x = fmaxf(x, dpp_any<kRowShr8>(x));
+  x = fmaxf(x, dpp<kRowBcast15, 0xa>(x, x));
+  x = fmaxf(x, dpp<kRowBcast31, 0xc>(x, x));
+  return readlane(x, 63);
 }
 
 __device__ __forceinline__ float wave_sum(float x) {

@@ -254,61 +254,125 @@ __device__ __forceinline__ void keep(char* to, float* scale, const f32x4 (&x)[2 
 }
 
 // ---------------------------------------------------------------------------- walks over chunks
-// What the walks read of a chunk, in LDS: K and Q as frags, N and M, and per step exp(G),
-// exp(G_end - G) and beta.
-template <class E, int KD, int kTerms, int kOut>
+// A walk's workgroup: kWaves waves that compute and kWaves that bring the next chunk from memory to
+// LDS. A computing wave owns 16 columns of the state (all key rows, in registers, lane by column), so
+// the chain of a chunk, K S -> E -> S, passes from product to product without leaving the wave; the
+// left operands are shared in LDS. Of a pair of waves, columns interleave as key_col says.
+//
+// In LDS, of a chunk: K, Q and V (dO) as frags, N and M, and per step exp(G), exp(G_end - G), beta.
+template <class E, int KD, int kTerms, int kOut, int kWaves>
 struct ChunkLds {
   static constexpr int NI = InputPlanes<E>::n;
-  static constexpr int kBlocks = KD / 32;
-  static constexpr int kPlane = kChunk * KD * 2;
-  static constexpr int k = 0, q = k + NI * kPlane, n = q + NI * kPlane, m = n + kTerms * kTriBytes,
-                       gam = m + kOut * kTriBytes, end = gam + 4 * kChunk, beta = end + 4 * kChunk,
-                       size = beta + 4 * kChunk;
+  static constexpr int kBlocks = KD / 32, kCols = 16 * kWaves, kColBlocks = kCols / 32;
+  static constexpr int kPlane = kChunk * KD * 2, kColPlane = kChunk * kCols * 2;
+  static constexpr int k = 0, q = k + NI * kPlane, v = q + NI * kPlane, n = v + NI * kColPlane,
+                       m = n + kTerms * kTriBytes, gam = m + kOut * kTriBytes, end = gam + 4 * kChunk,
+                       beta = end + 4 * kChunk, size = beta + 4 * kChunk;
+  // per wave, to turn 16 columns of results into rows (half types)
+  static constexpr int kTurn = E::kSize == 2 ? 2048 : 0;
+  // two buffers where they fit: a chunk is then stored while the one before is still read
+  static constexpr int kBuffers = 2 * size + kWaves * kTurn <= 160 * 1024 ? 2 : 1;
+  static constexpr int turn = kBuffers * size, total = turn + kWaves * kTurn;
+  static_assert(total <= 160 * 1024, "a chunk fits LDS");
 };
 
-// K and Q of a chunk as frags, plane after plane.
-template <class E, int KD>
-__device__ __forceinline__ void stage_keys(char* k, char* q, const DeltaArgs& a, int64_t b, int64_t hk,
-                                           int64_t t0) {
-  constexpr int NI = InputPlanes<E>::n, G8 = KD / 8, kBlocks = KD / 32, kPlane = kChunk * KD * 2;
-  const int rows = rows_left(a.L, t0);
-  const Rsrc rk = head_rsrc(a.k, b, hk, t0, rows, a.Dk, E::kSize);
-  const Rsrc rq = head_rsrc(a.q, b, hk, t0, rows, a.Dk, E::kSize);
-  for (int i = threadIdx.x; i < kChunk * G8; i += blockDim.x) {
-    const int t = i / G8, d = (i % G8) * 8;
-    bf16x8 pk[NI], pq[NI];
-    load8<E>(rk, d < a.Dk ? (t * (int)a.k.t + d) * E::kSize : kNoOffset, pk);
-    load8<E>(rq, d < a.Dk ? (t * (int)a.q.t + d) * E::kSize : kNoOffset, pq);
-    const int u0 = frag_unit<kBlocks>(t, d), u1 = frag_unit<kBlocks>(t, d + 4);
+// kCols columns of a chunk's 64 rows, in blocks of 16 x 32 shared among kWaves waves: on the way from
+// memory, and in LDS as planes.
+template <class E, int kCols, int kWaves>
+struct RowBlocks {
+  static constexpr int NI = InputPlanes<E>::n, kBlocks = kCols / 32, n = 4 * kBlocks / kWaves;
+  static constexpr int kVec = E::kSize / 2, kPlane = kChunk * kCols * 2;
+  u32x4 x[n][kVec];
+
+  // columns col0 .. of `dim`
+  __device__ __forceinline__ void load(const Heads& from, int64_t b, int64_t h, int64_t t0, int rows,
+                                       int dim, int col0, int w) {
+    const Rsrc r = head_rsrc(from, b, h, t0, rows, dim, E::kSize);
+    const int lane = threadIdx.x & 63, st = (int)from.t * E::kSize;
 #pragma unroll
-    for (int p = 0; p < NI; ++p) {
-      const u32x4 vk = __builtin_bit_cast(u32x4, pk[p]), vq = __builtin_bit_cast(u32x4, pq[p]);
-      *reinterpret_cast<u32x2*>(k + p * kPlane + u0) = u32x2{vk[0], vk[1]};
-      *reinterpret_cast<u32x2*>(k + p * kPlane + u1) = u32x2{vk[2], vk[3]};
-      *reinterpret_cast<u32x2*>(q + p * kPlane + u0) = u32x2{vq[0], vq[1]};
-      *reinterpret_cast<u32x2*>(q + p * kPlane + u1) = u32x2{vq[2], vq[3]};
+    for (int i = 0; i < n; ++i) {
+      const int block = w * n + i, t = 16 * (block / kBlocks) + (lane & 15),
+                d = col0 + 32 * (block % kBlocks) + 8 * (lane >> 4);
+#pragma unroll
+      for (int v = 0; v < kVec; ++v)
+        x[i][v] = bld16<0>(r, d < dim ? t * st + d * E::kSize + 16 * v : kNoOffset);
     }
   }
-}
 
-template <class E, int KD, int kTerms, int kOut>
-__device__ __forceinline__ void stage(char* lds, const DeltaArgs& a, int64_t ch, int64_t b, int64_t hk,
-                                      int64_t t0) {
-  using C = ChunkLds<E, KD, kTerms, kOut>;
-  const int tid = threadIdx.x, nt = blockDim.x;
-  stage_keys<E, KD>(lds + C::k, lds + C::q, a, b, hk, t0);
-  for (int i = tid; i < kTerms * kTriBytes / 16; i += nt)
-    reinterpret_cast<u32x4*>(lds + C::n)[i] =
-        reinterpret_cast<const u32x4*>(a.n + ch * kTerms * kTriBytes)[i];
-  for (int i = tid; i < kOut * kTriBytes / 16; i += nt)
-    reinterpret_cast<u32x4*>(lds + C::m)[i] =
-        reinterpret_cast<const u32x4*>(a.m + ch * kOut * kTriBytes)[i];
-  if (tid < kChunk) {
-    const f32x4* gb = reinterpret_cast<const f32x4*>(a.gb) + ch * kChunk;
-    const f32x4 x = gb[tid], l = gb[kChunk - 1];
-    reinterpret_cast<float*>(lds + C::gam)[tid] = expf(x[0]) * (1.0f + x[1]);
-    reinterpret_cast<float*>(lds + C::end)[tid] = expf((l[0] - x[0]) + (l[1] - x[1]));
-    reinterpret_cast<float*>(lds + C::beta)[tid] = x[2];
+  __device__ __forceinline__ void store(char* to, int w) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      bf16x8 p[NI];
+      if constexpr (NI == 1)
+        p[0] = __builtin_bit_cast(bf16x8, x[i][0]);
+      else if constexpr (NI == 2)
+        split(__builtin_convertvector(__builtin_bit_cast(f16x8, x[i][0]), f32x8), p);
+      else
+        split(join(__builtin_bit_cast(f32x4, x[i][0]), __builtin_bit_cast(f32x4, x[i][kVec - 1])), p);
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<bf16x8*>(to + j * kPlane + (w * n + i) * 1024 +
+                                   frag_lane(lane & 15, lane >> 4)) = p[j];
+    }
+  }
+};
+
+// Whole KiB copied as they are, shared among kWaves waves.
+template <int kCount, int kWaves>
+struct Copies {
+  static constexpr int n = (kCount + kWaves - 1) / kWaves;
+  u32x4 x[n];
+
+  __device__ __forceinline__ void load(const char* from, int w) {
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (kCount % kWaves == 0 || w + i * kWaves < kCount)
+        x[i] = reinterpret_cast<const u32x4*>(from + (w + i * kWaves) * 1024)[threadIdx.x & 63];
+  }
+  __device__ __forceinline__ void store(char* to, int w) const {
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (kCount % kWaves == 0 || w + i * kWaves < kCount)
+        reinterpret_cast<u32x4*>(to + (w + i * kWaves) * 1024)[threadIdx.x & 63] = x[i];
+  }
+};
+
+// The waves that bring chunks: `value` is V or dO, chunks first, first + step .. of `count`.
+template <class E, int KD, int kTerms, int kOut, int kWaves>
+__device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const Heads& value, int64_t bh,
+                                      int64_t b, int64_t h, int64_t hk, int col0, int w, int64_t first,
+                                      int64_t step) {
+  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
+  const int lane = threadIdx.x & 63;
+  for (int64_t i = 0, c = first; i < a.chunks; ++i, c += step) {
+    const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
+    const int rows = rows_left(a.L, t0);
+    RowBlocks<E, KD, kWaves> k, q;
+    RowBlocks<E, C::kCols, kWaves> v;
+    Copies<6 * kTerms, kWaves> n;
+    Copies<6 * kOut, kWaves> m;
+    f32x4 gb = {};
+    k.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
+    n.load(a.n + ch * kTerms * kTriBytes, w);
+    v.load(value, b, h, t0, rows, a.Dv, col0, w);
+    q.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
+    m.load(a.m + ch * kOut * kTriBytes, w);
+    if (w == 0) gb = reinterpret_cast<const f32x4*>(a.gb)[ch * kChunk + lane];
+    if (C::kBuffers == 1 && i > 0) lds_barrier();  // the chunk before is read
+    char* const lds = buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0);
+    k.store(lds + C::k, w);
+    n.store(lds + C::n, w);
+    v.store(lds + C::v, w);
+    q.store(lds + C::q, w);
+    m.store(lds + C::m, w);
+    if (w == 0) {
+      const float hi = readlane(gb[0], 63), lo = readlane(gb[1], 63);
+      reinterpret_cast<float*>(lds + C::gam)[lane] = expf(gb[0]) * (1.0f + gb[1]);
+      reinterpret_cast<float*>(lds + C::end)[lane] = expf((hi - gb[0]) + (lo - gb[1]));
+      reinterpret_cast<float*>(lds + C::beta)[lane] = gb[2];
+    }
+    lds_barrier();
   }
 }
 
@@ -326,128 +390,251 @@ __device__ __forceinline__ void cols_of(const char* lo, const char* hi, int plan
   for (int i = 0; i < NP; ++i) p[i] = frag_cols(lo + i * plane_bytes, hi + i * plane_bytes, ct, lane);
 }
 
-// Forward. A wave owns 16 columns of the state (all key rows, in registers, lane by column), so the
-// chain of a chunk, K S -> E -> S, passes from product to product without leaving the wave: a
-// workgroup's waves share the left operands in LDS and meet only to exchange those.
-template <class E, int KD, int kTerms, bool kSave>
-__global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a) {
+// The value that planes stand for.
+template <int NP>
+__device__ __forceinline__ f32x8 whole(const bf16x8 (&p)[NP]) {
+  f32x8 x = __builtin_convertvector(p[NP - 1], f32x8);
+#pragma unroll
+  for (int i = NP - 2; i >= 0; --i) x += __builtin_convertvector(p[i], f32x8);
+  return x;
+}
+
+// c += the lower triangle `f` times b, 64 steps by the wave's columns.
+template <int kTerms, int NA, int NB>
+__device__ __forceinline__ void mma_triangle(const bf16x8 (&f)[6][NA], const bf16x8 (&b)[2][NB],
+                                             f32x4 (&c)[4]) {
+#pragma unroll
+  for (int t = kTerms - 1; t >= 0; --t)
+#pragma unroll
+    for (int i = 0; i <= t; ++i)
+      if (i < NA && t - i < NB)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int mt = 2 * s; mt < 4; ++mt)
+            c[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[tri_block(mt, s)][i], b[s][t - i], c[mt],
+                                                            0, 0, 0);
+}
+
+// c += its transpose times b; operands as triangle_t loads them.
+__device__ __forceinline__ constexpr int upper_block(int mt, int s) { return s == 0 ? mt : 2 + mt; }
+template <int kTerms, int NA, int NB>
+__device__ __forceinline__ void mma_triangle_t(const bf16x8 (&f)[6][NA], const bf16x8 (&b)[2][NB],
+                                               f32x4 (&c)[4]) {
+#pragma unroll
+  for (int t = kTerms - 1; t >= 0; --t)
+#pragma unroll
+    for (int i = 0; i <= t; ++i)
+      if (i < NA && t - i < NB)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int mt = 0; mt < 2 * s + 2; ++mt)
+            c[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[upper_block(mt, s)][i], b[s][t - i], c[mt],
+                                                            0, 0, 0);
+}
+
+// Operands of a lower triangle, and of its transpose.
+template <int NP>
+__device__ __forceinline__ void triangle(const char* from, int lane, bf16x8 (&f)[6][NP]) {
+#pragma unroll
+  for (int i = 0; i < 6; ++i) rows_of(from + i * 1024, kTriBytes, lane, f[i]);
+}
+template <int NP>
+__device__ __forceinline__ void triangle_t(const char* from, int lane, bf16x8 (&f)[6][NP]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int mt = 0; mt < 2 * s + 2; ++mt)
+      cols_of(from + tri_block(2 * s, mt / 2) * 1024, from + tri_block(2 * s + 1, mt / 2) * 1024, kTriBytes,
+              mt, lane, f[upper_block(mt, s)]);
+}
+
+// A wave's 16 columns of 64 result rows to the contiguous (batch, seqlen, heads, value_dim) tensor:
+// the half types by way of `turn`, four columns a lane and store.
+template <class E>
+__device__ __forceinline__ void write_columns(const DeltaArgs& a, int64_t b, int64_t h, int64_t t0,
+                                              int rows, int col0, int tile, char* turn,
+                                              const f32x4 (&x)[4], int lane) {
+  const int li = lane & 15, lg = lane >> 4, st = a.H * a.Dv * E::kSize;
+  const Rsrc r = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
+                          ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+  if constexpr (E::kSize == 2) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      u32x4 p;
+      if constexpr (InputPlanes<E>::n == 1)
+        p = __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * s], x[2 * s + 1]), bf16x8));
+      else
+        p = __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * s], x[2 * s + 1]), f16x8));
+      *reinterpret_cast<u32x4*>(turn + s * 1024 + frag_lane(li, lg)) = p;
+    }
+    const int d = col0 + key_col(tile, 4 * lg);
+    typedef __attribute__((address_space(3))) s16x4* ldsp;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const char* from = turn + mt / 2 * 1024 + frag_lane(4 * lg + ((lane >> 2) & 3), lane & 3) +
+                         (mt & 1) * 8;
+      const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ldsp)from);
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r,
+                                            d < a.Dv ? (16 * mt + li) * st + d * 2 : kNoOffset, 0, 0);
+    }
+  } else {
+    const int d = col0 + key_col(tile, li);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store1<E>(r, d < a.Dv ? (16 * mt + 4 * lg + i) * st + d * E::kSize : kNoOffset, x[mt][i]);
+  }
+}
+
+// A walk's workgroup: which head and value columns. The workgroups of one head, which read the same K,
+// Q, N and M, are eight apart: on one XCD.
+struct Place {
+  int64_t bh, b, h, hk;
+  int col0;
+};
+template <int kWaves>
+__device__ __forceinline__ Place place_of(const DeltaArgs& a) {
+  const int64_t id = blockIdx.x, bh = id / (8 * a.vblocks) * 8 + id % 8, b = bh / a.H, h = bh - b * a.H;
+  return {bh, b, h, h / a.R, (int)(id / 8 % a.vblocks) * 16 * kWaves};
+}
+
+template <class E, int KD, int kTerms, bool kSave, int kWaves>
+__global__ __launch_bounds__(128 * kWaves) void delta_chunks(DeltaArgs a) {
   constexpr int kOut = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
-  using C = ChunkLds<E, KD, kTerms, kOut>;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  // the workgroups of one head, which read the same K, Q, N and M, on one XCD
-  const int64_t id = blockIdx.x, bh = id / (8 * a.vblocks) * 8 + id % 8;
-  const int vb = (int)(id / 8 % a.vblocks);
-  if (bh >= a.heads_total) return;
-  const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / a.R;
+  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
+  extern __shared__ __attribute__((aligned(16))) char buffers[];
+  const Place p = place_of<kWaves>(a);
+  if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
-  const int tile = vb * (blockDim.x >> 6) + w, col = tile * 16 + li;
+  if (w >= kWaves) {
+    bring<E, KD, kTerms, kOut, kWaves>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves, 0, 1);
+    return;
+  }
+  const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2, col = p.col0 + key_col(w, li);
   const bool in = col < a.Dv;
-  const int tiles = (a.Dv + 15) >> 4;
-  const int vst = (int)a.v.t * E::kSize, ost = a.H * a.Dv * E::kSize;
 
   f32x4 S[KT];
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * lg + r;
-      S[t][r] = a.state && in && row < a.Dk ? a.state[(bh * a.Dk + row) * a.Dv + col] : 0.0f;
+      const int row = key_col(t, 4 * lg + r);
+      S[t][r] = a.state && in && row < a.Dk ? a.state[(p.bh * a.Dk + row) * a.Dv + col] : 0.0f;
     }
 
+  lds_barrier();
   for (int64_t c = 0; c < a.chunks; ++c) {
-    const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
-    const int rows = rows_left(a.L, t0);
-    const Rsrc rv = head_rsrc(a.v, b, h, t0, rows, a.Dv, E::kSize);
-    f32x4 x[4];
+    const int64_t ch = p.bh * a.chunks + c, t0 = c * kChunk;
+    const char* const lds = buffers + (C::kBuffers == 2 && (c & 1) ? C::size : 0);
+    // operands of the next steps on their way while a step's products run
+    constexpr int kAhead = NI == 1 ? 2 : 1;
+    auto keys_at = [&](int step, bf16x8 (&f)[4][NI]) {  // K and Q in turn, 32 key columns a step
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+      for (int mt = 0; mt < 4; ++mt)
+        rows_of(lds + (step & 1 ? C::q : C::k) + (mt * C::kBlocks + step / 2) * 1024, C::kPlane, lane,
+                f[mt]);
+    };
+    auto steps_at = [&](int step, bf16x8 (&f)[4][NI]) {  // K^T, four tiles by 32 steps
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        x[mt][r] = load1<E>(rv, in ? (16 * mt + 4 * lg + r) * vst + col * E::kSize : kNoOffset);
-    __syncthreads();
-    stage<E, KD, kTerms, kOut>(lds, a, ch, b, hk, t0);
-    __syncthreads();
+      for (int i = 0; i < 4; ++i) {
+        const int t = 4 * (step / 2) + i;
+        const char* at = lds + C::k + (2 * (step & 1) * C::kBlocks + t / 2) * 1024;
+        cols_of(at, at + C::kBlocks * 1024, C::kPlane, t, lane, f[i]);
+      }
+    };
+    // a per-step value of the wave's rows of tile mt
+    auto row_of = [&](int which, int mt) {
+      return *reinterpret_cast<const f32x4*>(lds + which + (16 * mt + 4 * lg) * 4);
+    };
+    constexpr int kSteps = 2 * C::kBlocks, kUpdates = KT / 2;
+    f32x4 ks[4] = {}, o[4] = {};
+    bf16x8 ring[kAhead + 1][4][NI], nf[6][kTerms], vp[2][NI], sp[kTerms];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) keys_at(i, ring[i]);
     if (kSave && tile < tiles)
       keep<E, KT / 2>(a.s + (ch * tiles + tile) * KD * 16 * kept_size<E>(), a.ss + ch * tiles + tile,
                       S, lane);
-
-    f32x4 ks[4] = {}, o[4] = {};
 #pragma unroll
-    for (int s = 0; s < KD / 32; ++s) {
-      bf16x8 sp[kTerms];
-      split(join(S[2 * s], S[2 * s + 1]), sp);
+    for (int i = 0; i < kSteps; ++i) {
+      if (i + kAhead < kSteps) {
+        keys_at(i + kAhead, ring[(i + kAhead) % (kAhead + 1)]);
+      } else if (i + 1 == kSteps) {
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        bf16x8 f[NI];
-        const int at = (mt * C::kBlocks + s) * 1024;
-        rows_of(lds + C::k + at, C::kPlane, lane, f);
-        ks[mt] = mma<kTerms>(f, sp, ks[mt]);
-        rows_of(lds + C::q + at, C::kPlane, lane, f);
-        o[mt] = mma<kOut>(f, sp, o[mt]);
+        for (int s = 0; s < 2; ++s) {
+          const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
+          cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+        }
+        triangle(lds + C::n, lane, nf);
       }
+      if (i % 2 == 0) split(join(S[i], S[i + 1]), sp);
+      in_order();
+      if (i % 2 == 0)
+        mma_tiles<kTerms>(ring[i % (kAhead + 1)], sp, ks);
+      else
+        mma_tiles<kOut>(ring[i % (kAhead + 1)], sp, o);
+      in_order();
     }
     // x: V -> R -> E; u: beta R -> U
-    f32x4 gam[4], u[4];
+    f32x4 x[4], u[4], y[4] = {};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const f32x8 v = whole(vp[s]);
+      x[2 * s] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+      x[2 * s + 1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      gam[mt] = *reinterpret_cast<const f32x4*>(lds + C::gam + (16 * mt + 4 * lg) * 4);
-      x[mt] -= gam[mt] * ks[mt];
-      u[mt] = *reinterpret_cast<const f32x4*>(lds + C::beta + (16 * mt + 4 * lg) * 4) * x[mt];
+      const f32x4 gam = row_of(C::gam, mt);
+      x[mt] -= gam * ks[mt];
+      u[mt] = row_of(C::beta, mt) * x[mt];
+      o[mt] *= gam * a.scale;
     }
     bf16x8 up[2][kTerms];
     split(join(u[0], u[1]), up[0]);
     split(join(u[2], u[3]), up[1]);
+    in_order();
+    mma_triangle<kTerms>(nf, up, y);
+    in_order();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) steps_at(i, ring[i]);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      f32x4 y = {};
-#pragma unroll
-      for (int s = 0; s <= mt / 2; ++s) {
-        bf16x8 f[kTerms];
-        rows_of(lds + C::n + tri_block(mt, s) * 1024, kTriBytes, lane, f);
-        y = mma<kTerms>(f, up[s], y);
-      }
-      x[mt] -= y;
-      u[mt] = *reinterpret_cast<const f32x4*>(lds + C::beta + (16 * mt + 4 * lg) * 4) * x[mt];
+      x[mt] -= y[mt];
+      u[mt] = row_of(C::beta, mt) * x[mt];
     }
-    if (kSave && tile < tiles)
-      keep<E, 2>(a.e + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.es + ch * tiles + tile, x,
-                 lane);
-    {
-      bf16x8 uo[2][kOut];
-      split(join(u[0], u[1]), uo[0]);
-      split(join(u[2], u[3]), uo[1]);
-      const Rsrc ro = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
-                               ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+    bf16x8 uo[2][kOut];
+    split(join(u[0], u[1]), uo[0]);
+    split(join(u[2], u[3]), uo[1]);
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        f32x4 y = o[mt] * (gam[mt] * a.scale);
-#pragma unroll
-        for (int s = 0; s <= mt / 2; ++s) {
-          bf16x8 f[kOut];
-          rows_of(lds + C::m + tri_block(mt, s) * 1024, kTriBytes, lane, f);
-          y = mma<kOut>(f, uo[s], y);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          store1<E>(ro, in ? (16 * mt + 4 * lg + r) * ost + col * E::kSize : kNoOffset, y[r]);
-      }
-    }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-      u[mt] *= *reinterpret_cast<const f32x4*>(lds + C::end + (16 * mt + 4 * lg) * 4);
+    for (int mt = 0; mt < 4; ++mt) u[mt] *= row_of(C::end, mt);
     split(join(u[0], u[1]), up[0]);
     split(join(u[2], u[3]), up[1]);
     const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+    bf16x8 mf[6][kOut];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      S[t] *= last;
+    for (int t = 0; t < KT; ++t) S[t] *= last;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 f[NI];
-        const char* at = lds + C::k + (2 * s * C::kBlocks + t / 2) * 1024;
-        cols_of(at, at + C::kBlocks * 1024, C::kPlane, t, lane, f);
-        S[t] = mma<kTerms>(f, up[s], S[t]);
-      }
+    for (int i = 0; i < kUpdates; ++i) {
+      if (i + kAhead < kUpdates)
+        steps_at(i + kAhead, ring[(i + kAhead) % (kAhead + 1)]);
+      else if (i + 1 == kUpdates)
+        triangle(lds + C::m, lane, mf);
+      in_order();
+      mma_tiles<kTerms>(ring[i % (kAhead + 1)], up[i & 1], &S[4 * (i / 2)]);
+      in_order();
+    }
+    mma_triangle<kOut>(mf, uo, o);
+    if (kSave && tile < tiles)
+      keep<E, 2>(a.e + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.es + ch * tiles + tile, x,
+                 lane);
+    write_columns<E>(a, p.b, p.h, t0, rows_left(a.L, t0), p.col0, w, buffers + C::turn + w * C::kTurn, o,
+                     lane);
+    if (c + 1 < a.chunks) {
+      if (C::kBuffers == 1) lds_barrier();  // this chunk is read
+      lds_barrier();                        // the next one is there
     }
   }
   if (a.state && in)
@@ -455,123 +642,123 @@ __global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a) {
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = 16 * t + 4 * lg + r;
-        if (row < a.Dk) a.state[(bh * a.Dk + row) * a.Dv + col] = S[t][r];
+        const int row = key_col(t, 4 * lg + r);
+        if (row < a.Dk) a.state[(p.bh * a.Dk + row) * a.Dv + col] = S[t][r];
       }
 }
 
 // Backward walk, the same way: a wave owns 16 columns of dS' and gives dV, and for the gradients of q
 // and k the dS' and Y of every chunk.
-template <class E, int KD>
-__global__ __launch_bounds__(256) void delta_chunks_bwd(DeltaArgs a) {
+template <class E, int KD, int kWaves>
+__global__ __launch_bounds__(128 * kWaves) void delta_chunks_bwd(DeltaArgs a) {
   constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
-  using C = ChunkLds<E, KD, kT, kT>;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int64_t id = blockIdx.x, bh = id / (8 * a.vblocks) * 8 + id % 8;
-  const int vb = (int)(id / 8 % a.vblocks);
-  if (bh >= a.heads_total) return;
-  const int64_t b = bh / a.H, h = bh - b * a.H, hk = h / a.R;
-  const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
-  const int tile = vb * (blockDim.x >> 6) + w, col = tile * 16 + li;
-  const bool in = col < a.Dv;
-  const int tiles = (a.Dv + 15) >> 4;
-  const int gst = (int)a.go.t * E::kSize, ost = a.H * a.Dv * E::kSize;
+  using C = ChunkLds<E, KD, kT, kT, kWaves>;
+  extern __shared__ __attribute__((aligned(16))) char buffers[];
+  const Place p = place_of<kWaves>(a);
+  if (p.bh >= a.heads_total) return;
+  const int lane = threadIdx.x & 63, w = wave_index(), lg = lane >> 4;
+  if (w >= kWaves) {
+    bring<E, KD, kT, kT, kWaves>(buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves,
+                                 a.chunks - 1, -1);
+    return;
+  }
+  const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2;
 
   f32x4 dS[KT] = {};
-  for (int64_t c = a.chunks - 1; c >= 0; --c) {
-    const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
-    const int rows = rows_left(a.L, t0);
-    const Rsrc rg = head_rsrc(a.go, b, h, t0, rows, a.Dv, E::kSize);
-    f32x4 x[4];
+  lds_barrier();
+  for (int64_t i = 0; i < a.chunks; ++i) {
+    const int64_t c = a.chunks - 1 - i, ch = p.bh * a.chunks + c, t0 = c * kChunk;
+    const char* const lds = buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0);
+    constexpr int kAhead = NI == 1 ? 2 : 1, kSteps = C::kBlocks, kUpdates = KT;
+    auto keys_at = [&](int step, bf16x8 (&f)[4][NI]) {
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+      for (int mt = 0; mt < 4; ++mt)
+        rows_of(lds + C::k + (mt * C::kBlocks + step) * 1024, C::kPlane, lane, f[mt]);
+    };
+    auto steps_at = [&](int step, bf16x8 (&f)[4][NI]) {  // Q^T and K^T, four tiles by 32 steps
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        x[mt][r] = load1<E>(rg, in ? (16 * mt + 4 * lg + r) * gst + col * E::kSize : kNoOffset);
-    __syncthreads();
-    stage<E, KD, kT, kT>(lds, a, ch, b, hk, t0);
-    __syncthreads();
+      for (int j = 0; j < 4; ++j) {
+        const int t = 4 * (step / 2 % (KT / 4)) + j;
+        const char* at = lds + (step < KT / 2 ? C::q : C::k) + (2 * (step & 1) * C::kBlocks + t / 2) * 1024;
+        cols_of(at, at + C::kBlocks * 1024, C::kPlane, t, lane, f[j]);
+      }
+    };
+    auto row_of = [&](int which, int mt) {
+      return *reinterpret_cast<const f32x4*>(lds + which + (16 * mt + 4 * lg) * 4);
+    };
+    f32x4 u[4] = {}, y[4] = {};
+    bf16x8 ring[kAhead + 1][4][NI], nf[6][kT], vp[2][NI], sp[kT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
+      cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+    }
+    triangle_t(lds + C::m, lane, nf);
     if (tile < tiles)
       keep<E, KT / 2>(a.ds + (ch * tiles + tile) * KD * 16 * kept_size<E>(), a.dss + ch * tiles + tile,
                       dS, lane);
-
-    f32x4 u[4] = {}, beta[4];
+    in_order();
 #pragma unroll
-    for (int s = 0; s < KD / 32; ++s) {
-      bf16x8 sp[kT];
-      split(join(dS[2 * s], dS[2 * s + 1]), sp);
+    for (int j = 0; j < kAhead; ++j) keys_at(j, ring[j]);
+    mma_triangle_t<kT>(nf, vp, y);
+    in_order();
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        bf16x8 f[NI];
-        rows_of(lds + C::k + (mt * C::kBlocks + s) * 1024, C::kPlane, lane, f);
-        u[mt] = mma<kT>(f, sp, u[mt]);
-      }
+    for (int j = 0; j < kSteps; ++j) {
+      if (j + kAhead < kSteps)
+        keys_at(j + kAhead, ring[(j + kAhead) % (kAhead + 1)]);
+      else if (j + 1 == kSteps)
+        triangle_t(lds + C::n, lane, nf);
+      split(join(dS[2 * j], dS[2 * j + 1]), sp);
+      in_order();
+      mma_tiles<kT>(ring[j % (kAhead + 1)], sp, u);
+      in_order();
     }
-    {
-      bf16x8 xp[2][NI];
-      split(join(x[0], x[1]), xp[0]);
-      split(join(x[2], x[3]), xp[1]);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        u[mt] *= *reinterpret_cast<const f32x4*>(lds + C::end + (16 * mt + 4 * lg) * 4);
-        beta[mt] = *reinterpret_cast<const f32x4*>(lds + C::beta + (16 * mt + 4 * lg) * 4);
-#pragma unroll
-        for (int s = mt / 2; s < 2; ++s) {
-          bf16x8 f[kT];
-          cols_of(lds + C::m + tri_block(2 * s, mt / 2) * 1024,
-                  lds + C::m + tri_block(2 * s + 1, mt / 2) * 1024, kTriBytes, mt, lane, f);
-          u[mt] = mma<kT>(f, xp[s], u[mt]);
-        }
-      }
-    }
-    bf16x8 up[2][kT];
-    split(join(beta[0] * u[0], beta[1] * u[1]), up[0]);
-    split(join(beta[2] * u[2], beta[3] * u[3]), up[1]);
+    bf16x8 up[2][kT], xp[2][kT];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      f32x4 y = {};
+      u[mt] = y[mt] + u[mt] * row_of(C::end, mt);
+      y[mt] = row_of(C::beta, mt) * u[mt];
+    }
+    split(join(y[0], y[1]), up[0]);
+    split(join(y[2], y[3]), up[1]);
 #pragma unroll
-      for (int s = mt / 2; s < 2; ++s) {
-        bf16x8 f[kT];
-        cols_of(lds + C::n + tri_block(2 * s, mt / 2) * 1024,
-                lds + C::n + tri_block(2 * s + 1, mt / 2) * 1024, kTriBytes, mt, lane, f);
-        y = mma<kT>(f, up[s], y);
-      }
-      u[mt] -= y;
+    for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{};
+    in_order();
+    mma_triangle_t<kT>(nf, up, y);
+    in_order();
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) steps_at(j, ring[j]);
+    // u: Y; y: -exp(G) dV; xp: scale exp(G) dO
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      u[mt] -= y[mt];
+      y[mt] = u[mt] * (row_of(C::beta, mt) * -row_of(C::gam, mt));
+    }
+    split(join(y[0], y[1]), up[0]);
+    split(join(y[2], y[3]), up[1]);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      split(whole(vp[s]) * (join(row_of(C::gam, 2 * s), row_of(C::gam, 2 * s + 1)) * a.scale), xp[s]);
+    const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) dS[t] *= last;
+#pragma unroll
+    for (int j = 0; j < kUpdates; ++j) {
+      if (j + kAhead < kUpdates) steps_at(j + kAhead, ring[(j + kAhead) % (kAhead + 1)]);
+      in_order();
+      mma_tiles<kT>(ring[j % (kAhead + 1)], j < KT / 2 ? xp[j & 1] : up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
+      in_order();
     }
     if (tile < tiles)
       keep<E, 2>(a.y + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.ys + ch * tiles + tile, u,
                  lane);
-    const Rsrc ro = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
-                             ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      u[mt] *= beta[mt];
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store1<E>(ro, in ? (16 * mt + 4 * lg + r) * ost + col * E::kSize : kNoOffset, u[mt][r]);
-      const f32x4 gam = *reinterpret_cast<const f32x4*>(lds + C::gam + (16 * mt + 4 * lg) * 4);
-      u[mt] *= -gam;
-      x[mt] *= gam * a.scale;
-    }
-    split(join(u[0], u[1]), up[0]);
-    split(join(u[2], u[3]), up[1]);
-    bf16x8 xp[2][kT];
-    split(join(x[0], x[1]), xp[0]);
-    split(join(x[2], x[3]), xp[1]);
-    const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      dS[t] *= last;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 f[NI];
-        const int at = (2 * s * C::kBlocks + t / 2) * 1024;
-        cols_of(lds + C::k + at, lds + C::k + at + C::kBlocks * 1024, C::kPlane, t, lane, f);
-        dS[t] = mma<kT>(f, up[s], dS[t]);
-        cols_of(lds + C::q + at, lds + C::q + at + C::kBlocks * 1024, C::kPlane, t, lane, f);
-        dS[t] = mma<kT>(f, xp[s], dS[t]);
-      }
+    for (int mt = 0; mt < 4; ++mt) u[mt] *= row_of(C::beta, mt);
+    write_columns<E>(a, p.b, p.h, t0, rows_left(a.L, t0), p.col0, w, buffers + C::turn + w * C::kTurn, u,
+                     lane);
+    if (c > 0) {
+      if (C::kBuffers == 1) lds_barrier();
+      lds_barrier();
     }
   }
 }
@@ -636,7 +823,7 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
   const int64_t group = blockIdx.x / a.chunks, c = blockIdx.x - group * a.chunks, t0 = c * kChunk;
   const int Hk = a.H / a.R;
   const int64_t b = group / Hk, hk = group - b * Hk;
-  const int rows = rows_left(a.L, t0), tiles = (a.Dv + 15) >> 4;
+  const int rows = rows_left(a.L, t0), tiles = (a.Dv + 31) / 32 * 2;
   float* const row_hi = reinterpret_cast<float*>(lds + C::hi);
   float* const row_lo = reinterpret_cast<float*>(lds + C::lo);
   float* const row_beta = reinterpret_cast<float*>(lds + C::beta);
@@ -701,15 +888,13 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
         cols_of(lds + C::s + at, lds + C::s + at + kBlocks * 1024, C::kState, ct, lane, sp[n]);
         cols_of(lds + C::ds + at, lds + C::ds + at + kBlocks * 1024, C::kState, ct, lane, dsp[n]);
       }
-      const int d0 = 32 * vb + 4 * lg;
-      load4x2<E>(rg, d0 < a.Dv ? (16 * w + li) * gst + d0 * E::kSize : kNoOffset,
-                 d0 + 16 < a.Dv ? (16 * w + li) * gst + (d0 + 16) * E::kSize : kNoOffset, ow);
+      const int d0 = 32 * vb + 8 * lg;
+      load8<E>(rg, d0 < a.Dv ? (16 * w + li) * gst + d0 * E::kSize : kNoOffset, ow);
       cols_of(lds + C::dv + w / 2 * 1024, lds + C::dv + (2 + w / 2) * 1024, C::kSteps, w, lane, vw);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         bf16x8 op[NI], vp[kT], upl[kT];
-        load4x2<E>(rg, d0 < a.Dv ? (16 * mt + li) * gst + d0 * E::kSize : kNoOffset,
-                   d0 + 16 < a.Dv ? (16 * mt + li) * gst + (d0 + 16) * E::kSize : kNoOffset, op);
+        load8<E>(rg, d0 < a.Dv ? (16 * mt + li) * gst + d0 * E::kSize : kNoOffset, op);
         cols_of(lds + C::dv + mt / 2 * 1024, lds + C::dv + (2 + mt / 2) * 1024, C::kSteps, mt, lane, vp);
         cols_of(lds + C::u + mt / 2 * 1024, lds + C::u + (2 + mt / 2) * 1024, C::kSteps, mt, lane, upl);
 #pragma unroll
@@ -725,7 +910,13 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
       }
     }
     __syncthreads();
-    stage_keys<E, KD>(lds + C::k, lds + C::q, a, b, hk, t0);
+    {
+      RowBlocks<E, KD, 4> keys, queries;
+      keys.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
+      queries.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
+      keys.store(lds + C::k, w);
+      queries.store(lds + C::q, w);
+    }
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt)
       if (nt <= (w | 1)) {
@@ -792,7 +983,7 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int col = 16 * ct + (li & ~3), unit = frag_unit<kBlocks>(16 * mt + 4 * lg + r, col);
+          const int unit = (mt * kBlocks + ct / 2) * 1024 + frag_lane(4 * lg + r, li >> 2) + (ct & 1) * 8;
           const float kv = key_at<NI>(lds + C::k, unit, li & 3, C::kKeys);
           const float qv = key_at<NI>(lds + C::q, unit, li & 3, C::kKeys);
           dG[mt][r] += qv * x[r] + kv * y[r];
@@ -848,7 +1039,7 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
   const Rsrc oq = row_rsrc(a.gq, base, E::kSize, bytes), ok = row_rsrc(a.gk, base, E::kSize, bytes);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int col = (w * NT + n) * 16 + li;
+    const int col = key_col(w * NT + n, li);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -911,7 +1102,7 @@ __global__ __launch_bounds__(256) void delta_steps(DeltaArgs a) {
     const float alpha = expf(element<E>(a.g, b, t, h)), beta = element<E>(a.beta, b, t, h);
     f32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = load1<E>(rv, in ? (col + j) * E::kSize : kNoOffset);
+    for (int j = 0; j < 4; ++j) v[j] = value_of<E>(load1_raw<E>(rv, in ? (col + j) * E::kSize : kNoOffset));
 
     f32x4 ks = {}, qs = {};
     float qk = 0.0f;
@@ -1066,7 +1257,7 @@ void carve_prep(Carver& w, DeltaArgs& a, const fpscan_delta* p, bool keeps_state
 
 // What a forward keeps for the gradients; the states and E, of 16 value columns a block.
 void carve_saved(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
-  const size_t blocks = (size_t)(a.heads_total * a.chunks) * ((a.Dv + 15) / 16);
+  const size_t blocks = (size_t)(a.heads_total * a.chunks) * ((a.Dv + 31) / 32 * 2);
   const size_t each = p->dtype == FPSCAN_DTYPE_BF16 ? 2 : 4;
   carve_prep(w, a, p, false);
   a.s = w.take(blocks * padded_key_dim(p) * 16 * each);
@@ -1077,7 +1268,7 @@ void carve_saved(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
 
 // What the walk backwards leaves for the gradients of q and k.
 void carve_bwd(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
-  const size_t blocks = (size_t)(a.heads_total * a.chunks) * ((a.Dv + 15) / 16);
+  const size_t blocks = (size_t)(a.heads_total * a.chunks) * ((a.Dv + 31) / 32 * 2);
   const size_t each = p->dtype == FPSCAN_DTYPE_BF16 ? 2 : 4;
   a.ds = w.take(blocks * padded_key_dim(p) * 16 * each);
   a.y = w.take(blocks * kChunk * 16 * each);
@@ -1107,34 +1298,39 @@ int allow_lds(K kernel, int bytes) {
              ? FPSCAN_OK : FPSCAN_ERR_LAUNCH;
 }
 
-// Waves of a walk's workgroup, each with 16 value columns, and the grid: groups of eight heads.
-int walk_waves(const DeltaArgs& a) { return a.Dv >= 64 ? 4 : (a.Dv + 15) / 16; }
+// A walk's grid, `waves` times 16 value columns a workgroup: groups of eight heads.
 unsigned walk_grid(DeltaArgs& a, int waves) {
   a.vblocks = (a.Dv + 16 * waves - 1) / (16 * waves);
   return (unsigned)((a.heads_total + 7) / 8 * 8 * a.vblocks);
 }
 
+// Computing waves of a walk's workgroup.
+template <class E>
+constexpr int walk_waves() { return InputPlanes<E>::n == 3 ? 2 : 4; }
+
 template <class E, int KD, int kTerms, bool kSave>
 int walk_forward(DeltaArgs& a, hipStream_t stream) {
-  constexpr int kOut = out_terms<E>(), lds = ChunkLds<E, KD, kTerms, kOut>::size;
+  constexpr int kOut = out_terms<E>(), kWaves = walk_waves<E>();
+  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
   delta_prep<E, KD, kTerms, kOut><<<(unsigned)(a.heads_total * a.chunks), 256, 0, stream>>>(a);
   int st = launched();
   if (st != FPSCAN_OK) return st;
-  if ((st = allow_lds(delta_chunks<E, KD, kTerms, kSave>, lds)) != FPSCAN_OK) return st;
-  const int waves = walk_waves(a);
-  const unsigned grid = walk_grid(a, waves);
-  delta_chunks<E, KD, kTerms, kSave><<<grid, 64 * waves, lds, stream>>>(a);
+  const auto walk = delta_chunks<E, KD, kTerms, kSave, kWaves>;
+  if ((st = allow_lds(walk, C::total)) != FPSCAN_OK) return st;
+  const unsigned grid = walk_grid(a, kWaves);
+  walk<<<grid, 128 * kWaves, C::total, stream>>>(a);
   return launched();
 }
 
 template <class E, int KD>
 int backward(DeltaArgs& a, hipStream_t stream) {
-  constexpr int kT = out_terms<E>(), lds = ChunkLds<E, KD, kT, kT>::size, glds = GradLds<E, KD>::size;
-  int st = allow_lds(delta_chunks_bwd<E, KD>, lds);
+  constexpr int kT = out_terms<E>(), kWaves = walk_waves<E>(), glds = GradLds<E, KD>::size;
+  using C = ChunkLds<E, KD, kT, kT, kWaves>;
+  const auto walk = delta_chunks_bwd<E, KD, kWaves>;
+  int st = allow_lds(walk, C::total);
   if (st != FPSCAN_OK) return st;
-  const int waves = walk_waves(a);
-  const unsigned grid = walk_grid(a, waves);
-  delta_chunks_bwd<E, KD><<<grid, 64 * waves, lds, stream>>>(a);
+  const unsigned grid = walk_grid(a, kWaves);
+  walk<<<grid, 128 * kWaves, C::total, stream>>>(a);
   if ((st = launched()) != FPSCAN_OK) return st;
   const auto kernel = a.R > 1 ? delta_grads<E, KD, true> : delta_grads<E, KD, false>;
   if ((st = allow_lds(kernel, glds)) != FPSCAN_OK) return st;
