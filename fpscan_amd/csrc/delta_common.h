@@ -40,16 +40,25 @@ template <> struct InputPlanes<BF16> { static constexpr int n = 1; };
 template <> struct InputPlanes<F16> { static constexpr int n = 2; };
 template <> struct InputPlanes<F32> { static constexpr int n = 3; };
 
-// x as kPlanes bf16 planes.
+// x as kPlanes bf16 planes. (The rounded values are taken back out of the packed pairs by hand: the
+// compiler would convert each of them a second time.)
 template <int kPlanes>
 __device__ __forceinline__ void split(f32x8 x, bf16x8 (&p)[kPlanes]) {
 #pragma unroll
   for (int i = 0; i < kPlanes; ++i) {
-    p[i] = __builtin_convertvector(x, bf16x8);
-    if (i + 1 < kPlanes) x -= __builtin_convertvector(p[i], f32x8);
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = __builtin_bit_cast(unsigned int,
+                                __builtin_convertvector(f32x2{x[2 * j], x[2 * j + 1]}, bf16x2));
+      if (i + 1 < kPlanes) {
+        x[2 * j] -= __uint_as_float(w[j] << 16);
+        x[2 * j + 1] -= __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+    p[i] = __builtin_bit_cast(bf16x8, w);
   }
 }
-
 template <int kPlanes>
 __device__ __forceinline__ void split(f32x4 x, bf16x4 (&p)[kPlanes]) {
 #pragma unroll
@@ -93,6 +102,28 @@ __device__ __forceinline__ void mma_tiles(const bf16x8 (&a)[kTiles][NA], const b
 // Keeps the order of loads and products as written: a wave alone on its SIMD has nothing but its own
 // products to cover the latency of its loads, and the compiler would put each load before its use.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Asks for the instructions since the last in_order() to be issued as kProducts times one matrix
+// product, kAlu vector instructions and one LDS load: a product takes 16 cycles of its unit, in which
+// the wave may issue three others.
+template <int kProducts, int kAlu, int kLoads>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < kProducts; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if (kLoads) __builtin_amdgcn_sched_group_barrier(0x100, kLoads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, kAlu, 0);
+  }
+  in_order();
+}
+
+// Plane products of kTerms terms.
+constexpr int products(int na, int nb, int terms) {
+  int n = 0;
+  for (int i = 0; i < na; ++i)
+    for (int j = 0; j < nb; ++j) n += i + j < terms;
+  return n;
+}
 
 // Byte offset of lane (row i of 16, group q of 4 columns) in a 1 KiB block. The bit that moves row
 // i by eight for odd q spreads the transposing loads over all banks: their 16 lanes of a group read

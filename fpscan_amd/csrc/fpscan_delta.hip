@@ -232,24 +232,29 @@ __device__ __forceinline__ float block_scale(float most) {
   return __uint_as_float((unsigned)(up + 127) << 23);
 }
 
+// `live`: whether the block exists (its stores are dropped otherwise, without a branch).
 template <class E, int kPairs>
-__device__ __forceinline__ void keep(char* to, float* scale, const f32x4 (&x)[2 * kPairs], int lane) {
+__device__ __forceinline__ void keep(char* base, float* scales, int64_t block, bool live,
+                                     const f32x4 (&x)[2 * kPairs], int lane) {
+  constexpr int kBytes = kPairs * 512 * kept_size<E>();
+  const Rsrc r = row_rsrc(base, block, kBytes, live ? kBytes : 0);
   if constexpr (kept_size<E>() == 2) {
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2 * kPairs; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(x[i][r]));
+      for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[i][j]));
     const float up = block_scale(wave_max(most));
 #pragma unroll
     for (int i = 0; i < kPairs; ++i)
-      reinterpret_cast<f16x8*>(to)[i * 64 + lane] =
-          __builtin_convertvector(join(x[2 * i], x[2 * i + 1]) * up, f16x8);
-    if (lane == 0) *scale = 1.0f / up;
+      bst16<0>(r, (i * 64 + lane) * 16,
+               __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * i], x[2 * i + 1]) * up, f16x8)));
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(1.0f / up),
+                                          row_rsrc(scales, block, 4, live ? 4 : 0), lane * 4, 0, 0);
   } else {
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i)
-      reinterpret_cast<f32x8*>(to)[i * 64 + lane] = join(x[2 * i], x[2 * i + 1]);
+    for (int i = 0; i < 2 * kPairs; ++i)
+      bst16<0>(r, ((i >> 1) * 64 + lane) * 32 + (i & 1) * 16, __builtin_bit_cast(u32x4, x[i]));
   }
 }
 
@@ -339,7 +344,7 @@ struct Copies {
 };
 
 // The waves that bring chunks: `value` is V or dO, chunks first, first + step .. of `count`.
-template <class E, int KD, int kTerms, int kOut, int kWaves>
+template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring>
 __device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const Heads& value, int64_t bh,
                                       int64_t b, int64_t h, int64_t hk, int col0, int w, int64_t first,
                                       int64_t step) {
@@ -348,10 +353,10 @@ __device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const H
   for (int64_t i = 0, c = first; i < a.chunks; ++i, c += step) {
     const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
     const int rows = rows_left(a.L, t0);
-    RowBlocks<E, KD, kWaves> k, q;
-    RowBlocks<E, C::kCols, kWaves> v;
-    Copies<6 * kTerms, kWaves> n;
-    Copies<6 * kOut, kWaves> m;
+    RowBlocks<E, KD, kBring> k, q;
+    RowBlocks<E, C::kCols, kBring> v;
+    Copies<6 * kTerms, kBring> n;
+    Copies<6 * kOut, kBring> m;
     f32x4 gb = {};
     k.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
     n.load(a.n + ch * kTerms * kTriBytes, w);
@@ -501,8 +506,8 @@ __device__ __forceinline__ Place place_of(const DeltaArgs& a) {
   return {bh, b, h, h / a.R, (int)(id / 8 % a.vblocks) * 16 * kWaves};
 }
 
-template <class E, int KD, int kTerms, bool kSave, int kWaves>
-__global__ __launch_bounds__(128 * kWaves) void delta_chunks(DeltaArgs a) {
+template <class E, int KD, int kTerms, bool kSave, int kWaves, int kBring>
+__global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs a) {
   constexpr int kOut = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
   using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
   extern __shared__ __attribute__((aligned(16))) char buffers[];
@@ -510,7 +515,7 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks(DeltaArgs a) {
   if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
   if (w >= kWaves) {
-    bring<E, KD, kTerms, kOut, kWaves>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves, 0, 1);
+    bring<E, KD, kTerms, kOut, kWaves, kBring>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves, 0, 1);
     return;
   }
   const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2, col = p.col0 + key_col(w, li);
@@ -529,8 +534,7 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks(DeltaArgs a) {
   for (int64_t c = 0; c < a.chunks; ++c) {
     const int64_t ch = p.bh * a.chunks + c, t0 = c * kChunk;
     const char* const lds = buffers + (C::kBuffers == 2 && (c & 1) ? C::size : 0);
-    // operands of the next steps on their way while a step's products run
-    constexpr int kAhead = NI == 1 ? 2 : 1;
+    // operands of the next step are on their way while a step's products run
     auto keys_at = [&](int step, bf16x8 (&f)[4][NI]) {  // K and Q in turn, 32 key columns a step
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
@@ -549,89 +553,88 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks(DeltaArgs a) {
     auto row_of = [&](int which, int mt) {
       return *reinterpret_cast<const f32x4*>(lds + which + (16 * mt + 4 * lg) * 4);
     };
-    constexpr int kSteps = 2 * C::kBlocks, kUpdates = KT / 2;
-    f32x4 ks[4] = {}, o[4] = {};
-    bf16x8 ring[kAhead + 1][4][NI], nf[6][kTerms], vp[2][NI], sp[kTerms];
+    constexpr int kUpdates = KT / 2, kS = 4 * products(NI, kTerms, kTerms),
+                  kO = 4 * products(NI, kOut, kOut);
+    f32x4 ks[4] = {}, o[4] = {}, x[4], u[4], y[4] = {};
+    bf16x8 ring[2][4][NI], sp[C::kBlocks][kTerms];
+    // K S, with the planes of the state a step ahead
+    keys_at(0, ring[0]);
+    split(join(S[0], S[1]), sp[0]);
+    in_order();
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) keys_at(i, ring[i]);
-    if (kSave && tile < tiles)
-      keep<E, KT / 2>(a.s + (ch * tiles + tile) * KD * 16 * kept_size<E>(), a.ss + ch * tiles + tile,
-                      S, lane);
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      if (i + kAhead < kSteps) {
-        keys_at(i + kAhead, ring[(i + kAhead) % (kAhead + 1)]);
-      } else if (i + 1 == kSteps) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
-          cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
-        }
-        triangle(lds + C::n, lane, nf);
-      }
-      if (i % 2 == 0) split(join(S[i], S[i + 1]), sp);
-      in_order();
-      if (i % 2 == 0)
-        mma_tiles<kTerms>(ring[i % (kAhead + 1)], sp, ks);
-      else
-        mma_tiles<kOut>(ring[i % (kAhead + 1)], sp, o);
-      in_order();
+    for (int i = 0; i < C::kBlocks; ++i) {
+      keys_at(i + 1 < C::kBlocks ? 2 * i + 2 : 1, ring[(i + 1) & 1]);
+      if (i + 1 < C::kBlocks) split(join(S[2 * i + 2], S[2 * i + 3]), sp[i + 1]);
+      mma_tiles<kTerms>(ring[i & 1], sp[i], ks);
+      interleave<kS, 4, 1>();
     }
-    // x: V -> R -> E; u: beta R -> U
-    f32x4 x[4], u[4], y[4] = {};
+    // Q S, meanwhile V -> R (x) and the planes of beta R
+    bf16x8 nf[6][kTerms], up[2][kTerms], vp[2][NI];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
+      cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+    }
+#pragma unroll
+    for (int i = 0; i < C::kBlocks; ++i) {
+      if (i + 1 < C::kBlocks)
+        keys_at(2 * i + 3, ring[(i + 1 + C::kBlocks) & 1]);
+      else if (kTerms == 2)
+        triangle(lds + C::n, lane, nf);
+      mma_tiles<kOut>(ring[(i + C::kBlocks) & 1], sp[i], o);
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const f32x8 v = whole(vp[s]);
       x[2 * s] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
       x[2 * s + 1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+#pragma unroll
+      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
+        x[mt] -= row_of(C::gam, mt) * ks[mt];
+        u[mt] = row_of(C::beta, mt) * x[mt];
+      }
+      split(join(u[2 * s], u[2 * s + 1]), up[s]);
     }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const f32x4 gam = row_of(C::gam, mt);
-      x[mt] -= gam * ks[mt];
-      u[mt] = row_of(C::beta, mt) * x[mt];
-      o[mt] *= gam * a.scale;
-    }
-    bf16x8 up[2][kTerms];
-    split(join(u[0], u[1]), up[0]);
-    split(join(u[2], u[3]), up[1]);
-    in_order();
-    mma_triangle<kTerms>(nf, up, y);
-    in_order();
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) steps_at(i, ring[i]);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      x[mt] -= y[mt];
-      u[mt] = row_of(C::beta, mt) * x[mt];
-    }
-    bf16x8 uo[2][kOut];
-    split(join(u[0], u[1]), uo[0]);
-    split(join(u[2], u[3]), uo[1]);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) u[mt] *= row_of(C::end, mt);
-    split(join(u[0], u[1]), up[0]);
-    split(join(u[2], u[3]), up[1]);
-    const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+    interleave<C::kBlocks * kO, 4, 1>();
+    // N (beta R), meanwhile what of the state and the output needs no more than a factor
+    if (kTerms > 2) triangle(lds + C::n, lane, nf);  // three planes are too many registers before
     bf16x8 mf[6][kOut];
+    const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+    if (kSave) keep<E, KT / 2>(a.s, a.ss, ch * tiles + tile, tile < tiles, S, lane);
 #pragma unroll
     for (int t = 0; t < KT; ++t) S[t] *= last;
 #pragma unroll
-    for (int i = 0; i < kUpdates; ++i) {
-      if (i + kAhead < kUpdates)
-        steps_at(i + kAhead, ring[(i + kAhead) % (kAhead + 1)]);
-      else if (i + 1 == kUpdates)
-        triangle(lds + C::m, lane, mf);
-      in_order();
-      mma_tiles<kTerms>(ring[i % (kAhead + 1)], up[i & 1], &S[4 * (i / 2)]);
-      in_order();
+    for (int mt = 0; mt < 4; ++mt) o[mt] *= row_of(C::gam, mt) * a.scale;
+    triangle(lds + C::m, lane, mf);
+    mma_triangle<kTerms>(nf, up, y);
+    interleave<6 * products(kTerms, kTerms, kTerms), 4, 1>();
+    // U, its planes and those of what it adds to the state
+    bf16x8 uo[2][kOut];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
+        x[mt] -= y[mt];
+        u[mt] = row_of(C::beta, mt) * x[mt];
+      }
+      split(join(u[2 * s], u[2 * s + 1]), uo[s]);
+#pragma unroll
+      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) u[mt] *= row_of(C::end, mt);
+      split(join(u[2 * s], u[2 * s + 1]), up[s]);
     }
+    steps_at(0, ring[0]);
     mma_triangle<kOut>(mf, uo, o);
-    if (kSave && tile < tiles)
-      keep<E, 2>(a.e + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.es + ch * tiles + tile, x,
-                 lane);
+    in_order();
+    // the state, meanwhile the output
+    if (kSave) keep<E, 2>(a.e, a.es, ch * tiles + tile, tile < tiles, x, lane);
     write_columns<E>(a, p.b, p.h, t0, rows_left(a.L, t0), p.col0, w, buffers + C::turn + w * C::kTurn, o,
                      lane);
+#pragma unroll
+    for (int i = 0; i < kUpdates; ++i) {
+      if (i + 1 < kUpdates) steps_at(i + 1, ring[(i + 1) & 1]);
+      mma_tiles<kTerms>(ring[i & 1], up[i & 1], &S[4 * (i / 2)]);
+    }
+    interleave<kUpdates * kS, 3, 1>();
     if (c + 1 < a.chunks) {
       if (C::kBuffers == 1) lds_barrier();  // this chunk is read
       lds_barrier();                        // the next one is there
@@ -649,8 +652,8 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks(DeltaArgs a) {
 
 // Backward walk, the same way: a wave owns 16 columns of dS' and gives dV, and for the gradients of q
 // and k the dS' and Y of every chunk.
-template <class E, int KD, int kWaves>
-__global__ __launch_bounds__(128 * kWaves) void delta_chunks_bwd(DeltaArgs a) {
+template <class E, int KD, int kWaves, int kBring>
+__global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(DeltaArgs a) {
   constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
   using C = ChunkLds<E, KD, kT, kT, kWaves>;
   extern __shared__ __attribute__((aligned(16))) char buffers[];
@@ -658,7 +661,7 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks_bwd(DeltaArgs a) {
   if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), lg = lane >> 4;
   if (w >= kWaves) {
-    bring<E, KD, kT, kT, kWaves>(buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves,
+    bring<E, KD, kT, kT, kWaves, kBring>(buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves,
                                  a.chunks - 1, -1);
     return;
   }
@@ -669,7 +672,6 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks_bwd(DeltaArgs a) {
   for (int64_t i = 0; i < a.chunks; ++i) {
     const int64_t c = a.chunks - 1 - i, ch = p.bh * a.chunks + c, t0 = c * kChunk;
     const char* const lds = buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0);
-    constexpr int kAhead = NI == 1 ? 2 : 1, kSteps = C::kBlocks, kUpdates = KT;
     auto keys_at = [&](int step, bf16x8 (&f)[4][NI]) {
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
@@ -686,76 +688,86 @@ __global__ __launch_bounds__(128 * kWaves) void delta_chunks_bwd(DeltaArgs a) {
     auto row_of = [&](int which, int mt) {
       return *reinterpret_cast<const f32x4*>(lds + which + (16 * mt + 4 * lg) * 4);
     };
+    constexpr int kS = 4 * products(NI, kT, kT);
     f32x4 u[4] = {}, y[4] = {};
-    bf16x8 ring[kAhead + 1][4][NI], nf[6][kT], vp[2][NI], sp[kT];
+    bf16x8 ring[2][4][NI], mf[6][kT], nf[6][kT], vp[2][NI], sp[2][kT];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
       cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
     }
-    triangle_t(lds + C::m, lane, nf);
-    if (tile < tiles)
-      keep<E, KT / 2>(a.ds + (ch * tiles + tile) * KD * 16 * kept_size<E>(), a.dss + ch * tiles + tile,
-                      dS, lane);
+    triangle_t(lds + C::m, lane, mf);
     in_order();
+    // M^T dO, meanwhile the planes of dS'
+    keys_at(0, ring[0]);
+    split(join(dS[0], dS[1]), sp[0]);
+    keep<E, KT / 2>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
+    mma_triangle_t<kT>(mf, vp, y);
+    interleave<6 * products(kT, NI, kT), 4, 1>();
+    // K dS'
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) keys_at(j, ring[j]);
-    mma_triangle_t<kT>(nf, vp, y);
-    in_order();
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      if (j + kAhead < kSteps)
-        keys_at(j + kAhead, ring[(j + kAhead) % (kAhead + 1)]);
-      else if (j + 1 == kSteps)
-        triangle_t(lds + C::n, lane, nf);
-      split(join(dS[2 * j], dS[2 * j + 1]), sp);
-      in_order();
-      mma_tiles<kT>(ring[j % (kAhead + 1)], sp, u);
-      in_order();
+    for (int j = 0; j < C::kBlocks; ++j) {
+      if (j + 1 < C::kBlocks) {
+        keys_at(j + 1, ring[(j + 1) & 1]);
+        split(join(dS[2 * j + 2], dS[2 * j + 3]), sp[(j + 1) & 1]);
+      } else {
+        steps_at(0, ring[(j + 1) & 1]);
+      }
+      mma_tiles<kT>(ring[j & 1], sp[j & 1], u);
+      interleave<kS, 4, 1>();
     }
     bf16x8 up[2][kT], xp[2][kT];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      u[mt] = y[mt] + u[mt] * row_of(C::end, mt);
-      y[mt] = row_of(C::beta, mt) * u[mt];
-    }
-    split(join(y[0], y[1]), up[0]);
-    split(join(y[2], y[3]), up[1]);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{};
-    in_order();
-    mma_triangle_t<kT>(nf, up, y);
-    in_order();
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) steps_at(j, ring[j]);
-    // u: Y; y: -exp(G) dV; xp: scale exp(G) dO
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      u[mt] -= y[mt];
-      y[mt] = u[mt] * (row_of(C::beta, mt) * -row_of(C::gam, mt));
-    }
-    split(join(y[0], y[1]), up[0]);
-    split(join(y[2], y[3]), up[1]);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
       split(whole(vp[s]) * (join(row_of(C::gam, 2 * s), row_of(C::gam, 2 * s + 1)) * a.scale), xp[s]);
     const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
 #pragma unroll
     for (int t = 0; t < KT; ++t) dS[t] *= last;
+    in_order();
+    // Q^T (scale exp(G) dO), meanwhile dU (u) and the planes of beta dU
 #pragma unroll
-    for (int j = 0; j < kUpdates; ++j) {
-      if (j + kAhead < kUpdates) steps_at(j + kAhead, ring[(j + kAhead) % (kAhead + 1)]);
-      in_order();
-      mma_tiles<kT>(ring[j % (kAhead + 1)], j < KT / 2 ? xp[j & 1] : up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
-      in_order();
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
+        u[mt] = y[mt] + u[mt] * row_of(C::end, mt);
+        y[mt] = row_of(C::beta, mt) * u[mt];
+      }
+      split(join(y[2 * s], y[2 * s + 1]), up[s]);
     }
-    if (tile < tiles)
-      keep<E, 2>(a.y + (ch * tiles + tile) * kChunk * 16 * kept_size<E>(), a.ys + ch * tiles + tile, u,
-                 lane);
+#pragma unroll
+    for (int j = 0; j < KT / 2; ++j) {
+      steps_at(j + 1, ring[(C::kBlocks + j + 1) & 1]);
+      mma_tiles<kT>(ring[(C::kBlocks + j) & 1], xp[j & 1], &dS[4 * (j / 2)]);
+    }
+    triangle_t(lds + C::n, lane, nf);
+    interleave<KT / 2 * kS, 4, 2>();
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{};
+    mma_triangle_t<kT>(nf, up, y);
+    in_order();
+    // u: Y; y: -exp(G) dV
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
+        u[mt] -= y[mt];
+        y[mt] = u[mt] * (row_of(C::beta, mt) * -row_of(C::gam, mt));
+      }
+      split(join(y[2 * s], y[2 * s + 1]), up[s]);
+    }
+    in_order();
+    // K^T (exp(G) dV), meanwhile dV
+    keep<E, 2>(a.y, a.ys, ch * tiles + tile, tile < tiles, u, lane);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) u[mt] *= row_of(C::beta, mt);
     write_columns<E>(a, p.b, p.h, t0, rows_left(a.L, t0), p.col0, w, buffers + C::turn + w * C::kTurn, u,
                      lane);
+#pragma unroll
+    for (int j = KT / 2; j < KT; ++j) {
+      if (j + 1 < KT) steps_at(j + 1, ring[(C::kBlocks + j + 1) & 1]);
+      mma_tiles<kT>(ring[(C::kBlocks + j) & 1], up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
+    }
+    interleave<KT / 2 * kS, 3, 1>();
     if (c > 0) {
       if (C::kBuffers == 1) lds_barrier();
       lds_barrier();
@@ -1306,31 +1318,33 @@ unsigned walk_grid(DeltaArgs& a, int waves) {
 
 // Computing waves of a walk's workgroup.
 template <class E>
-constexpr int walk_waves() { return InputPlanes<E>::n == 3 ? 2 : 4; }
+constexpr int walk_waves() { return 2; }
+template <class E>
+constexpr int bring_waves() { return InputPlanes<E>::n == 3 ? 2 : 4; }
 
 template <class E, int KD, int kTerms, bool kSave>
 int walk_forward(DeltaArgs& a, hipStream_t stream) {
-  constexpr int kOut = out_terms<E>(), kWaves = walk_waves<E>();
+  constexpr int kOut = out_terms<E>(), kWaves = walk_waves<E>(), kBring = bring_waves<E>();
   using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
   delta_prep<E, KD, kTerms, kOut><<<(unsigned)(a.heads_total * a.chunks), 256, 0, stream>>>(a);
   int st = launched();
   if (st != FPSCAN_OK) return st;
-  const auto walk = delta_chunks<E, KD, kTerms, kSave, kWaves>;
+  const auto walk = delta_chunks<E, KD, kTerms, kSave, kWaves, kBring>;
   if ((st = allow_lds(walk, C::total)) != FPSCAN_OK) return st;
   const unsigned grid = walk_grid(a, kWaves);
-  walk<<<grid, 128 * kWaves, C::total, stream>>>(a);
+  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
   return launched();
 }
 
 template <class E, int KD>
 int backward(DeltaArgs& a, hipStream_t stream) {
-  constexpr int kT = out_terms<E>(), kWaves = walk_waves<E>(), glds = GradLds<E, KD>::size;
+  constexpr int kT = out_terms<E>(), kWaves = walk_waves<E>(), kBring = bring_waves<E>(), glds = GradLds<E, KD>::size;
   using C = ChunkLds<E, KD, kT, kT, kWaves>;
-  const auto walk = delta_chunks_bwd<E, KD, kWaves>;
+  const auto walk = delta_chunks_bwd<E, KD, kWaves, kBring>;
   int st = allow_lds(walk, C::total);
   if (st != FPSCAN_OK) return st;
   const unsigned grid = walk_grid(a, kWaves);
-  walk<<<grid, 128 * kWaves, C::total, stream>>>(a);
+  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
   if ((st = launched()) != FPSCAN_OK) return st;
   const auto kernel = a.R > 1 ? delta_grads<E, KD, true> : delta_grads<E, KD, false>;
   if ((st = allow_lds(kernel, glds)) != FPSCAN_OK) return st;
