@@ -104,17 +104,30 @@ __device__ __forceinline__ void mma_tiles(const bf16x8 (&a)[kTiles][NA], const b
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // Asks for the instructions since the last in_order() to be issued as kProducts times one matrix
-// product, kAlu vector instructions and one LDS load: a product takes 16 cycles of its unit, in which
-// the wave may issue three others.
-template <int kProducts, int kAlu, int kLoads>
+// product and kAlu vector instructions, the LDS loads (which are for the next such step) after the
+// first ones: a product takes 16 cycles of its unit, in which the wave may issue three others, and an
+// LDS load comes back after some eight products.
+template <int kProducts, int kAlu>
 __device__ __forceinline__ void interleave() {
 #pragma unroll
   for (int i = 0; i < kProducts; ++i) {
     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    if (kLoads) __builtin_amdgcn_sched_group_barrier(0x100, kLoads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
     __builtin_amdgcn_sched_group_barrier(0x2, kAlu, 0);
   }
   in_order();
+}
+
+// Values that are to be there before the next in_order(): without memory to order it by, the compiler
+// would compute them where they are used.
+template <class T>
+__device__ __forceinline__ void settle(T& x) {
+  asm volatile("" : "+v"(x));
+}
+template <class T, int N>
+__device__ __forceinline__ void settle(T (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) settle(x[i]);
 }
 
 // Plane products of kTerms terms.

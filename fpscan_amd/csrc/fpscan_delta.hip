@@ -323,49 +323,50 @@ struct RowBlocks {
   }
 };
 
-// Whole KiB copied as they are, shared among kWaves waves.
+// Whole KiB copied as they are, shared among kWaves waves (the last one more than once where they do
+// not divide: no wave's loads then depend on a branch).
 template <int kCount, int kWaves>
 struct Copies {
   static constexpr int n = (kCount + kWaves - 1) / kWaves;
   u32x4 x[n];
 
+  static __device__ __forceinline__ int at(int i, int w) {
+    const int k = w + i * kWaves;
+    return (kCount % kWaves == 0 || k < kCount ? k : kCount - 1) * 1024;
+  }
   __device__ __forceinline__ void load(const char* from, int w) {
 #pragma unroll
-    for (int i = 0; i < n; ++i)
-      if (kCount % kWaves == 0 || w + i * kWaves < kCount)
-        x[i] = reinterpret_cast<const u32x4*>(from + (w + i * kWaves) * 1024)[threadIdx.x & 63];
+    for (int i = 0; i < n; ++i) x[i] = reinterpret_cast<const u32x4*>(from + at(i, w))[threadIdx.x & 63];
   }
   __device__ __forceinline__ void store(char* to, int w) const {
 #pragma unroll
-    for (int i = 0; i < n; ++i)
-      if (kCount % kWaves == 0 || w + i * kWaves < kCount)
-        reinterpret_cast<u32x4*>(to + (w + i * kWaves) * 1024)[threadIdx.x & 63] = x[i];
+    for (int i = 0; i < n; ++i) reinterpret_cast<u32x4*>(to + at(i, w))[threadIdx.x & 63] = x[i];
   }
 };
 
-// The waves that bring chunks: `value` is V or dO, chunks first, first + step .. of `count`.
+// A chunk on its way from memory to LDS, in the registers of kBring waves. `value` is V or dO.
 template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring>
-__device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const Heads& value, int64_t bh,
-                                      int64_t b, int64_t h, int64_t hk, int col0, int w, int64_t first,
-                                      int64_t step) {
+struct Brought {
   using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
-  const int lane = threadIdx.x & 63;
-  for (int64_t i = 0, c = first; i < a.chunks; ++i, c += step) {
+  RowBlocks<E, KD, kBring> k, q;
+  RowBlocks<E, C::kCols, kBring> v;
+  Copies<6 * kTerms, kBring> n;
+  Copies<6 * kOut, kBring> m;
+  f32x4 gb;
+
+  __device__ __forceinline__ void load(const DeltaArgs& a, const Heads& value, int64_t bh, int64_t b,
+                                       int64_t h, int64_t hk, int col0, int w, int64_t c) {
     const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
     const int rows = rows_left(a.L, t0);
-    RowBlocks<E, KD, kBring> k, q;
-    RowBlocks<E, C::kCols, kBring> v;
-    Copies<6 * kTerms, kBring> n;
-    Copies<6 * kOut, kBring> m;
-    f32x4 gb = {};
     k.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
     n.load(a.n + ch * kTerms * kTriBytes, w);
     v.load(value, b, h, t0, rows, a.Dv, col0, w);
     q.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
     m.load(a.m + ch * kOut * kTriBytes, w);
-    if (w == 0) gb = reinterpret_cast<const f32x4*>(a.gb)[ch * kChunk + lane];
-    if (C::kBuffers == 1 && i > 0) lds_barrier();  // the chunk before is read
-    char* const lds = buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0);
+    gb = reinterpret_cast<const f32x4*>(a.gb)[ch * kChunk + (threadIdx.x & 63)];
+  }
+  __device__ __forceinline__ void store(char* lds, int w) const {
+    const int lane = threadIdx.x & 63;
     k.store(lds + C::k, w);
     n.store(lds + C::n, w);
     v.store(lds + C::v, w);
@@ -377,7 +378,33 @@ __device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const H
       reinterpret_cast<float*>(lds + C::end)[lane] = expf((hi - gb[0]) + (lo - gb[1]));
       reinterpret_cast<float*>(lds + C::beta)[lane] = gb[2];
     }
+  }
+};
+
+// The waves that bring chunks first, first + step .. to LDS: a chunk's loads are under way while the
+// one before is waited for and stored (past the last, it is loaded again and dropped).
+template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring>
+__device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const Heads& value, int64_t bh,
+                                      int64_t b, int64_t h, int64_t hk, int col0, int w, int64_t first,
+                                      int64_t step) {
+  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
+  Brought<E, KD, kTerms, kOut, kWaves, kBring> even, odd;
+  const int64_t end = a.chunks - 1;
+  auto chunk = [&](int64_t i) { return first + step * (i < end ? i : end); };
+  auto pass = [&](const auto& x, int64_t i) {
+    if (C::kBuffers == 1 && i > 0) lds_barrier();  // the chunk before is read
+    x.store(buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0), w);
     lds_barrier();
+  };
+  even.load(a, value, bh, b, h, hk, col0, w, chunk(0));
+  for (int64_t i = 0; i < a.chunks; i += 2) {
+    odd.load(a, value, bh, b, h, hk, col0, w, chunk(i + 1));
+    in_order();
+    pass(even, i);
+    if (i + 1 >= a.chunks) break;
+    even.load(a, value, bh, b, h, hk, col0, w, chunk(i + 2));
+    in_order();
+    pass(odd, i + 1);
   }
 }
 
@@ -455,25 +482,30 @@ __device__ __forceinline__ void triangle_t(const char* from, int lane, bf16x8 (&
               mt, lane, f[upper_block(mt, s)]);
 }
 
-// A wave's 16 columns of 64 result rows to the contiguous (batch, seqlen, heads, value_dim) tensor:
-// the half types by way of `turn`, four columns a lane and store.
+// A wave's 16 columns of 64 result rows to the contiguous (batch, seqlen, heads, value_dim) tensor.
+// The half types by way of LDS: turn_in, and then turn_out stores four columns a lane. fp32 as it is.
 template <class E>
-__device__ __forceinline__ void write_columns(const DeltaArgs& a, int64_t b, int64_t h, int64_t t0,
-                                              int rows, int col0, int tile, char* turn,
-                                              const f32x4 (&x)[4], int lane) {
-  const int li = lane & 15, lg = lane >> 4, st = a.H * a.Dv * E::kSize;
-  const Rsrc r = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
-                          ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+__device__ __forceinline__ void turn_in(char* turn, const f32x4 (&x)[4], int lane) {
   if constexpr (E::kSize == 2) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
+      const f32x8 v = join(x[2 * s], x[2 * s + 1]);
       u32x4 p;
       if constexpr (InputPlanes<E>::n == 1)
-        p = __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * s], x[2 * s + 1]), bf16x8));
+        p = __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
       else
-        p = __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * s], x[2 * s + 1]), f16x8));
-      *reinterpret_cast<u32x4*>(turn + s * 1024 + frag_lane(li, lg)) = p;
+        p = __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8));
+      *reinterpret_cast<u32x4*>(turn + s * 1024 + frag_lane(lane & 15, lane >> 4)) = p;
     }
+  }
+}
+template <class E>
+__device__ __forceinline__ void turn_out(const DeltaArgs& a, int64_t b, int64_t h, int64_t t0, int col0,
+                                         int tile, const char* turn, const f32x4 (&x)[4], int lane) {
+  const int li = lane & 15, lg = lane >> 4, st = a.H * a.Dv * E::kSize, rows = rows_left(a.L, t0);
+  const Rsrc r = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
+                          ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+  if constexpr (E::kSize == 2) {
     const int d = col0 + key_col(tile, 4 * lg);
     typedef __attribute__((address_space(3))) s16x4* ldsp;
 #pragma unroll
@@ -555,86 +587,115 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
     };
     constexpr int kUpdates = KT / 2, kS = 4 * products(NI, kTerms, kTerms),
                   kO = 4 * products(NI, kOut, kOut);
+    // two planes of one: registers for the triangles' operands a phase ahead
+    constexpr bool kRoom = NI == 1 && kTerms == 2;
     f32x4 ks[4] = {}, o[4] = {}, x[4], u[4], y[4] = {};
     bf16x8 ring[2][4][NI], sp[C::kBlocks][kTerms];
+    char* const turn = buffers + C::turn + w * C::kTurn;
     // K S, with the planes of the state a step ahead
     keys_at(0, ring[0]);
     split(join(S[0], S[1]), sp[0]);
+    bf16x8 vp[2][NI];
     in_order();
 #pragma unroll
     for (int i = 0; i < C::kBlocks; ++i) {
       keys_at(i + 1 < C::kBlocks ? 2 * i + 2 : 1, ring[(i + 1) & 1]);
-      if (i + 1 < C::kBlocks) split(join(S[2 * i + 2], S[2 * i + 3]), sp[i + 1]);
+      if (i + 1 < C::kBlocks) {
+        split(join(S[2 * i + 2], S[2 * i + 3]), sp[i + 1]);
+        settle(sp[i + 1]);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
+          cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+        }
+      }
       mma_tiles<kTerms>(ring[i & 1], sp[i], ks);
-      interleave<kS, 4, 1>();
+      interleave<kS, 4>();
     }
     // Q S, meanwhile V -> R (x) and the planes of beta R
-    bf16x8 nf[6][kTerms], up[2][kTerms], vp[2][NI];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
-      cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
-    }
+    bf16x8 nf[6][kTerms], up[2][kTerms];
+    f32x4 gam[4], beta[4], end[4];
 #pragma unroll
     for (int i = 0; i < C::kBlocks; ++i) {
       if (i + 1 < C::kBlocks)
         keys_at(2 * i + 3, ring[(i + 1 + C::kBlocks) & 1]);
-      else if (kTerms == 2)
+      else if (kRoom)
         triangle(lds + C::n, lane, nf);
-      mma_tiles<kOut>(ring[(i + C::kBlocks) & 1], sp[i], o);
-    }
+      if (i == 0)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const f32x8 v = whole(vp[s]);
-      x[2 * s] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-      x[2 * s + 1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        for (int mt = 0; mt < 4; ++mt) {
+          gam[mt] = row_of(C::gam, mt);
+          beta[mt] = row_of(C::beta, mt);
+        }
+      constexpr int kFirst = C::kBlocks == 4 ? 1 : 0;
+      if (i >= kFirst && i < kFirst + 2) {
+        const int s = i - kFirst;
+        const f32x8 v = whole(vp[s]);
+        x[2 * s] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+        x[2 * s + 1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
 #pragma unroll
-      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
-        x[mt] -= row_of(C::gam, mt) * ks[mt];
-        u[mt] = row_of(C::beta, mt) * x[mt];
+        for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
+          x[mt] -= gam[mt] * ks[mt];
+          u[mt] = beta[mt] * x[mt];
+        }
+        split(join(u[2 * s], u[2 * s + 1]), up[s]);
+        settle(up[s]);
       }
-      split(join(u[2 * s], u[2 * s + 1]), up[s]);
+      mma_tiles<kOut>(ring[(i + C::kBlocks) & 1], sp[i], o);
+      interleave<kO, 5>();
     }
-    interleave<C::kBlocks * kO, 4, 1>();
     // N (beta R), meanwhile what of the state and the output needs no more than a factor
-    if (kTerms > 2) triangle(lds + C::n, lane, nf);  // three planes are too many registers before
+    if (!kRoom) triangle(lds + C::n, lane, nf);
     bf16x8 mf[6][kOut];
     const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
     if (kSave) keep<E, KT / 2>(a.s, a.ss, ch * tiles + tile, tile < tiles, S, lane);
 #pragma unroll
     for (int t = 0; t < KT; ++t) S[t] *= last;
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) o[mt] *= row_of(C::gam, mt) * a.scale;
-    triangle(lds + C::m, lane, mf);
+    for (int mt = 0; mt < 4; ++mt) o[mt] *= gam[mt] * a.scale;
+    settle(S);
+    settle(o);
+    if (kRoom) triangle(lds + C::m, lane, mf);
     mma_triangle<kTerms>(nf, up, y);
-    interleave<6 * products(kTerms, kTerms, kTerms), 4, 1>();
+    interleave<6 * products(kTerms, kTerms, kTerms), 4>();
     // U, its planes and those of what it adds to the state
     bf16x8 uo[2][kOut];
+    if (!kRoom) triangle(lds + C::m, lane, mf);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) end[mt] = row_of(C::end, mt);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
         x[mt] -= y[mt];
-        u[mt] = row_of(C::beta, mt) * x[mt];
+        u[mt] = beta[mt] * x[mt];
       }
       split(join(u[2 * s], u[2 * s + 1]), uo[s]);
-#pragma unroll
-      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) u[mt] *= row_of(C::end, mt);
-      split(join(u[2 * s], u[2 * s + 1]), up[s]);
     }
-    steps_at(0, ring[0]);
-    mma_triangle<kOut>(mf, uo, o);
+    settle(uo[0]);
+    settle(uo[1]);
     in_order();
+    // M U, meanwhile the planes for the state
+    steps_at(0, ring[0]);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      split(join(u[2 * s] * end[2 * s], u[2 * s + 1] * end[2 * s + 1]), up[s]);
+      settle(up[s]);
+    }
+    mma_triangle<kOut>(mf, uo, o);
+    interleave<6 * products(kOut, kOut, kOut), 4>();
     // the state, meanwhile the output
-    if (kSave) keep<E, 2>(a.e, a.es, ch * tiles + tile, tile < tiles, x, lane);
-    write_columns<E>(a, p.b, p.h, t0, rows_left(a.L, t0), p.col0, w, buffers + C::turn + w * C::kTurn, o,
-                     lane);
 #pragma unroll
     for (int i = 0; i < kUpdates; ++i) {
       if (i + 1 < kUpdates) steps_at(i + 1, ring[(i + 1) & 1]);
+      if (i == 0) turn_in<E>(turn, o, lane);
+      if (i + 1 == kUpdates) turn_out<E>(a, p.b, p.h, t0, p.col0, w, turn, o, lane);
+      if (kSave && i == kUpdates / 2 - 1)
+        keep<E, 2>(a.e, a.es, ch * tiles + tile, tile < tiles, x, lane);
       mma_tiles<kTerms>(ring[i & 1], up[i & 1], &S[4 * (i / 2)]);
+      interleave<kS, 4>();
     }
-    interleave<kUpdates * kS, 3, 1>();
     if (c + 1 < a.chunks) {
       if (C::kBuffers == 1) lds_barrier();  // this chunk is read
       lds_barrier();                        // the next one is there
@@ -697,50 +758,63 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
       cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
     }
     triangle_t(lds + C::m, lane, mf);
+    char* const turn = buffers + C::turn + w * C::kTurn;
+    f32x4 gam[4], beta[4], end[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      gam[mt] = row_of(C::gam, mt);
+      end[mt] = row_of(C::end, mt);
+    }
     in_order();
-    // M^T dO, meanwhile the planes of dS'
+    // M^T dO, meanwhile dS' is kept
     keys_at(0, ring[0]);
     split(join(dS[0], dS[1]), sp[0]);
+    settle(sp[0]);
     keep<E, KT / 2>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
     mma_triangle_t<kT>(mf, vp, y);
-    interleave<6 * products(kT, NI, kT), 4, 1>();
-    // K dS'
+    interleave<6 * products(kT, NI, kT), 5>();
+    // K dS', meanwhile the planes of scale exp(G) dO
+    bf16x8 up[2][kT], xp[2][kT];
 #pragma unroll
     for (int j = 0; j < C::kBlocks; ++j) {
       if (j + 1 < C::kBlocks) {
         keys_at(j + 1, ring[(j + 1) & 1]);
         split(join(dS[2 * j + 2], dS[2 * j + 3]), sp[(j + 1) & 1]);
+        settle(sp[(j + 1) & 1]);
       } else {
         steps_at(0, ring[(j + 1) & 1]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          split(whole(vp[s]) * (join(gam[2 * s], gam[2 * s + 1]) * a.scale), xp[s]);
+          settle(xp[s]);
+        }
       }
       mma_tiles<kT>(ring[j & 1], sp[j & 1], u);
-      interleave<kS, 4, 1>();
+      interleave<kS, 4>();
     }
-    bf16x8 up[2][kT], xp[2][kT];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      split(whole(vp[s]) * (join(row_of(C::gam, 2 * s), row_of(C::gam, 2 * s + 1)) * a.scale), xp[s]);
     const float last = reinterpret_cast<const float*>(lds + C::gam)[kChunk - 1];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) beta[mt] = row_of(C::beta, mt);
 #pragma unroll
     for (int t = 0; t < KT; ++t) dS[t] *= last;
     in_order();
     // Q^T (scale exp(G) dO), meanwhile dU (u) and the planes of beta dU
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
-        u[mt] = y[mt] + u[mt] * row_of(C::end, mt);
-        y[mt] = row_of(C::beta, mt) * u[mt];
-      }
-      split(join(y[2 * s], y[2 * s + 1]), up[s]);
-    }
-#pragma unroll
     for (int j = 0; j < KT / 2; ++j) {
       steps_at(j + 1, ring[(C::kBlocks + j + 1) & 1]);
+      if (j < 2) {
+#pragma unroll
+        for (int mt = 2 * j; mt < 2 * j + 2; ++mt) {
+          u[mt] = y[mt] + u[mt] * end[mt];
+          y[mt] = beta[mt] * u[mt];
+        }
+        split(join(y[2 * j], y[2 * j + 1]), up[j]);
+        settle(up[j]);
+      }
+      if (j + 1 == KT / 2) triangle_t(lds + C::n, lane, nf);
       mma_tiles<kT>(ring[(C::kBlocks + j) & 1], xp[j & 1], &dS[4 * (j / 2)]);
+      interleave<kS, 5>();
     }
-    triangle_t(lds + C::n, lane, nf);
-    interleave<KT / 2 * kS, 4, 2>();
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) y[mt] = f32x4{};
     mma_triangle_t<kT>(nf, up, y);
@@ -751,23 +825,33 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
 #pragma unroll
       for (int mt = 2 * s; mt < 2 * s + 2; ++mt) {
         u[mt] -= y[mt];
-        y[mt] = u[mt] * (row_of(C::beta, mt) * -row_of(C::gam, mt));
+        y[mt] = u[mt] * (beta[mt] * -gam[mt]);
       }
       split(join(y[2 * s], y[2 * s + 1]), up[s]);
     }
+    settle(up[0]);
+    settle(up[1]);
     in_order();
-    // K^T (exp(G) dV), meanwhile dV
-    keep<E, 2>(a.y, a.ys, ch * tiles + tile, tile < tiles, u, lane);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) u[mt] *= row_of(C::beta, mt);
-    write_columns<E>(a, p.b, p.h, t0, rows_left(a.L, t0), p.col0, w, buffers + C::turn + w * C::kTurn, u,
-                     lane);
+    // K^T (exp(G) dV), meanwhile Y is kept and dV written
 #pragma unroll
     for (int j = KT / 2; j < KT; ++j) {
       if (j + 1 < KT) steps_at(j + 1, ring[(C::kBlocks + j + 1) & 1]);
+      if (j == KT / 2) {
+        f32x4 v[4];
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
+        turn_in<E>(turn, v, lane);
+      }
+      if (j + 1 == KT / 4 * 3) keep<E, 2>(a.y, a.ys, ch * tiles + tile, tile < tiles, u, lane);
+      if (j + 1 == KT) {
+        f32x4 v[4];
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
+        turn_out<E>(a, p.b, p.h, t0, p.col0, w, turn, v, lane);
+      }
       mma_tiles<kT>(ring[(C::kBlocks + j) & 1], up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
+      interleave<kS, 4>();
     }
-    interleave<KT / 2 * kS, 3, 1>();
     if (c > 0) {
       if (C::kBuffers == 1) lds_barrier();
       lds_barrier();
