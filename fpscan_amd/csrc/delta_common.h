@@ -84,6 +84,11 @@ __device__ __forceinline__ f32x4 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB
   return c;
 }
 
+// Single fp16 operands.
+__device__ __forceinline__ f32x4 mma1(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
 // The same for kTiles left operands, tile by tile within a plane product, so that no product waits
 // for the one before it.
 template <int kTerms, int kTiles, int NA, int NB>

@@ -42,7 +42,7 @@ struct DeltaArgs {
   char *s, *e;        // saved per chunk: S before it, E
   float *ss, *es;     // and their scales
   char *ds, *y;       // the same of dS' and Y
-  float *dss, *ys;
+  float *dss, *ys, *gs;  // gs: of dO
   char *gq, *gk, *gg, *gbeta;
   const int32_t* slots;
   int64_t L, chunks, heads_total, nslots;
@@ -499,12 +499,11 @@ __device__ __forceinline__ void turn_in(char* turn, const f32x4 (&x)[4], int lan
     }
   }
 }
+// `col0`, `tile`: which columns of `dim` they are; r and st: the rows' tensor and their distance in bytes.
 template <class E>
-__device__ __forceinline__ void turn_out(const DeltaArgs& a, int64_t b, int64_t h, int64_t t0, int col0,
-                                         int tile, const char* turn, const f32x4 (&x)[4], int lane) {
-  const int li = lane & 15, lg = lane >> 4, st = a.H * a.Dv * E::kSize, rows = rows_left(a.L, t0);
-  const Rsrc r = row_rsrc(a.out, ((b * a.L + t0) * a.H + h) * a.Dv, E::kSize,
-                          ((rows - 1) * a.H + 1) * a.Dv * E::kSize);
+__device__ __forceinline__ void turn_out(Rsrc r, int st, int dim, int col0, int tile, const char* turn,
+                                         const f32x4 (&x)[4], int lane) {
+  const int li = lane & 15, lg = lane >> 4;
   if constexpr (E::kSize == 2) {
     const int d = col0 + key_col(tile, 4 * lg);
     typedef __attribute__((address_space(3))) s16x4* ldsp;
@@ -514,7 +513,7 @@ __device__ __forceinline__ void turn_out(const DeltaArgs& a, int64_t b, int64_t 
                          (mt & 1) * 8;
       const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ldsp)from);
       __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), r,
-                                            d < a.Dv ? (16 * mt + li) * st + d * 2 : kNoOffset, 0, 0);
+                                            d < dim ? (16 * mt + li) * st + d * 2 : kNoOffset, 0, 0);
     }
   } else {
     const int d = col0 + key_col(tile, li);
@@ -522,8 +521,16 @@ __device__ __forceinline__ void turn_out(const DeltaArgs& a, int64_t b, int64_t 
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        store1<E>(r, d < a.Dv ? (16 * mt + 4 * lg + i) * st + d * E::kSize : kNoOffset, x[mt][i]);
+        store1<E>(r, d < dim ? (16 * mt + 4 * lg + i) * st + d * E::kSize : kNoOffset, x[mt][i]);
   }
+}
+
+// The rows of a chunk in a contiguous (batch, seqlen, heads, dim) tensor.
+template <class E>
+__device__ __forceinline__ Rsrc rows_rsrc(const char* p, int64_t b, int64_t L, int64_t t0, int heads, int64_t h,
+                                          int dim) {
+  return row_rsrc(p, ((b * L + t0) * heads + h) * dim, E::kSize,
+                  ((rows_left(L, t0) - 1) * heads + 1) * dim * E::kSize);
 }
 
 // A walk's workgroup: which head and value columns. The workgroups of one head, which read the same K,
@@ -690,7 +697,8 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
     for (int i = 0; i < kUpdates; ++i) {
       if (i + 1 < kUpdates) steps_at(i + 1, ring[(i + 1) & 1]);
       if (i == 0) turn_in<E>(turn, o, lane);
-      if (i + 1 == kUpdates) turn_out<E>(a, p.b, p.h, t0, p.col0, w, turn, o, lane);
+      if (i + 1 == kUpdates) turn_out<E>(rows_rsrc<E>(a.out, p.b, a.L, t0, a.H, p.h, a.Dv), a.H * a.Dv * E::kSize, a.Dv, p.col0, w,
+                    turn, o, lane);
       if (kSave && i == kUpdates / 2 - 1)
         keep<E, 2>(a.e, a.es, ch * tiles + tile, tile < tiles, x, lane);
       mma_tiles<kTerms>(ring[i & 1], up[i & 1], &S[4 * (i / 2)]);
@@ -767,6 +775,19 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
     }
     in_order();
     // M^T dO, meanwhile dS' is kept
+    if constexpr (kept_size<E>() == 2) {
+      // the scale at which dO's 16 columns are fp16, as keep's
+      float most = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const f32x8 v = whole(vp[s]);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) most = fmaxf(most, fabsf(v[r]));
+      }
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(1.0f / block_scale(wave_max(most))),
+                                            row_rsrc(a.gs, ch * tiles + tile, 4, tile < tiles ? 4 : 0),
+                                            lane * 4, 0, 0);
+    }
     keys_at(0, ring[0]);
     split(join(dS[0], dS[1]), sp[0]);
     settle(sp[0]);
@@ -847,7 +868,8 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
         f32x4 v[4];
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
-        turn_out<E>(a, p.b, p.h, t0, p.col0, w, turn, v, lane);
+        turn_out<E>(rows_rsrc<E>(a.out, p.b, a.L, t0, a.H, p.h, a.Dv), a.H * a.Dv * E::kSize, a.Dv, p.col0, w,
+                    turn, v, lane);
       }
       mma_tiles<kT>(ring[(C::kBlocks + j) & 1], up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
       interleave<kS, 4>();
@@ -864,12 +886,19 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
 // key head; wave w makes KD / 4 key columns of dQ and dK. First the sums over the value columns, 32
 // at a time: dO S^T, dV S^T, U dS'^T (for its key columns) and dO U^T, dV U^T (rows 16 w..); then the
 // sums over steps, with P and F by way of LDS.
+//
+// bf16 tensors: the first sums are single fp16 products of what the walks kept in fp16 (2^-12 of a
+// block's largest), brought to one scale for all value columns, and of dO, U and dV rounded to fp16
+// on the same terms; each of these roundings is an eighth of the gradients' own to bf16. The others
+// take products of planes.
 template <class E, int KD>
 struct GradLds {
+  static constexpr bool kHalf = kept_size<E>() == 2;
   static constexpr int NI = InputPlanes<E>::n, kT = out_terms<E>();
+  static constexpr int NP = kHalf ? 1 : kT, NO = kHalf ? 1 : NI;  // planes of the first sums' operands
   static constexpr int kState = 32 * KD * 2, kSteps = 32 * kChunk * 2;  // one plane, 32 value columns
-  static constexpr int s = 0, ds = s + kT * kState, u = ds + kT * kState, dv = u + kT * kSteps,
-                       first = dv + kT * kSteps;
+  static constexpr int s = 0, ds = s + NP * kState, u = ds + NP * kState, dv = u + NP * kSteps,
+                       go = dv + NP * kSteps, first = go + NO * kSteps;
   static constexpr int kKeys = kChunk * KD * 2, kSquare = kChunk * kChunk * 2;
   static constexpr int k = 0, q = k + NI * kKeys, p = q + NI * kKeys, f = p + kT * kSquare,
                        second = f + kT * kSquare;
@@ -877,49 +906,64 @@ struct GradLds {
   static constexpr int kRow = 4 * kChunk;
   static constexpr int hi = rows, lo = hi + kRow, beta = lo + kRow, gam = beta + kRow,
                        end = gam + kRow, dbeta = end + kRow, dg = dbeta + 2 * kRow,
-                       sums = dg + 4 * kRow, size = sums + 64;
+                       sums = dg + 4 * kRow, scales = sums + 64;
+  // per 16 value columns, of S, dS', E and Y: the factor to the scale of all of them
+  static constexpr int kTiles = FPSCAN_DELTA_MAX_VALUE_DIM / 16;
+  static constexpr int size = scales + (kHalf ? 4 * kTiles * 4 : 0);
 };
 
-// Eight kept values of block `block`, piece `at`.
+// Eight kept values of a block, as they are in memory.
 template <class E>
-__device__ __forceinline__ f32x8 kept(const char* from, const float* scale, int64_t block, int pieces,
-                                      int at) {
-  if constexpr (kept_size<E>() == 2)
-    return __builtin_convertvector(reinterpret_cast<const f16x8*>(from)[block * pieces + at], f32x8) *
-           scale[block];
-  else
-    return reinterpret_cast<const f32x8*>(from)[block * pieces + at];
-}
+struct Kept {
+  static constexpr int n = kept_size<E>() / 2;
+  u32x4 x[n];
+  __device__ __forceinline__ void load(const char* from, int64_t block, int pieces, int at, bool live) {
+    const Rsrc r = row_rsrc(from, block, pieces * 16 * n, live ? pieces * 16 * n : 0);
+#pragma unroll
+    for (int i = 0; i < n; ++i) x[i] = bld16<0>(r, (at * n + i) * 16);
+  }
+  __device__ __forceinline__ f32x8 value() const {
+    if constexpr (n == 1)
+      return __builtin_convertvector(__builtin_bit_cast(f16x8, x[0]), f32x8);
+    else
+      return join(__builtin_bit_cast(f32x4, x[0]), __builtin_bit_cast(f32x4, x[n - 1]));
+  }
+};
 
-// x's planes as one piece of frags.
-template <int NP>
+// x's planes (or x in fp16) as one piece of frags.
+template <bool kHalf, int NP>
 __device__ __forceinline__ void put(char* to, int plane_bytes, f32x8 x) {
-  bf16x8 p[NP];
-  split(x, p);
+  if constexpr (kHalf) {
+    *reinterpret_cast<f16x8*>(to) = __builtin_convertvector(x, f16x8);
+  } else {
+    bf16x8 p[NP];
+    split(x, p);
 #pragma unroll
-  for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(to + i * plane_bytes) = p[i];
+    for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(to + i * plane_bytes) = p[i];
+  }
 }
 
-// The value at (row, col) of staged keys.
-template <int NI>
-__device__ __forceinline__ float key_at(const char* keys, int unit, int r, int plane_bytes) {
-  float x = 0.0f;
-#pragma unroll
-  for (int p = NI - 1; p >= 0; --p)
-    x += (float)reinterpret_cast<const __bf16*>(keys + p * plane_bytes + unit)[r];
-  return x;
+// c + a b for the first sums' operands.
+template <bool kHalf, int kTerms, int NA, int NB>
+__device__ __forceinline__ f32x4 mma_first(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+  if constexpr (kHalf)
+    return mma1(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c);
+  else
+    return mma<kTerms>(a, b, c);
 }
 
 template <class E, int KD, bool kShared>
-__global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
+__global__ __launch_bounds__(256, InputPlanes<E>::n == 1 && !kShared ? 2 : 1) void delta_grads(DeltaArgs a) {
   using C = GradLds<E, KD>;
-  constexpr int kT = C::kT, NI = C::NI, NT = KD / 64, kBlocks = KD / 32;
+  constexpr int kT = C::kT, NI = C::NI, NP = C::NP, NO = C::NO, NT = KD / 64, kBlocks = KD / 32;
+  constexpr bool kHalf = C::kHalf;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
+  const int w = wave_index();
+  int lane = threadIdx.x & 63;
   const int64_t group = blockIdx.x / a.chunks, c = blockIdx.x - group * a.chunks, t0 = c * kChunk;
   const int Hk = a.H / a.R;
   const int64_t b = group / Hk, hk = group - b * Hk;
-  const int rows = rows_left(a.L, t0), tiles = (a.Dv + 31) / 32 * 2;
+  const int rows = rows_left(a.L, t0), tiles = (a.Dv + 31) / 32 * 2, vblocks = tiles / 2;
   float* const row_hi = reinterpret_cast<float*>(lds + C::hi);
   float* const row_lo = reinterpret_cast<float*>(lds + C::lo);
   float* const row_beta = reinterpret_cast<float*>(lds + C::beta);
@@ -927,92 +971,165 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
   float* const row_end = reinterpret_cast<float*>(lds + C::end);
   float* const part_dbeta = reinterpret_cast<float*>(lds + C::dbeta);  // [2][64]
   float* const part_dg = reinterpret_cast<float*>(lds + C::dg);        // [4][64]
-  float* const sums = reinterpret_cast<float*>(lds + C::sums);         // [4] <S, dS'>, [4] rest
-  const int gst = (int)a.go.t * E::kSize;
+  float* const sums = reinterpret_cast<float*>(lds + C::sums);  // <S, dS'>, the rest, five scales
+  float* const scales = reinterpret_cast<float*>(lds + C::scales);
 
-  f32x4 dq[4][NT] = {}, dk[4][NT] = {};  // over the value heads
-  for (int j = 0; j < a.R; ++j) {
+  f32x4 dq[NT][4], dk[NT][4];  // over the value heads
+  if (kShared)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) dq[n][mt] = dk[n][mt] = f32x4{};
+  // addresses in LDS are made where they are used: kept over the loops they would take the registers
+  auto anew = [&] { settle(lane); };
+  for (int j = 0; j < (kShared ? a.R : 1); ++j) {
     const int64_t h = hk * a.R + j, bh = b * a.H + h, ch = bh * a.chunks + c;
-    const Rsrc rg = head_rsrc(a.go, b, h, t0, rows, a.Dv, E::kSize);
-    __syncthreads();  // the last head's rows are read
-    if (tid < kChunk) {
+    // the next 32 value columns on their way: S and dS', E and Y, dO
+    Kept<E> s[kBlocks / 2], ds[kBlocks / 2], e, y;
+    RowBlocks<E, 32, 4> go;
+    auto load = [&](int vb) {
+      const int64_t block = ch * tiles + 2 * vb;
+#pragma unroll
+      for (int i = 0; i < kBlocks / 2; ++i) {
+        const int at = 64 * w + lane + 256 * i;  // of two tiles' pieces, one after the other in memory
+        s[i].load(a.s, block / 2, 2 * kBlocks * 64, at, true);
+        ds[i].load(a.ds, block / 2, 2 * kBlocks * 64, at, true);
+      }
+      e.load(a.e, block / 2, 256, 64 * w + lane, true);
+      y.load(a.y, block / 2, 256, 64 * w + lane, true);
+      go.load(a.go, b, h, t0, rows, a.Dv, 32 * vb, w);
+    };
+    load(0);
+    float beta_scale = 1.0f;
+    lds_barrier();  // the last head's rows are read
+    if (w == 0) {
       const f32x4* gb = reinterpret_cast<const f32x4*>(a.gb) + ch * kChunk;
-      const f32x4 x = gb[tid], l = gb[kChunk - 1];
-      row_hi[tid] = x[0];
-      row_lo[tid] = x[1];
-      row_beta[tid] = x[2];
-      row_gam[tid] = expf(x[0]) * (1.0f + x[1]);
-      row_end[tid] = expf((l[0] - x[0]) + (l[1] - x[1]));
+      const f32x4 x = gb[lane], l = gb[kChunk - 1];
+      row_hi[lane] = x[0];
+      row_lo[lane] = x[1];
+      row_beta[lane] = x[2];
+      row_gam[lane] = expf(x[0]) * (1.0f + x[1]);
+      row_end[lane] = expf((l[0] - x[0]) + (l[1] - x[1]));
     }
-    f32x4 os[4][NT] = {}, vs[4][NT] = {}, us[4][NT] = {}, ou[4] = {}, vu[4] = {};
+    if constexpr (kHalf) {
+      auto common = [&](int which, const float* from) {
+        from += ch * tiles;
+        float most = 0.0f;
+        for (int t = lane; t < tiles; t += 64) most = fmaxf(most, from[t]);
+        most = wave_max(most);
+        if (which < 4)
+          for (int t = lane; t < tiles; t += 64) scales[which * C::kTiles + t] = from[t] / most;
+        if (lane == 0) sums[8 + which] = most;
+      };
+      if (w == 0) common(0, a.ss);
+      if (w == 1) common(1, a.dss);
+      if (w == 2) common(2, a.es);
+      if (w == 3) common(3, a.ys);
+      if (w == 0) common(4, a.gs);
+    }
+    f32x4 os[NT][4] = {}, vs[NT][4] = {}, us[NT][4] = {}, ou[4] = {}, vu[4] = {};
     f32x8 db = {};
     float sds = 0.0f;
-    for (int vb = 0; vb < (a.Dv + 31) / 32; ++vb) {
-      __syncthreads();  // rows are there, or the block before is read
-      for (int i = tid; i < 2 * kBlocks * 64; i += 256) {
-        const int vt = i / (kBlocks * 64), at = i % (kBlocks * 64), tile = 2 * vb + vt;
-        f32x8 x = {}, y = {};
-        if (tile < tiles) {
-          x = kept<E>(a.s, a.ss, ch * tiles + tile, kBlocks * 64, at);
-          y = kept<E>(a.ds, a.dss, ch * tiles + tile, kBlocks * 64, at);
-        }
+    lds_barrier();
+    if constexpr (kHalf) {
+      // |beta| up to a power of two: U and dV keep to fp16's range
+      const float most = wave_max(fabsf(row_beta[lane]));
+      if (most > 1.0f) beta_scale = 0x1p-15f * block_scale(most);
+    }
+    for (int vb = 0; vb < vblocks; ++vb) {
+      if (vb > 0) lds_barrier();  // the block before is read
+      anew();
+      const int li = lane & 15, lg = lane >> 4;
+      auto scale_of = [&](int which, int vt) {
+        return kHalf ? scales[which * C::kTiles + 2 * vb + vt] : 1.0f;
+      };
 #pragma unroll
-        for (int r = 0; r < 8; ++r) sds = fmaf(x[r], y[r], sds);
-        const int to = (i >> 6) * 1024 + frag_lane(i & 15, (i >> 4) & 3);
-        put<kT>(lds + C::s + to, C::kState, x);
-        put<kT>(lds + C::ds + to, C::kState, y);
+      for (int i = 0; i < kBlocks / 2; ++i) {
+        const int piece = w + 4 * i, vt = piece / kBlocks;
+        const int to = piece * 1024 + frag_lane(li, lg);
+        if constexpr (kHalf) {
+          const f16x8 x = __builtin_bit_cast(f16x8, s[i].x[0]) * (_Float16)scale_of(0, vt);
+          const f16x8 z = __builtin_bit_cast(f16x8, ds[i].x[0]) * (_Float16)scale_of(1, vt);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            sds = __builtin_amdgcn_fdot2(f16x2{x[2 * r], x[2 * r + 1]}, f16x2{z[2 * r], z[2 * r + 1]}, sds,
+                                         false);
+          *reinterpret_cast<f16x8*>(lds + C::s + to) = x;
+          *reinterpret_cast<f16x8*>(lds + C::ds + to) = z;
+        } else {
+          const f32x8 x = s[i].value(), z = ds[i].value();
+#pragma unroll
+          for (int r = 0; r < 8; ++r) sds = fmaf(x[r], z[r], sds);
+          put<false, NP>(lds + C::s + to, C::kState, x);
+          put<false, NP>(lds + C::ds + to, C::kState, z);
+        }
       }
       {
-        const int vt = tid >> 7, s = w & 1, tile = 2 * vb + vt;
-        f32x8 x = {}, y = {};
-        if (tile < tiles) {
-          x = kept<E>(a.e, a.es, ch * tiles + tile, 128, s * 64 + lane);
-          y = kept<E>(a.y, a.ys, ch * tiles + tile, 128, s * 64 + lane);
-        }
-        const f32x8 beta = join(*reinterpret_cast<const f32x4*>(row_beta + 32 * s + 4 * lg),
-                                *reinterpret_cast<const f32x4*>(row_beta + 32 * s + 16 + 4 * lg));
-        db += x * y;
-        const int to = (2 * vt + s) * 1024 + frag_lane(li, lg);
-        put<kT>(lds + C::u + to, C::kSteps, x * beta);
-        put<kT>(lds + C::dv + to, C::kSteps, y * beta);
+        const int vt = w >> 1, st = w & 1;
+        const f32x8 beta = join(*reinterpret_cast<const f32x4*>(row_beta + 32 * st + 4 * lg),
+                                *reinterpret_cast<const f32x4*>(row_beta + 32 * st + 16 + 4 * lg)) *
+                           beta_scale;
+        const f32x8 x = e.value() * scale_of(2, vt), z = y.value() * scale_of(3, vt);
+        db += x * z;
+        const int to = (2 * vt + st) * 1024 + frag_lane(li, lg);
+        put<kHalf, NP>(lds + C::u + to, C::kSteps, x * beta);
+        put<kHalf, NP>(lds + C::dv + to, C::kSteps, z * beta);
       }
-      __syncthreads();
-      bf16x8 sp[NT][kT], dsp[NT][kT], ow[NI], vw[kT];
+      if constexpr (kHalf) {
+        bf16x8 p[1] = {__builtin_bit_cast(bf16x8, go.x[0][0])};
+        put<true, 1>(lds + C::go + w * 1024 + frag_lane(li, lg), C::kSteps, whole(p) * (1.0f / sums[12]));
+      } else {
+        go.store(lds + C::go, w);
+      }
+      lds_barrier();
+      if (vb + 1 < vblocks) load(vb + 1);
+      anew();
+      bf16x8 sp[NT][NP], dsp[NT][NP], ow[NO], vw[NP];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int ct = w * NT + n, at = ct / 2 * 1024;
         cols_of(lds + C::s + at, lds + C::s + at + kBlocks * 1024, C::kState, ct, lane, sp[n]);
         cols_of(lds + C::ds + at, lds + C::ds + at + kBlocks * 1024, C::kState, ct, lane, dsp[n]);
       }
-      const int d0 = 32 * vb + 8 * lg;
-      load8<E>(rg, d0 < a.Dv ? (16 * w + li) * gst + d0 * E::kSize : kNoOffset, ow);
+      rows_of(lds + C::go + w * 1024, C::kSteps, lane, ow);
       cols_of(lds + C::dv + w / 2 * 1024, lds + C::dv + (2 + w / 2) * 1024, C::kSteps, w, lane, vw);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        bf16x8 op[NI], vp[kT], upl[kT];
-        load8<E>(rg, d0 < a.Dv ? (16 * mt + li) * gst + d0 * E::kSize : kNoOffset, op);
+        bf16x8 op[NO], vp[NP], up[NP];
+        rows_of(lds + C::go + mt * 1024, C::kSteps, lane, op);
         cols_of(lds + C::dv + mt / 2 * 1024, lds + C::dv + (2 + mt / 2) * 1024, C::kSteps, mt, lane, vp);
-        cols_of(lds + C::u + mt / 2 * 1024, lds + C::u + (2 + mt / 2) * 1024, C::kSteps, mt, lane, upl);
+        cols_of(lds + C::u + mt / 2 * 1024, lds + C::u + (2 + mt / 2) * 1024, C::kSteps, mt, lane, up);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          os[mt][n] = mma<kT>(op, sp[n], os[mt][n]);
-          vs[mt][n] = mma<kT>(vp, sp[n], vs[mt][n]);
-          us[mt][n] = mma<kT>(upl, dsp[n], us[mt][n]);
+          os[n][mt] = mma_first<kHalf, kT>(op, sp[n], os[n][mt]);
+          vs[n][mt] = mma_first<kHalf, kT>(vp, sp[n], vs[n][mt]);
+          us[n][mt] = mma_first<kHalf, kT>(up, dsp[n], us[n][mt]);
         }
         if (mt <= w) {
-          ou[mt] = mma<kT>(ow, upl, ou[mt]);
-          vu[mt] = mma<kT>(vw, upl, vu[mt]);
+          ou[mt] = mma_first<kHalf, kT>(ow, up, ou[mt]);
+          vu[mt] = mma_first<kHalf, kT>(vw, up, vu[mt]);
         }
+        in_order();
       }
     }
-    __syncthreads();
-    {
-      RowBlocks<E, KD, 4> keys, queries;
-      keys.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
-      queries.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
-      keys.store(lds + C::k, w);
-      queries.store(lds + C::q, w);
+    anew();
+    const int li = lane & 15, lg = lane >> 4;
+    RowBlocks<E, KD, 4> keys, queries;
+    keys.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
+    queries.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
+    // the sums' scales: of a product's operands one after the other, as each may be far from 1
+    float fs = 1.0f, fds = 1.0f, fe = 1.0f, fy = 1.0f, fo = 1.0f;
+    if constexpr (kHalf) {
+      const float unit = 1.0f / beta_scale;
+      fs = sums[8];
+      fds = sums[9];
+      fe = sums[10] * unit;
+      fy = sums[11] * unit;
+      fo = sums[12];
+      sds = sds * fs * fds;
+      db = db * sums[10] * sums[11];
     }
+    lds_barrier();
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt)
       if (nt <= (w | 1)) {
@@ -1023,8 +1140,8 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
           const int i = i0 + r;
           const float gam =
               jj <= i ? expf((row_hi[i] - row_hi[jj]) + (row_lo[i] - row_lo[jj])) : 0.0f;
-          p[r] = jj <= i ? a.scale * (gam * ou[nt][r]) : 0.0f;
-          f[r] = jj < i ? -(gam * vu[nt][r]) : 0.0f;
+          p[r] = jj <= i ? a.scale * (gam * (ou[nt][r] * fo * fe)) : 0.0f;
+          f[r] = jj < i ? -(gam * (vu[nt][r] * fy * fe)) : 0.0f;
         }
         bf16x4 pp[kT], fp[kT];
         split(p, pp);
@@ -1036,13 +1153,16 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
           *reinterpret_cast<bf16x4*>(lds + C::f + x * C::kSquare + to) = fp[x];
         }
       }
+    keys.store(lds + C::k, w);
+    queries.store(lds + C::q, w);
     // dbeta: over the 16 value columns of a lane group, then the two tiles
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const float x = group_sum(db[r]);
-      if (li == 0) part_dbeta[(tid >> 7) * kChunk + 32 * (w & 1) + (r >> 2) * 16 + 4 * lg + (r & 3)] = x;
+      if (li == 0) part_dbeta[(w >> 1) * kChunk + 32 * (w & 1) + (r >> 2) * 16 + 4 * lg + (r & 3)] = x;
     }
-    __syncthreads();
+    lds_barrier();
+    anew();
     float rest = 0.0f;
     f32x4 dG[4] = {};
 #pragma unroll
@@ -1050,48 +1170,44 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
       const int ct = w * NT + n;
       bf16x8 kp[2][NI], qp[2][NI];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int at = (2 * s * kBlocks + ct / 2) * 1024;
-        cols_of(lds + C::k + at, lds + C::k + at + kBlocks * 1024, C::kKeys, ct, lane, kp[s]);
-        cols_of(lds + C::q + at, lds + C::q + at + kBlocks * 1024, C::kKeys, ct, lane, qp[s]);
+      for (int st = 0; st < 2; ++st) {
+        const int at = (2 * st * kBlocks + ct / 2) * 1024;
+        cols_of(lds + C::k + at, lds + C::k + at + kBlocks * 1024, C::kKeys, ct, lane, kp[st]);
+        cols_of(lds + C::q + at, lds + C::q + at + kBlocks * 1024, C::kKeys, ct, lane, qp[st]);
       }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const f32x4 gam = *reinterpret_cast<const f32x4*>(row_gam + 16 * mt + 4 * lg);
-        const f32x4 write = us[mt][n] * *reinterpret_cast<const f32x4*>(row_end + 16 * mt + 4 * lg);
-        f32x4 x = os[mt][n] * (gam * a.scale), y = write - vs[mt][n] * gam;
+        const f32x4 end = *reinterpret_cast<const f32x4*>(row_end + 16 * mt + 4 * lg);
+        const f32x4 write = us[n][mt] * end * fe * fds;
+        f32x4 x = os[n][mt] * (gam * a.scale) * fo * fs, z = write - vs[n][mt] * gam * fy * fs;
         bf16x8 f[kT];
 #pragma unroll
-        for (int s = 0; s <= mt / 2; ++s) {
-          const int at = (4 * s + mt / 2) * 1024;  // P^T and F^T: rows 32 s.., columns 16 mt..
+        for (int st = 0; st <= mt / 2; ++st) {
+          const int at = (4 * st + mt / 2) * 1024;  // P^T and F^T: rows 32 st.., columns 16 mt..
           cols_of(lds + C::p + at, lds + C::p + at + 2048, C::kSquare, mt, lane, f);
-          x = mma<kT>(f, kp[s], x);
+          x = mma<kT>(f, kp[st], x);
           cols_of(lds + C::f + at, lds + C::f + at + 2048, C::kSquare, mt, lane, f);
-          y = mma<kT>(f, kp[s], y);
+          z = mma<kT>(f, kp[st], z);
         }
 #pragma unroll
-        for (int s = mt / 2; s < 2; ++s) {
-          const int at = (2 * mt + s) * 1024;
+        for (int st = mt / 2; st < 2; ++st) {
+          const int at = (2 * mt + st) * 1024;
           rows_of(lds + C::p + at, C::kSquare, lane, f);
-          y = mma<kT>(f, qp[s], y);
+          z = mma<kT>(f, qp[st], z);
           rows_of(lds + C::f + at, C::kSquare, lane, f);
-          y = mma<kT>(f, kp[s], y);
+          z = mma<kT>(f, kp[st], z);
         }
+        // the operands' lanes hold the very values of K and Q that this result belongs to
+        const f32x8 kv = whole(kp[mt / 2]), qv = whole(qp[mt / 2]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int unit = (mt * kBlocks + ct / 2) * 1024 + frag_lane(4 * lg + r, li >> 2) + (ct & 1) * 8;
-          const float kv = key_at<NI>(lds + C::k, unit, li & 3, C::kKeys);
-          const float qv = key_at<NI>(lds + C::q, unit, li & 3, C::kKeys);
-          dG[mt][r] += qv * x[r] + kv * y[r];
-          rest = fmaf(kv, write[r], rest);
+          dG[mt][r] += qv[(mt & 1) * 4 + r] * x[r] + kv[(mt & 1) * 4 + r] * z[r];
+          rest = fmaf(kv[(mt & 1) * 4 + r], write[r], rest);
         }
-        if constexpr (kShared) {
-          dq[mt][n] += x;
-          dk[mt][n] += y;
-        } else {
-          dq[mt][n] = x;
-          dk[mt][n] = y;
-        }
+        dq[n][mt] = kShared ? dq[n][mt] + x : x;
+        dk[n][mt] = kShared ? dk[n][mt] + z : z;
+        in_order();
       }
     }
 #pragma unroll
@@ -1106,7 +1222,7 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
       sums[w] = sum_s;
       sums[4 + w] = sum_r;
     }
-    __syncthreads();
+    lds_barrier();
     if (w == 0) {
       const float dbeta = part_dbeta[lane] + part_dbeta[kChunk + lane];
       float x = part_dg[lane] + part_dg[kChunk + lane] + part_dg[2 * kChunk + lane] +
@@ -1129,22 +1245,19 @@ __global__ __launch_bounds__(256) void delta_grads(DeltaArgs a) {
       }
     }
   }
+  // P and F are read: their place turns columns into rows
   const int st = Hk * a.Dk * E::kSize;
-  const int64_t base = ((b * a.L + t0) * Hk + hk) * a.Dk;
-  const int bytes = (rows - 1) * st + a.Dk * E::kSize;
-  const Rsrc oq = row_rsrc(a.gq, base, E::kSize, bytes), ok = row_rsrc(a.gk, base, E::kSize, bytes);
+  const Rsrc oq = rows_rsrc<E>(a.gq, b, a.L, t0, Hk, hk, a.Dk), ok = rows_rsrc<E>(a.gk, b, a.L, t0, Hk, hk, a.Dk);
+  char* const turn = lds + C::p + w * 4096 * NT;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int col = key_col(w * NT + n, li);
+    turn_in<E>(turn + 4096 * n, dq[n], lane);
+    turn_in<E>(turn + 4096 * n + 2048, dk[n], lane);
+  }
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t off =
-            col < a.Dk ? (16 * mt + 4 * lg + r) * st + col * E::kSize : kNoOffset;
-        store1<E>(oq, off, dq[mt][n][r]);
-        store1<E>(ok, off, dk[mt][n][r]);
-      }
+  for (int n = 0; n < NT; ++n) {
+    turn_out<E>(oq, st, a.Dk, 0, w * NT + n, turn + 4096 * n, dq[n], lane);
+    turn_out<E>(ok, st, a.Dk, 0, w * NT + n, turn + 4096 * n + 2048, dk[n], lane);
   }
 }
 
@@ -1370,6 +1483,7 @@ void carve_bwd(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
   a.y = w.take(blocks * kChunk * 16 * each);
   a.dss = reinterpret_cast<float*>(w.take(blocks * 4));
   a.ys = reinterpret_cast<float*>(w.take(blocks * 4));
+  a.gs = reinterpret_cast<float*>(w.take(blocks * 4));
 }
 
 template <class F>
