@@ -1514,21 +1514,40 @@ unsigned walk_grid(DeltaArgs& a, int waves) {
   return (unsigned)((a.heads_total + 7) / 8 * 8 * a.vblocks);
 }
 
-// Computing waves of a walk's workgroup.
-template <class E>
-constexpr int walk_waves() { return 2; }
-template <class E>
-constexpr int bring_waves() { return InputPlanes<E>::n == 3 ? 2 : 4; }
+// Waves of a walk's workgroup: two that compute and four that bring while that fills no more than the
+// CUs, four and four beyond (8 heads of 8 sequences, width 128, bf16: 117 us for 2048 steps against
+// 122; 80 heads, fp16, 777 steps: 88 us against 139). fp32 has LDS for two and registers for two more.
+bool walk_narrow(const DeltaArgs& a) { return a.heads_total * ((a.Dv + 63) / 64) <= 128; }
+
+template <class E, int KD, int kTerms, bool kSave, int kWaves, int kBring>
+int launch_forward(DeltaArgs& a, hipStream_t stream) {
+  using C = ChunkLds<E, KD, kTerms, out_terms<E>(), kWaves>;
+  const auto walk = delta_chunks<E, KD, kTerms, kSave, kWaves, kBring>;
+  const int st = allow_lds(walk, C::total);
+  if (st != FPSCAN_OK) return st;
+  const unsigned grid = walk_grid(a, kWaves);
+  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
+  return launched();
+}
 
 template <class E, int KD, int kTerms, bool kSave>
 int walk_forward(DeltaArgs& a, hipStream_t stream) {
-  constexpr int kOut = out_terms<E>(), kWaves = walk_waves<E>(), kBring = bring_waves<E>();
-  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
-  delta_prep<E, KD, kTerms, kOut><<<(unsigned)(a.heads_total * a.chunks), 256, 0, stream>>>(a);
-  int st = launched();
+  delta_prep<E, KD, kTerms, out_terms<E>()><<<(unsigned)(a.heads_total * a.chunks), 256, 0, stream>>>(a);
+  const int st = launched();
   if (st != FPSCAN_OK) return st;
-  const auto walk = delta_chunks<E, KD, kTerms, kSave, kWaves, kBring>;
-  if ((st = allow_lds(walk, C::total)) != FPSCAN_OK) return st;
+  if constexpr (InputPlanes<E>::n == 3)
+    return launch_forward<E, KD, kTerms, kSave, 2, 2>(a, stream);
+  else
+    return walk_narrow(a) ? launch_forward<E, KD, kTerms, kSave, 2, 4>(a, stream)
+                          : launch_forward<E, KD, kTerms, kSave, 4, 4>(a, stream);
+}
+
+template <class E, int KD, int kWaves, int kBring>
+int launch_backward(DeltaArgs& a, hipStream_t stream) {
+  using C = ChunkLds<E, KD, out_terms<E>(), out_terms<E>(), kWaves>;
+  const auto walk = delta_chunks_bwd<E, KD, kWaves, kBring>;
+  const int st = allow_lds(walk, C::total);
+  if (st != FPSCAN_OK) return st;
   const unsigned grid = walk_grid(a, kWaves);
   walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
   return launched();
@@ -1536,17 +1555,16 @@ int walk_forward(DeltaArgs& a, hipStream_t stream) {
 
 template <class E, int KD>
 int backward(DeltaArgs& a, hipStream_t stream) {
-  constexpr int kT = out_terms<E>(), kWaves = walk_waves<E>(), kBring = bring_waves<E>(), glds = GradLds<E, KD>::size;
-  using C = ChunkLds<E, KD, kT, kT, kWaves>;
-  const auto walk = delta_chunks_bwd<E, KD, kWaves, kBring>;
-  int st = allow_lds(walk, C::total);
+  int st;
+  if constexpr (InputPlanes<E>::n == 3)
+    st = launch_backward<E, KD, 2, 2>(a, stream);
+  else
+    st = walk_narrow(a) ? launch_backward<E, KD, 2, 4>(a, stream) : launch_backward<E, KD, 4, 4>(a, stream);
   if (st != FPSCAN_OK) return st;
-  const unsigned grid = walk_grid(a, kWaves);
-  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
-  if ((st = launched()) != FPSCAN_OK) return st;
+  constexpr int lds = GradLds<E, KD>::size;
   const auto kernel = a.R > 1 ? delta_grads<E, KD, true> : delta_grads<E, KD, false>;
-  if ((st = allow_lds(kernel, glds)) != FPSCAN_OK) return st;
-  kernel<<<(unsigned)(a.heads_total / a.R * a.chunks), 256, glds, stream>>>(a);
+  if ((st = allow_lds(kernel, lds)) != FPSCAN_OK) return st;
+  kernel<<<(unsigned)(a.heads_total / a.R * a.chunks), 256, lds, stream>>>(a);
   return launched();
 }
 

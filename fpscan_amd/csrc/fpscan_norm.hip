@@ -44,6 +44,9 @@ __device__ __forceinline__ void load_vec(const char* p, float (&f)[E::V]) {
   E::unpack(*reinterpret_cast<const u32x4*>(p), f);
 }
 
+// The same as it is in memory: loads of several rows go out before the first is used.
+__device__ __forceinline__ u32x4 raw_vec(const char* p) { return *reinterpret_cast<const u32x4*>(p); }
+
 template <class E>
 __device__ __forceinline__ void store_vec(char* p, const float (&f)[E::V]) {
   *reinterpret_cast<u32x4*>(p) = E::pack(f);
@@ -108,31 +111,58 @@ __device__ __forceinline__ void group_sums(const NormArgs& a, const float* buf, 
   }
 }
 
-// The sum of a thread's channels over their groups in its row, back per channel. kAligned: groups are
-// `lanes` whole vectors, a power of two up to the wave, and the lanes that hold one add up among
-// themselves. Otherwise through LDS: rows * (dim + groups) floats.
-template <int V, bool kAligned>
-__device__ __forceinline__ void row_sums(const NormArgs& a, const Place& p, float* lds,
-                                         const float (&x)[V], float (&s)[V]) {
-  if constexpr (kAligned) {
-    float t = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) t += x[i];
-    for (int m = a.lanes >> 1; m > 0; m >>= 1) t += __shfl_xor(t, m);
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = t;
-  } else {
-    float* const sums = lds + a.rows * a.dim;
-    if (p.in)
-#pragma unroll
-      for (int i = 0; i < V; ++i) lds[p.row * a.dim + p.c + i] = x[i];
-    __syncthreads();
-    group_sums(a, lds, sums, a.rows, a.lanes);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = p.in ? sums[p.row * a.groups + (p.c + i) / a.width] : 0.0f;
-  }
+// The sum over `lanes` consecutive lanes (a power of two), in each of them. Within 16 lanes by DPP.
+__device__ __forceinline__ float lane_sums(float t, int lanes) {
+  if (lanes > 1) t += dpp_any<0xB1>(t);   // quad_perm: the neighbour
+  if (lanes > 2) t += dpp_any<0x4E>(t);   // quad_perm: the other pair
+  if (lanes > 4) t += dpp_any<0x141>(t);  // row_half_mirror: the other four
+  if (lanes > 8) t += dpp_any<0x140>(t);  // row_mirror: the other eight
+  if (lanes > 16) t += __shfl_xor(t, 16);
+  if (lanes > 32) t += __shfl_xor(t, 32);
+  return t;
 }
+
+// Sums over groups of a row, as a thread needs them. kAligned: a group is `lanes` whole vectors, a
+// power of two up to the wave: a thread has one group, and the lanes that hold it add up among
+// themselves. Otherwise each channel has its own, through LDS: rows * (dim + groups) floats.
+template <int V, bool kAligned>
+struct GroupSums {
+  static constexpr int n = kAligned ? 1 : V;
+  int group[n];  // in the row
+  bool first;    // kAligned: whether the group begins with this thread
+
+  __device__ __forceinline__ GroupSums(const NormArgs& a, const Place& p) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) group[i] = (p.c + i) / a.width;
+    first = p.c == group[0] * a.width;
+  }
+  __device__ __forceinline__ void sum(const NormArgs& a, const Place& p, float* lds, const float (&x)[V],
+                                      float (&s)[n]) const {
+    if constexpr (kAligned) {
+      float t = x[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) t += x[i];
+      s[0] = lane_sums(t, a.lanes);
+    } else {
+      float* const sums = lds + a.rows * a.dim;
+      if (p.in)
+#pragma unroll
+        for (int i = 0; i < V; ++i) lds[p.row * a.dim + p.c + i] = x[i];
+      __syncthreads();
+      group_sums(a, lds, sums, a.rows, a.lanes);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = p.in ? sums[p.row * a.groups + group[i]] : 0.0f;
+    }
+  }
+  // a statistic, written by the thread of a group's first channel
+  __device__ __forceinline__ void write(const NormArgs& a, const Place& p, float* to, const float (&x)[n]) const {
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      if (kAligned ? first : p.c + i == group[i] * a.width) to[group[i]] = x[i];
+  }
+  static __device__ __forceinline__ int at(int i) { return kAligned ? 0 : i; }
+};
 
 // A thread's per-channel values, summed over the workgroup's rows: to[c] (through lds, rows * dim).
 template <int V>
@@ -154,42 +184,43 @@ __device__ __forceinline__ void column_sums(const NormArgs& a, const Place& p, f
 template <class E, bool kAct, bool kGate, bool kAligned>
 __global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
   constexpr int V = E::V;
+  using G = GroupSums<V, kAligned>;
   extern __shared__ float lds[];
   const Place p = place<E>(a);
+  const G groups(a, p);
   float w[V], b[V];
   params(a, p, w, b);
   const float inv = 1.0f / (float)a.width;
   for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
     const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
     const bool in = p.in && r < a.batch;
-    float x[V] = {}, z[V] = {}, s[V], q[V], off[V];
+    float x[V] = {}, z[V] = {}, q[V], s[G::n], mu[G::n], off[G::n];
     if (in) load_vec<E>(a.x + at, x);
     if (kGate && in) load_vec<E>(a.gate + at, z);
-    row_sums<V, kAligned>(a, p, lds, x, s);
-    float mu[V];
+    groups.sum(a, p, lds, x, mu);
+#pragma unroll
+    for (int i = 0; i < G::n; ++i) mu[i] *= inv;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      mu[i] = s[i] * inv;
-      x[i] -= mu[i];
+      x[i] -= mu[G::at(i)];
       q[i] = x[i] * x[i];
     }
     // the sum's own rounding, where means are far from 0, is the mean of the differences
-    row_sums<V, kAligned>(a, p, lds, x, s);
+    groups.sum(a, p, lds, x, off);
+    groups.sum(a, p, lds, q, s);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s[i] *= inv;
-      mu[i] += s[i];
-      x[i] -= s[i];
-      off[i] = s[i];
-      if (a.mean && in && (p.c + i) % a.width == 0) a.mean[r * a.groups + (p.c + i) / a.width] = mu[i];
+    for (int i = 0; i < G::n; ++i) {
+      off[i] *= inv;
+      mu[i] += off[i];
+      s[i] = __builtin_amdgcn_rsqf(fmaf(-off[i], off[i], s[i] * inv) + a.eps);
     }
-    row_sums<V, kAligned>(a, p, lds, q, s);
+    if (a.mean && in) {
+      groups.write(a, p, a.mean + r * a.groups, mu);
+      groups.write(a, p, a.rstd + r * a.groups, s);
+    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s[i] = 1.0f / sqrtf(fmaf(-off[i], off[i], s[i] * inv) + a.eps);
-      if (a.mean && in && (p.c + i) % a.width == 0) a.rstd[r * a.groups + (p.c + i) / a.width] = s[i];
-      x[i] = activate<E, kAct, kGate>(fmaf(x[i] * s[i], w[i], b[i]), z[i]);
-    }
+    for (int i = 0; i < V; ++i)
+      x[i] = activate<E, kAct, kGate>(fmaf((x[i] - off[G::at(i)]) * s[G::at(i)], w[i], b[i]), z[i]);
     if (in) store_vec<E>(a.out + at, x);
   }
 }
@@ -197,37 +228,46 @@ __global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
 template <class E, bool kAct, bool kGate, bool kAligned>
 __global__ __launch_bounds__(1024) void norm_tokens_bwd(NormArgs a) {
   constexpr int V = E::V;
+  using G = GroupSums<V, kAligned>;
   extern __shared__ float lds[];
   const Place p = place<E>(a);
+  const G groups(a, p);
   float w[V], b[V], gw[V] = {}, gb[V] = {};
   params(a, p, w, b);
   const float inv = 1.0f / (float)a.width;
   for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
     const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
     const bool in = p.in && r < a.batch;
-    float x[V] = {}, z[V] = {}, go[V] = {}, rs[V] = {}, s1[V], s2[V];
+    float x[V] = {}, z[V] = {}, go[V] = {}, mu[G::n] = {}, rs[G::n] = {}, m1[G::n], m2[G::n], t[V];
     if (in) {
       load_vec<E>(a.x + at, x);
       load_vec<E>(a.go + at, go);
       if (kGate) load_vec<E>(a.gate + at, z);
+#pragma unroll
+      for (int i = 0; i < G::n; ++i) {
+        mu[i] = a.mean[r * a.groups + groups.group[i]];
+        rs[i] = a.rstd[r * a.groups + groups.group[i]];
+      }
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (in) {
-        const int64_t g = r * a.groups + (p.c + i) / a.width;
-        rs[i] = a.rstd[g];
-        x[i] = (x[i] - a.mean[g]) * rs[i];
-      }
+      x[i] = (x[i] - mu[G::at(i)]) * rs[G::at(i)];
       go[i] = slope<E, kAct, kGate>(fmaf(x[i], w[i], b[i]), z[i], go[i], z[i]);
       gb[i] += go[i];
       gw[i] = fmaf(go[i], x[i], gw[i]);
       go[i] *= w[i];
-      s2[i] = go[i] * x[i];
+      t[i] = go[i] * x[i];
     }
-    row_sums<V, kAligned>(a, p, lds, go, s1);
-    row_sums<V, kAligned>(a, p, lds, s2, s2);
+    groups.sum(a, p, lds, go, m1);
+    groups.sum(a, p, lds, t, m2);
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = rs[i] * (go[i] - s1[i] * inv - x[i] * (s2[i] * inv));
+    for (int i = 0; i < G::n; ++i) {
+      m1[i] *= inv * rs[i];
+      m2[i] *= inv * rs[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      x[i] = fmaf(rs[G::at(i)], go[i], -fmaf(x[i], m2[G::at(i)], m1[G::at(i)]));
     if (in) {
       store_vec<E>(a.gx + at, x);
       if (kGate) store_vec<E>(a.ggate + at, z);
@@ -243,10 +283,37 @@ __global__ __launch_bounds__(1024) void norm_tokens_bwd(NormArgs a) {
 struct Chunk {
   int64_t b, first, rows;
 };
+// kBack: chunks from the last one on, for a second pass: what the first read last is still in the
+// memory-side cache.
+template <bool kBack = false>
 __device__ __forceinline__ Chunk chunk_of(const NormArgs& a) {
-  const int64_t b = blockIdx.x / a.chunks, first = (blockIdx.x - b * a.chunks) * a.chunk_rows;
+  const int64_t i = kBack ? (int64_t)gridDim.x - 1 - blockIdx.x : (int64_t)blockIdx.x;
+  const int64_t b = i / a.chunks, first = (i - b * a.chunks) * a.chunk_rows;
   const int64_t left = a.seqlen - first;
   return {b, first, left < a.chunk_rows ? left : a.chunk_rows};
+}
+
+// A thread's rows of a chunk, of the first kTensors of `from`: two rows' loads go out together.
+template <class E, int kTensors, class F>
+__device__ __forceinline__ void by_two(const NormArgs& a, const Place& p, const Chunk& k, int64_t step,
+                                       int64_t at, const char* const (&from)[3],
+                                       F&& take) {
+  int64_t r = p.row;
+  for (; p.in && r + a.rows < k.rows; r += 2 * a.rows, at += 2 * step) {
+    u32x4 raw[2][kTensors];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < kTensors; ++i) raw[j][i] = raw_vec(from[i] + at + j * step);
+    take(at, raw[0]);
+    take(at + step, raw[1]);
+  }
+  if (p.in && r < k.rows) {
+    u32x4 raw[kTensors];
+#pragma unroll
+    for (int i = 0; i < kTensors; ++i) raw[i] = raw_vec(from[i] + at);
+    take(at, raw);
+  }
 }
 
 template <class E>
@@ -259,18 +326,27 @@ __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
   const char* at = a.x + ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
   const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
   float x0[V] = {}, s[V] = {}, q[V] = {}, n = 0.0f;
-  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+  auto take = [&](u32x4 raw) {
     float x[V];
-    load_vec<E>(at, x);
+    E::unpack(raw, x);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (n == 0.0f) x0[i] = x[i];
       const float d = x[i] - x0[i];
       s[i] += d;
       q[i] = fmaf(d, d, q[i]);
     }
     n += 1.0f;
+  };
+  int64_t r = p.row;
+  if (p.in && r < k.rows) load_vec<E>(at, x0);
+  for (; p.in && r + 3 * a.rows < k.rows; r += 4 * a.rows, at += 4 * step) {
+    u32x4 raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = raw_vec(at + j * step);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) take(raw[j]);
   }
+  for (; p.in && r < k.rows; r += a.rows, at += step) take(raw_vec(at));
   const float inv = n > 0.0f ? 1.0f / n : 0.0f;
   // means are taken from the group's first value, so that sums of means far from 0 lose nothing
   float* const base = sums + a.rows * a.groups;
@@ -332,7 +408,7 @@ __global__ __launch_bounds__(256) void norm_join(NormArgs a) {
   q = wave_sum(q);
   if (lane == 0) {
     a.mean[i] = mean;
-    a.rstd[i] = 1.0f / sqrtf(fmaf(q, inv, a.eps));
+    a.rstd[i] = __builtin_amdgcn_rsqf(fmaf(q, inv, a.eps));
   }
 }
 
@@ -352,7 +428,7 @@ template <class E, bool kAct, bool kGate>
 __global__ __launch_bounds__(1024) void norm_apply(NormArgs a) {
   constexpr int V = E::V;
   const Place p = place<E>(a);
-  const Chunk k = chunk_of(a);
+  const Chunk k = chunk_of<true>(a);
   float w[V], b[V], mu[V], rs[V];
   params(a, p, w, b);
   statistics(a, p, k.b, mu, rs);
@@ -360,15 +436,15 @@ __global__ __launch_bounds__(1024) void norm_apply(NormArgs a) {
   for (int i = 0; i < V; ++i) w[i] *= rs[i];
   int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
   const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
-  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+  by_two<E, 1 + kGate>(a, p, k, step, at, {a.x, a.gate, nullptr}, [&](int64_t at, const u32x4* raw) {
     float x[V], z[V] = {};
-    load_vec<E>(a.x + at, x);
-    if (kGate) load_vec<E>(a.gate + at, z);
+    E::unpack(raw[0], x);
+    if (kGate) E::unpack(raw[kGate], z);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       x[i] = activate<E, kAct, kGate>(fmaf(x[i] - mu[i], w[i], b[i]), z[i]);
     store_vec<E>(a.out + at, x);
-  }
+  });
 }
 
 // Per chunk and channel: sum dy, sum dy h.
@@ -383,11 +459,11 @@ __global__ __launch_bounds__(1024) void norm_sums_bwd(NormArgs a) {
   statistics(a, p, k.b, mu, rs);
   int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
   const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
-  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+  by_two<E, 2 + kGate>(a, p, k, step, at, {a.x, a.go, a.gate}, [&](int64_t, const u32x4* raw) {
     float x[V], go[V], z[V] = {};
-    load_vec<E>(a.x + at, x);
-    load_vec<E>(a.go + at, go);
-    if (kGate) load_vec<E>(a.gate + at, z);
+    E::unpack(raw[0], x);
+    E::unpack(raw[1], go);
+    if (kGate) E::unpack(raw[1 + kGate], z);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float h = (x[i] - mu[i]) * rs[i];
@@ -395,7 +471,7 @@ __global__ __launch_bounds__(1024) void norm_sums_bwd(NormArgs a) {
       gb[i] += dy;
       gw[i] = fmaf(dy, h, gw[i]);
     }
-  }
+  });
   float* const part = a.part + (int64_t)blockIdx.x * 2 * a.dim;
   column_sums(a, p, lds, gb, part);
   column_sums(a, p, lds, gw, part + a.dim);
@@ -406,7 +482,7 @@ __global__ __launch_bounds__(1024) void norm_apply_bwd(NormArgs a) {
   constexpr int V = E::V;
   extern __shared__ float lds[];
   const Place p = place<E>(a);
-  const Chunk k = chunk_of(a);
+  const Chunk k = chunk_of<true>(a);
   // the means over the sequence's groups of w dy and w dy h
   float* const sums = lds + 2 * a.dim;
   for (int c = threadIdx.x; c < a.dim; c += blockDim.x) {
@@ -429,11 +505,11 @@ __global__ __launch_bounds__(1024) void norm_apply_bwd(NormArgs a) {
   }
   int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
   const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
-  for (int64_t r = p.row; p.in && r < k.rows; r += a.rows, at += step) {
+  by_two<E, 2 + kGate>(a, p, k, step, at, {a.x, a.go, a.gate}, [&](int64_t at, const u32x4* raw) {
     float x[V], go[V], z[V] = {};
-    load_vec<E>(a.x + at, x);
-    load_vec<E>(a.go + at, go);
-    if (kGate) load_vec<E>(a.gate + at, z);
+    E::unpack(raw[0], x);
+    E::unpack(raw[1], go);
+    if (kGate) E::unpack(raw[1 + kGate], z);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float h = (x[i] - mu[i]) * rs[i];
@@ -442,24 +518,33 @@ __global__ __launch_bounds__(1024) void norm_apply_bwd(NormArgs a) {
     }
     store_vec<E>(a.gx + at, x);
     if (kGate) store_vec<E>(a.ggate + at, z);
-  }
+  });
 }
 
-// Sums over the rows of slabs of a (slabs, rows, cols) array: 64 columns a workgroup, 16 threads each.
-// The first `split` columns go to `a`, the others to `b` (either may be null), slab after slab.
+// Sums over the rows of slabs of a (slabs, rows, cols) array: 16 columns a workgroup, 64 threads each
+// (a row's 64 bytes at a time; 64 columns by 16 threads left most CUs without work: 38 instead of 9 us
+// for 2048 rows of 2048). The first `split` columns go to `to_a`, the others to `to_b` (either may be
+// null), slab after slab.
 __global__ __launch_bounds__(1024) void norm_columns(const float* from, int64_t rows, int cols, int split,
                                                      float* to_a, float* to_b, int blocks) {
-  __shared__ float lds[16][64];
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  __shared__ float lds[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
   const int64_t slab = blockIdx.x / blocks;
-  const int c = (int)(blockIdx.x - slab * blocks) * 64 + x;
+  const int c = (int)(blockIdx.x - slab * blocks) * 16 + x;
   float s = 0.0f;
-  if (c < cols)
-    for (int64_t r = y; r < rows; r += 16) s += from[(slab * rows + r) * cols + c];
+  if (c < cols) {
+    const float* p = from + (slab * rows + y) * cols + c;
+#pragma unroll 8
+    for (int64_t r = y; r < rows; r += 64, p += (int64_t)64 * cols) s += *p;
+  }
   lds[y][x] = s;
   __syncthreads();
+  for (int n = 32; n > 0; n >>= 1) {
+    if (y < n) lds[y][x] += lds[y + n][x];
+    __syncthreads();
+  }
   if (y == 0 && c < cols) {
-    for (int i = 1; i < 16; ++i) s += lds[i][x];
+    s = lds[0][x];
     if (c < split) {
       if (to_a) to_a[slab * split + c] = s;
     } else if (to_b) {
@@ -471,7 +556,8 @@ __global__ __launch_bounds__(1024) void norm_columns(const float* from, int64_t 
 // ------------------------------------------------------------------------------------ host side
 struct Launch {
   NormArgs a;
-  int threads, blocks;  // blocks: of the token kernels
+  int threads, blocks;  // blocks: of the token kernel backward
+  int turns;            // and forward
   bool tokens, aligned;
   size_t lds;
 };
@@ -517,10 +603,11 @@ Launch launch_of(const fpscan_norm* p) {
   // rows of channels and of group sums, and the groups' first values; two such rows at least
   l.lds = ((size_t)a.rows * (a.dim + a.groups) + a.groups) * sizeof(float);
   if (a.rows == 1) l.lds = 2 * (size_t)(a.dim + a.groups) * sizeof(float);
-  // token kernels: a workgroup takes rows in turn, so that the parameters' gradients are summed in
-  // registers first
+  // token by token: workgroups take rows in turn, so that parameters are loaded and their gradients
+  // summed in registers (forward with a workgroup a turn: 65 instead of 24 us for 16384 rows of 1024)
   const int64_t turns = (a.batch + a.rows - 1) / a.rows;
-  l.blocks = (int)(turns < 2048 ? turns : 2048);
+  l.turns = turns < 2048 ? turns : 2048;
+  l.blocks = (int)(turns < 1024 ? turns : 1024);
   // chunks: some thousand workgroups, 8 to 128 rows a thread
   int64_t want = 2048 / a.batch;
   if (want < 1) want = 1;
@@ -581,7 +668,7 @@ int launch(K kernel, const Launch& l, int64_t blocks, hipStream_t stream) {
 
 int columns(const float* from, int64_t slabs, int64_t rows, int dim, float* to_a, float* to_b, int split,
             hipStream_t stream) {
-  const int blocks = (2 * dim + 63) / 64;
+  const int blocks = (2 * dim + 15) / 16;
   norm_columns<<<(unsigned)(slabs * blocks), 1024, 0, stream>>>(from, rows, 2 * dim, split, to_a, to_b,
                                                                blocks);
   return launched();
@@ -629,8 +716,8 @@ int fpscan_norm_fwd(const fpscan_norm* p, const void* x, const float* weight, co
   return by_kind(p, gate != nullptr, [&](auto e, auto act, auto gated) {
     using E = decltype(e);
     if (l.tokens)
-      return l.aligned ? launch(norm_tokens<E, act.value, gated.value, true>, l, l.blocks, s)
-                       : launch(norm_tokens<E, act.value, gated.value, false>, l, l.blocks, s);
+      return l.aligned ? launch(norm_tokens<E, act.value, gated.value, true>, l, l.turns, s)
+                       : launch(norm_tokens<E, act.value, gated.value, false>, l, l.turns, s);
     int st = launch(norm_stats<E>, l, a.batch * a.chunks, s);
     if (st != FPSCAN_OK) return st;
     norm_join<<<(unsigned)((a.batch * a.groups + 3) / 4), 256, 0, s>>>(a);
