@@ -29,6 +29,7 @@ struct NormArgs {
   int64_t batch, seqlen, chunk_rows, chunks;
   int dim, groups, width, vecs, rows, lanes;  // rows: of a workgroup at a time
   float eps;
+  bool wide;  // weight and bias are 16-byte aligned
 };
 
 template <class E>
@@ -64,13 +65,44 @@ __device__ __forceinline__ Place place(const NormArgs& a) {
   return {row, vec * E::V, row < a.rows};
 }
 
+// V floats of a thread's channels, four at a time where `wide` (16-byte aligned).
+template <int V>
+__device__ __forceinline__ void channel_values(const float* from, bool wide, const Place& p, float none,
+                                               float (&x)[V]) {
+  if (from == nullptr || !p.in) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = none;
+  } else if (wide) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(from + p.c + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i + j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = from[p.c + i];
+  }
+}
+
 // Weights and biases of a thread's channels; 1 and 0 where there are none.
 template <int V>
 __device__ __forceinline__ void params(const NormArgs& a, const Place& p, float (&w)[V], float (&b)[V]) {
+  channel_values(a.weight, a.wide, p, 1.0f, w);
+  channel_values(a.bias, a.wide, p, 0.0f, b);
+}
+
+// The groups of a thread's channels: one division, then counting.
+template <int V>
+__device__ __forceinline__ void groups_of(const NormArgs& a, const Place& p, int (&g)[V]) {
+  int at = p.in ? p.c / a.width : 0, left = (at + 1) * a.width - p.c;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    w[i] = a.weight && p.in ? a.weight[p.c + i] : 1.0f;
-    b[i] = a.bias && p.in ? a.bias[p.c + i] : 0.0f;
+    g[i] = at;
+    if (--left == 0) {
+      left = a.width;
+      at += p.in ? 1 : 0;
+    }
   }
 }
 
@@ -132,8 +164,7 @@ struct GroupSums {
   bool first;    // kAligned: whether the group begins with this thread
 
   __device__ __forceinline__ GroupSums(const NormArgs& a, const Place& p) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) group[i] = (p.c + i) / a.width;
+    groups_of(a, p, group);
     first = p.c == group[0] * a.width;
   }
   __device__ __forceinline__ void sum(const NormArgs& a, const Place& p, float* lds, const float (&x)[V],
@@ -181,6 +212,19 @@ __device__ __forceinline__ void column_sums(const NormArgs& a, const Place& p, f
 }
 
 // ------------------------------------------------------------------------------ token by token
+// A thread's vectors of the next rows on their way; zeros past the last.
+template <class E, int kTensors>
+struct TokenRows {
+  u32x4 raw[kTensors];
+  __device__ __forceinline__ void load(const NormArgs& a, const Place& p, int64_t r0,
+                                       const char* const (&from)[3]) {
+    const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
+    const bool in = p.in && r < a.batch;
+#pragma unroll
+    for (int i = 0; i < kTensors; ++i) raw[i] = in ? raw_vec(from[i] + at) : u32x4{};
+  }
+};
+
 template <class E, bool kAct, bool kGate, bool kAligned>
 __global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
   constexpr int V = E::V;
@@ -191,12 +235,16 @@ __global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
   float w[V], b[V];
   params(a, p, w, b);
   const float inv = 1.0f / (float)a.width;
-  for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
+  const int64_t turn = (int64_t)gridDim.x * a.rows;
+  TokenRows<E, 1 + kGate> next;
+  next.load(a, p, (int64_t)blockIdx.x * a.rows, {a.x, a.gate, nullptr});
+  for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += turn) {
     const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
     const bool in = p.in && r < a.batch;
-    float x[V] = {}, z[V] = {}, q[V], s[G::n], mu[G::n], off[G::n];
-    if (in) load_vec<E>(a.x + at, x);
-    if (kGate && in) load_vec<E>(a.gate + at, z);
+    float x[V], z[V] = {}, q[V], s[G::n], mu[G::n], off[G::n];
+    E::unpack(next.raw[0], x);
+    if (kGate) E::unpack(next.raw[kGate], z);
+    next.load(a, p, r0 + turn, {a.x, a.gate, nullptr});
     groups.sum(a, p, lds, x, mu);
 #pragma unroll
     for (int i = 0; i < G::n; ++i) mu[i] *= inv;
@@ -235,20 +283,33 @@ __global__ __launch_bounds__(1024) void norm_tokens_bwd(NormArgs a) {
   float w[V], b[V], gw[V] = {}, gb[V] = {};
   params(a, p, w, b);
   const float inv = 1.0f / (float)a.width;
-  for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += (int64_t)gridDim.x * a.rows) {
+  const int64_t turn = (int64_t)gridDim.x * a.rows;
+  TokenRows<E, 2 + kGate> next;
+  float next_mu[G::n], next_rs[G::n];
+  auto load = [&](int64_t r0) {
+    next.load(a, p, r0, {a.x, a.go, a.gate});
+    const bool in = p.in && r0 + p.row < a.batch;
+    const int64_t g = (r0 + p.row) * a.groups;
+#pragma unroll
+    for (int i = 0; i < G::n; ++i) {
+      next_mu[i] = in ? a.mean[g + groups.group[i]] : 0.0f;
+      next_rs[i] = in ? a.rstd[g + groups.group[i]] : 0.0f;
+    }
+  };
+  load((int64_t)blockIdx.x * a.rows);
+  for (int64_t r0 = (int64_t)blockIdx.x * a.rows; r0 < a.batch; r0 += turn) {
     const int64_t r = r0 + p.row, at = (r * a.dim + p.c) * E::kSize;
     const bool in = p.in && r < a.batch;
-    float x[V] = {}, z[V] = {}, go[V] = {}, mu[G::n] = {}, rs[G::n] = {}, m1[G::n], m2[G::n], t[V];
-    if (in) {
-      load_vec<E>(a.x + at, x);
-      load_vec<E>(a.go + at, go);
-      if (kGate) load_vec<E>(a.gate + at, z);
+    float x[V], z[V] = {}, go[V], mu[G::n], rs[G::n], m1[G::n], m2[G::n], t[V];
+    E::unpack(next.raw[0], x);
+    E::unpack(next.raw[1], go);
+    if (kGate) E::unpack(next.raw[1 + kGate], z);
 #pragma unroll
-      for (int i = 0; i < G::n; ++i) {
-        mu[i] = a.mean[r * a.groups + groups.group[i]];
-        rs[i] = a.rstd[r * a.groups + groups.group[i]];
-      }
+    for (int i = 0; i < G::n; ++i) {
+      mu[i] = next_mu[i];
+      rs[i] = next_rs[i];
     }
+    load(r0 + turn);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       x[i] = (x[i] - mu[G::at(i)]) * rs[G::at(i)];
@@ -350,16 +411,18 @@ __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
   const float inv = n > 0.0f ? 1.0f / n : 0.0f;
   // means are taken from the group's first value, so that sums of means far from 0 lose nothing
   float* const base = sums + a.rows * a.groups;
+  int group[V];
+  groups_of(a, p, group);
   if (p.in && p.row == 0)
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if ((p.c + i) % a.width == 0) base[(p.c + i) / a.width] = x0[i];
+      if (p.c + i == group[i] * a.width) base[group[i]] = x0[i];
   __syncthreads();
   if (p.in)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       q[i] = fmaf(-s[i] * inv, s[i], q[i]);
-      x0[i] = fmaf(s[i], inv, x0[i] - base[(p.c + i) / a.width]);  // of the thread's values
+      x0[i] = fmaf(s[i], inv, x0[i] - base[group[i]]);  // of the thread's values
       lds[p.row * a.dim + p.c + i] = n * x0[i];
     }
   const float all = 1.0f / ((float)k.rows * (float)a.width);
@@ -379,7 +442,7 @@ __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
     if (turn == 0 && p.in)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float d = x0[i] - sums[(p.c + i) / a.width];
+        const float d = x0[i] - sums[group[i]];
         lds[p.row * a.dim + p.c + i] = fmaf(n * d, d, q[i]);
       }
   }
@@ -416,11 +479,12 @@ __global__ __launch_bounds__(256) void norm_join(NormArgs a) {
 template <int V>
 __device__ __forceinline__ void statistics(const NormArgs& a, const Place& p, int64_t b, float (&mu)[V],
                                            float (&rs)[V]) {
+  int g[V];
+  groups_of(a, p, g);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int64_t g = b * a.groups + (p.in ? (p.c + i) / a.width : 0);
-    mu[i] = a.mean[g];
-    rs[i] = a.rstd[g];
+    mu[i] = a.mean[b * a.groups + g[i]];
+    rs[i] = a.rstd[b * a.groups + g[i]];
   }
 }
 
@@ -497,11 +561,12 @@ __global__ __launch_bounds__(1024) void norm_apply_bwd(NormArgs a) {
   params(a, p, w, b);
   statistics(a, p, k.b, mu, rs);
   const float inv = 1.0f / ((float)a.seqlen * (float)a.width);
+  int group[V];
+  groups_of(a, p, group);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int g = p.in ? (p.c + i) / a.width : 0;
-    m1[i] = sums[g] * inv;
-    m2[i] = sums[a.groups + g] * inv;
+    m1[i] = sums[group[i]] * inv;
+    m2[i] = sums[a.groups + group[i]] * inv;
   }
   int64_t at = ((k.b * a.seqlen + k.first + p.row) * a.dim + p.c) * E::kSize;
   const int64_t step = (int64_t)a.rows * a.dim * E::kSize;
@@ -608,12 +673,12 @@ Launch launch_of(const fpscan_norm* p) {
   const int64_t turns = (a.batch + a.rows - 1) / a.rows;
   l.turns = turns < 2048 ? turns : 2048;
   l.blocks = (int)(turns < 1024 ? turns : 1024);
-  // chunks: some thousand workgroups, 8 to 128 rows a thread
+  // chunks: some thousand workgroups, 4 to 128 rows a thread
   int64_t want = 2048 / a.batch;
   if (want < 1) want = 1;
   int64_t each = (a.seqlen + want - 1) / want;
   each = (each + a.rows - 1) / a.rows;
-  each = each < 8 ? 8 : each > 128 ? 128 : each;
+  each = each < 4 ? 4 : each > 128 ? 128 : each;
   a.chunk_rows = each * a.rows;
   a.chunks = (a.seqlen + a.chunk_rows - 1) / a.chunk_rows;
   return l;
@@ -707,6 +772,7 @@ int fpscan_norm_fwd(const fpscan_norm* p, const void* x, const float* weight, co
   a.gate = static_cast<const char*>(gate);
   a.weight = weight;
   a.bias = bias;
+  a.wide = aligned16({weight, bias});
   a.out = static_cast<char*>(out);
   if (stats) {
     a.mean = stats;
@@ -749,6 +815,7 @@ int fpscan_norm_bwd(const fpscan_norm* p, const void* x, const float* weight, co
   a.go = static_cast<const char*>(grad_out);
   a.weight = weight;
   a.bias = bias;
+  a.wide = aligned16({weight, bias});
   a.gx = static_cast<char*>(grad_x);
   a.ggate = static_cast<char*>(grad_gate);
   a.mean = const_cast<float*>(stats);
