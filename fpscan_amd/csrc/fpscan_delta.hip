@@ -44,9 +44,10 @@ struct DeltaArgs {
   char *ds, *y;       // the same of dS' and Y
   float *dss, *ys, *gs;  // gs: of dO
   char *gq, *gk, *gg, *gbeta;
+  float *tn, *tm, *ts;  // per segment: what it adds to a state, its map of states, the state before it
   const int32_t* slots;
-  int64_t L, chunks, heads_total, nslots;
-  int H, R, Dk, Dv, vblocks;
+  int64_t L, chunks, heads_total, nslots, seg_chunks;
+  int H, R, Dk, Dv, vblocks, segs;
   float scale;
 };
 
@@ -345,7 +346,8 @@ struct Copies {
 };
 
 // A chunk on its way from memory to LDS, in the registers of kBring waves. `value` is V or dO.
-template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring>
+// kReads: also Q and M, which a walk that only hands a state on does not read.
+template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring, bool kReads>
 struct Brought {
   using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
   RowBlocks<E, KD, kBring> k, q;
@@ -355,14 +357,16 @@ struct Brought {
   f32x4 gb;
 
   __device__ __forceinline__ void load(const DeltaArgs& a, const Heads& value, int64_t bh, int64_t b,
-                                       int64_t h, int64_t hk, int col0, int w, int64_t c) {
+                                       int64_t h, int64_t hk, int col0, int dim, int w, int64_t c) {
     const int64_t ch = bh * a.chunks + c, t0 = c * kChunk;
     const int rows = rows_left(a.L, t0);
     k.load(a.k, b, hk, t0, rows, a.Dk, 0, w);
     n.load(a.n + ch * kTerms * kTriBytes, w);
-    v.load(value, b, h, t0, rows, a.Dv, col0, w);
-    q.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
-    m.load(a.m + ch * kOut * kTriBytes, w);
+    v.load(value, b, h, t0, rows, dim, col0, w);
+    if (kReads) {
+      q.load(a.q, b, hk, t0, rows, a.Dk, 0, w);
+      m.load(a.m + ch * kOut * kTriBytes, w);
+    }
     gb = reinterpret_cast<const f32x4*>(a.gb)[ch * kChunk + (threadIdx.x & 63)];
   }
   __device__ __forceinline__ void store(char* lds, int w) const {
@@ -370,8 +374,10 @@ struct Brought {
     k.store(lds + C::k, w);
     n.store(lds + C::n, w);
     v.store(lds + C::v, w);
-    q.store(lds + C::q, w);
-    m.store(lds + C::m, w);
+    if (kReads) {
+      q.store(lds + C::q, w);
+      m.store(lds + C::m, w);
+    }
     if (w == 0) {
       const float hi = readlane(gb[0], 63), lo = readlane(gb[1], 63);
       reinterpret_cast<float*>(lds + C::gam)[lane] = expf(gb[0]) * (1.0f + gb[1]);
@@ -381,28 +387,28 @@ struct Brought {
   }
 };
 
-// The waves that bring chunks first, first + step .. to LDS: a chunk's loads are under way while the
-// one before is waited for and stored (past the last, it is loaded again and dropped).
-template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring>
+// The waves that bring chunks first, first + step .. (`count` of them) to LDS: a chunk's loads are under
+// way while the one before is waited for and stored (past the last, it is loaded again and dropped).
+// Of `value` the columns col0 .. below `dim`, zeros beyond.
+template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring, bool kReads>
 __device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const Heads& value, int64_t bh,
-                                      int64_t b, int64_t h, int64_t hk, int col0, int w, int64_t first,
-                                      int64_t step) {
+                                      int64_t b, int64_t h, int64_t hk, int col0, int dim, int w,
+                                      int64_t first, int64_t step, int64_t count) {
   using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
-  Brought<E, KD, kTerms, kOut, kWaves, kBring> even, odd;
-  const int64_t end = a.chunks - 1;
-  auto chunk = [&](int64_t i) { return first + step * (i < end ? i : end); };
+  Brought<E, KD, kTerms, kOut, kWaves, kBring, kReads> even, odd;
+  auto chunk = [&](int64_t i) { return first + step * (i < count ? i : count - 1); };
   auto pass = [&](const auto& x, int64_t i) {
     if (C::kBuffers == 1 && i > 0) lds_barrier();  // the chunk before is read
     x.store(buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0), w);
     lds_barrier();
   };
-  even.load(a, value, bh, b, h, hk, col0, w, chunk(0));
-  for (int64_t i = 0; i < a.chunks; i += 2) {
-    odd.load(a, value, bh, b, h, hk, col0, w, chunk(i + 1));
+  even.load(a, value, bh, b, h, hk, col0, dim, w, chunk(0));
+  for (int64_t i = 0; i < count; i += 2) {
+    odd.load(a, value, bh, b, h, hk, col0, dim, w, chunk(i + 1));
     in_order();
     pass(even, i);
-    if (i + 1 >= a.chunks) break;
-    even.load(a, value, bh, b, h, hk, col0, w, chunk(i + 2));
+    if (i + 1 >= count) break;
+    even.load(a, value, bh, b, h, hk, col0, dim, w, chunk(i + 2));
     in_order();
     pass(odd, i + 1);
   }
@@ -533,28 +539,112 @@ __device__ __forceinline__ Rsrc rows_rsrc(const char* p, int64_t b, int64_t L, i
                   ((rows_left(L, t0) - 1) * heads + 1) * dim * E::kSize);
 }
 
-// A walk's workgroup: which head and value columns. The workgroups of one head, which read the same K,
-// Q, N and M, are eight apart: on one XCD.
+// Segments. With few heads, a walk leaves most CUs idle. A segment of chunks maps the state before it
+// to the one after it by S -> M S + N, for all value columns alike; so a first walk (kMap) takes every
+// segment but the last at once, the value columns from a state of zero (N) and KD more columns from the
+// unit matrix with values of zero (M); delta_join hands the states from segment to segment; and then
+// all segments are walked at once from their own states. Backward likewise, with dS'.
+//
+// A walk's workgroup: which segment, head and columns. The workgroups of one head, which read the same
+// K, Q, N and M, are eight apart: on one XCD.
 struct Place {
   int64_t bh, b, h, hk;
-  int col0;
+  int64_t first, count;  // the segment's chunks, in the walk's order
+  int seg, col0, dim;    // value columns col0 .. below dim
+  bool unit;             // kMap: columns col0 .. of the unit matrix instead
 };
-template <int kWaves>
-__device__ __forceinline__ Place place_of(const DeltaArgs& a) {
-  const int64_t id = blockIdx.x, bh = id / (8 * a.vblocks) * 8 + id % 8, b = bh / a.H, h = bh - b * a.H;
-  return {bh, b, h, h / a.R, (int)(id / 8 % a.vblocks) * 16 * kWaves};
+template <int kWaves, bool kMap>
+__device__ __forceinline__ Place place_of(const DeltaArgs& a, int key_dim) {
+  const int units = kMap ? key_dim / (16 * kWaves) : 0, vb_all = a.vblocks + units;
+  const int64_t per = (a.heads_total + 7) / 8 * 8 * vb_all;  // workgroups of a segment
+  Place p;
+  p.seg = (int)(blockIdx.x / per);
+  const int64_t id = blockIdx.x - p.seg * per;
+  p.bh = id / (8 * vb_all) * 8 + id % 8;
+  p.b = p.bh / a.H;
+  p.h = p.bh - p.b * a.H;
+  p.hk = p.h / a.R;
+  const int vb = (int)(id / 8 % vb_all);
+  p.unit = kMap && vb >= a.vblocks;
+  p.col0 = (p.unit ? vb - a.vblocks : vb) * 16 * kWaves;
+  p.dim = p.unit ? 0 : a.Dv;
+  p.first = p.seg * a.seg_chunks;
+  const int64_t left = a.chunks - p.first;
+  p.count = left < a.seg_chunks ? left : a.seg_chunks;
+  return p;
 }
 
-template <class E, int KD, int kTerms, bool kSave, int kWaves, int kBring>
+// A state's columns (of one lane) between the registers and a segment's place in memory.
+template <int KD>
+__device__ __forceinline__ float* segment_state(float* base, const DeltaArgs& a, const Place& p) {
+  return base + (p.bh * a.segs + p.seg) * KD * ((a.Dv + 31) / 32 * 32);
+}
+template <int KD>
+__device__ __forceinline__ void write_map(const DeltaArgs& a, const Place& p, int col, int lg,
+                                          const f32x4 (&S)[KD / 16]) {
+  const int stride = (a.Dv + 31) / 32 * 32;
+  float* const n = segment_state<KD>(a.tn, a, p);
+  float* const m = a.tm + ((p.bh * a.segs + p.seg) * KD + col) * KD;
+#pragma unroll
+  for (int t = 0; t < KD / 16; ++t) {
+    if (p.unit) {
+      *reinterpret_cast<f32x4*>(m + key_col(t, 4 * lg)) = S[t];
+    } else if (col < stride) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) n[key_col(t, 4 * lg + r) * stride + col] = S[t][r];
+    }
+  }
+}
+
+// States from segment to segment, 16 value columns a workgroup: ts of each, from `state` or zero.
+template <int KD>
+__global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
+  __shared__ __attribute__((aligned(16))) float S[2][KD][16];
+  constexpr int kParts = 256 / KD, kCols = 16 / kParts;  // threads and columns a row
+  const int stride = (a.Dv + 31) / 32 * 32, blocks = stride / 16;
+  const int64_t bh = blockIdx.x / blocks;
+  const int col0 = (int)(blockIdx.x - bh * blocks) * 16, row = threadIdx.x % KD,
+            c0 = threadIdx.x / KD * kCols;
+  float x[kCols];
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    const int col = col0 + c0 + i;
+    x[i] = a.state && row < a.Dk && col < a.Dv ? a.state[(bh * a.Dk + row) * a.Dv + col] : 0.0f;
+  }
+  for (int p = 0;; ++p) {
+    const int64_t at = bh * a.segs + p;
+    float* const to = a.ts + (at * KD + row) * stride + col0 + c0;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      to[i] = x[i];
+      S[p & 1][row][c0 + i] = x[i];
+    }
+    if (p + 1 == a.segs) break;
+    __syncthreads();
+    const float* const n = a.tn + (at * KD + row) * stride + col0 + c0;
+    const float* const m = a.tm + at * KD * KD + row;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) x[i] = n[i];
+#pragma unroll 16
+    for (int k = 0; k < KD; ++k) {
+      const float f = m[k * KD];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) x[i] = fmaf(f, S[p & 1][k][c0 + i], x[i]);
+    }
+  }
+}
+
+template <class E, int KD, int kTerms, bool kSave, bool kMap, int kWaves, int kBring>
 __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs a) {
   constexpr int kOut = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
   using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
   extern __shared__ __attribute__((aligned(16))) char buffers[];
-  const Place p = place_of<kWaves>(a);
+  const Place p = place_of<kWaves, kMap>(a, KD);
   if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
   if (w >= kWaves) {
-    bring<E, KD, kTerms, kOut, kWaves, kBring>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves, 0, 1);
+    bring<E, KD, kTerms, kOut, kWaves, kBring, !kMap>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, p.dim,
+                                                      w - kWaves, p.first, 1, p.count);
     return;
   }
   const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2, col = p.col0 + key_col(w, li);
@@ -566,13 +656,18 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = key_col(t, 4 * lg + r);
-      S[t][r] = a.state && in && row < a.Dk ? a.state[(p.bh * a.Dk + row) * a.Dv + col] : 0.0f;
+      if (kMap)
+        S[t][r] = p.unit && row == col ? 1.0f : 0.0f;
+      else if (a.segs > 1)
+        S[t][r] = col < tiles * 16 ? segment_state<KD>(a.ts, a, p)[row * (tiles * 16) + col] : 0.0f;
+      else
+        S[t][r] = a.state && in && row < a.Dk ? a.state[(p.bh * a.Dk + row) * a.Dv + col] : 0.0f;
     }
 
   lds_barrier();
-  for (int64_t c = 0; c < a.chunks; ++c) {
-    const int64_t ch = p.bh * a.chunks + c, t0 = c * kChunk;
-    const char* const lds = buffers + (C::kBuffers == 2 && (c & 1) ? C::size : 0);
+  for (int64_t it = 0; it < p.count; ++it) {
+    const int64_t c = p.first + it, ch = p.bh * a.chunks + c, t0 = c * kChunk;
+    const char* const lds = buffers + (C::kBuffers == 2 && (it & 1) ? C::size : 0);
     // operands of the next step are on their way while a step's products run
     auto keys_at = [&](int step, bf16x8 (&f)[4][NI]) {  // K and Q in turn, 32 key columns a step
 #pragma unroll
@@ -606,7 +701,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
     in_order();
 #pragma unroll
     for (int i = 0; i < C::kBlocks; ++i) {
-      keys_at(i + 1 < C::kBlocks ? 2 * i + 2 : 1, ring[(i + 1) & 1]);
+      if (i + 1 < C::kBlocks || !kMap) keys_at(i + 1 < C::kBlocks ? 2 * i + 2 : 1, ring[(i + 1) & 1]);
       if (i + 1 < C::kBlocks) {
         split(join(S[2 * i + 2], S[2 * i + 3]), sp[i + 1]);
         settle(sp[i + 1]);
@@ -625,9 +720,9 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
     f32x4 gam[4], beta[4], end[4];
 #pragma unroll
     for (int i = 0; i < C::kBlocks; ++i) {
-      if (i + 1 < C::kBlocks)
+      if (i + 1 < C::kBlocks && !kMap)
         keys_at(2 * i + 3, ring[(i + 1 + C::kBlocks) & 1]);
-      else if (kRoom)
+      else if (kRoom && i + 1 == C::kBlocks)
         triangle(lds + C::n, lane, nf);
       if (i == 0)
 #pragma unroll
@@ -649,7 +744,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
         split(join(u[2 * s], u[2 * s + 1]), up[s]);
         settle(up[s]);
       }
-      mma_tiles<kOut>(ring[(i + C::kBlocks) & 1], sp[i], o);
+      if (!kMap) mma_tiles<kOut>(ring[(i + C::kBlocks) & 1], sp[i], o);
       interleave<kO, 5>();
     }
     // N (beta R), meanwhile what of the state and the output needs no more than a factor
@@ -662,13 +757,13 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) o[mt] *= gam[mt] * a.scale;
     settle(S);
-    settle(o);
-    if (kRoom) triangle(lds + C::m, lane, mf);
+    if (!kMap) settle(o);
+    if (kRoom && !kMap) triangle(lds + C::m, lane, mf);
     mma_triangle<kTerms>(nf, up, y);
     interleave<6 * products(kTerms, kTerms, kTerms), 4>();
     // U, its planes and those of what it adds to the state
     bf16x8 uo[2][kOut];
-    if (!kRoom) triangle(lds + C::m, lane, mf);
+    if (!kRoom && !kMap) triangle(lds + C::m, lane, mf);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) end[mt] = row_of(C::end, mt);
 #pragma unroll
@@ -678,10 +773,12 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
         x[mt] -= y[mt];
         u[mt] = beta[mt] * x[mt];
       }
-      split(join(u[2 * s], u[2 * s + 1]), uo[s]);
+      if (!kMap) split(join(u[2 * s], u[2 * s + 1]), uo[s]);
     }
-    settle(uo[0]);
-    settle(uo[1]);
+    if (!kMap) {
+      settle(uo[0]);
+      settle(uo[1]);
+    }
     in_order();
     // M U, meanwhile the planes for the state
     steps_at(0, ring[0]);
@@ -690,26 +787,29 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
       split(join(u[2 * s] * end[2 * s], u[2 * s + 1] * end[2 * s + 1]), up[s]);
       settle(up[s]);
     }
-    mma_triangle<kOut>(mf, uo, o);
+    if (!kMap) mma_triangle<kOut>(mf, uo, o);
     interleave<6 * products(kOut, kOut, kOut), 4>();
     // the state, meanwhile the output
 #pragma unroll
     for (int i = 0; i < kUpdates; ++i) {
       if (i + 1 < kUpdates) steps_at(i + 1, ring[(i + 1) & 1]);
-      if (i == 0) turn_in<E>(turn, o, lane);
-      if (i + 1 == kUpdates) turn_out<E>(rows_rsrc<E>(a.out, p.b, a.L, t0, a.H, p.h, a.Dv), a.H * a.Dv * E::kSize, a.Dv, p.col0, w,
+      if (!kMap && i == 0) turn_in<E>(turn, o, lane);
+      if (!kMap && i + 1 == kUpdates)
+        turn_out<E>(rows_rsrc<E>(a.out, p.b, a.L, t0, a.H, p.h, a.Dv), a.H * a.Dv * E::kSize, a.Dv, p.col0, w,
                     turn, o, lane);
       if (kSave && i == kUpdates / 2 - 1)
         keep<E, 2>(a.e, a.es, ch * tiles + tile, tile < tiles, x, lane);
       mma_tiles<kTerms>(ring[i & 1], up[i & 1], &S[4 * (i / 2)]);
       interleave<kS, 4>();
     }
-    if (c + 1 < a.chunks) {
+    if (it + 1 < p.count) {
       if (C::kBuffers == 1) lds_barrier();  // this chunk is read
       lds_barrier();                        // the next one is there
     }
   }
-  if (a.state && in)
+  if (kMap)
+    write_map<KD>(a, p, col, lg, S);
+  else if (a.state && in && p.seg + 1 == a.segs)
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -721,25 +821,36 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
 
 // Backward walk, the same way: a wave owns 16 columns of dS' and gives dV, and for the gradients of q
 // and k the dS' and Y of every chunk.
-template <class E, int KD, int kWaves, int kBring>
+template <class E, int KD, bool kMap, int kWaves, int kBring>
 __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(DeltaArgs a) {
   constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
   using C = ChunkLds<E, KD, kT, kT, kWaves>;
   extern __shared__ __attribute__((aligned(16))) char buffers[];
-  const Place p = place_of<kWaves>(a);
+  const Place p = place_of<kWaves, kMap>(a, KD);
   if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), lg = lane >> 4;
   if (w >= kWaves) {
-    bring<E, KD, kT, kT, kWaves, kBring>(buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, w - kWaves,
-                                 a.chunks - 1, -1);
+    bring<E, KD, kT, kT, kWaves, kBring, true>(buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, p.dim,
+                                               w - kWaves, a.chunks - 1 - p.first, -1, p.count);
     return;
   }
-  const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2;
+  const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2, col = p.col0 + key_col(w, lane & 15);
 
   f32x4 dS[KT] = {};
+  if (kMap || a.segs > 1)
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = key_col(t, 4 * lg + r);
+        if (kMap)
+          dS[t][r] = p.unit && row == col ? 1.0f : 0.0f;
+        else
+          dS[t][r] = col < tiles * 16 ? segment_state<KD>(a.ts, a, p)[row * (tiles * 16) + col] : 0.0f;
+      }
   lds_barrier();
-  for (int64_t i = 0; i < a.chunks; ++i) {
-    const int64_t c = a.chunks - 1 - i, ch = p.bh * a.chunks + c, t0 = c * kChunk;
+  for (int64_t i = 0; i < p.count; ++i) {
+    const int64_t c = a.chunks - 1 - p.first - i, ch = p.bh * a.chunks + c, t0 = c * kChunk;
     const char* const lds = buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0);
     auto keys_at = [&](int step, bf16x8 (&f)[4][NI]) {
 #pragma unroll
@@ -775,7 +886,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
     }
     in_order();
     // M^T dO, meanwhile dS' is kept
-    if constexpr (kept_size<E>() == 2) {
+    if constexpr (kept_size<E>() == 2 && !kMap) {
       // the scale at which dO's 16 columns are fp16, as keep's
       float most = 0.0f;
 #pragma unroll
@@ -791,7 +902,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
     keys_at(0, ring[0]);
     split(join(dS[0], dS[1]), sp[0]);
     settle(sp[0]);
-    keep<E, KT / 2>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
+    if (!kMap) keep<E, KT / 2>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
     mma_triangle_t<kT>(mf, vp, y);
     interleave<6 * products(kT, NI, kT), 5>();
     // K dS', meanwhile the planes of scale exp(G) dO
@@ -857,14 +968,14 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
 #pragma unroll
     for (int j = KT / 2; j < KT; ++j) {
       if (j + 1 < KT) steps_at(j + 1, ring[(C::kBlocks + j + 1) & 1]);
-      if (j == KT / 2) {
+      if (!kMap && j == KT / 2) {
         f32x4 v[4];
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
         turn_in<E>(turn, v, lane);
       }
-      if (j + 1 == KT / 4 * 3) keep<E, 2>(a.y, a.ys, ch * tiles + tile, tile < tiles, u, lane);
-      if (j + 1 == KT) {
+      if (!kMap && j + 1 == KT / 4 * 3) keep<E, 2>(a.y, a.ys, ch * tiles + tile, tile < tiles, u, lane);
+      if (!kMap && j + 1 == KT) {
         f32x4 v[4];
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
@@ -874,11 +985,12 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
       mma_tiles<kT>(ring[(C::kBlocks + j) & 1], up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
       interleave<kS, 4>();
     }
-    if (c > 0) {
+    if (i + 1 < p.count) {
       if (C::kBuffers == 1) lds_barrier();
       lds_barrier();
     }
   }
+  if (kMap) write_map<KD>(a, p, col, lg, dS);
 }
 
 // ------------------------------------------------------------------- gradients of q, k, g, beta
@@ -1456,12 +1568,42 @@ struct Carver {
   }
 };
 
+// Segments of a walk: as many as walk side by side on the CUs (two tiles of 16 value columns each), if
+// that is worth it. In microseconds, as measured: a chunk of a walk 3, of a map 2 (on twice the
+// columns), a segment's join 3, and 12 for the two launches more.
+void choose_segments(DeltaArgs& a) {
+  const int64_t tiles = a.heads_total * ((a.Dv + 31) / 32 * 2);
+  a.segs = 1;
+  a.seg_chunks = a.chunks;
+  int64_t best = 3 * a.chunks;
+  for (int64_t n = 2; n * tiles <= 512 && n <= a.chunks; ++n) {
+    const int64_t each = (a.chunks + n - 1) / n, segs = (a.chunks + each - 1) / each;
+    const int64_t cost = 5 * each + 3 * segs + 12;
+    if (segs > 1 && cost < best) {
+      best = cost;
+      a.segs = (int)segs;
+      a.seg_chunks = each;
+    }
+  }
+}
+
+void carve_segments(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
+  choose_segments(a);
+  if (a.segs == 1) return;
+  const size_t n = (size_t)a.heads_total * a.segs * padded_key_dim(p);
+  const size_t cols = (size_t)(a.Dv + 31) / 32 * 32;
+  a.tn = reinterpret_cast<float*>(w.take(n * cols * 4));
+  a.ts = reinterpret_cast<float*>(w.take(n * cols * 4));
+  a.tm = reinterpret_cast<float*>(w.take(n * padded_key_dim(p) * 4));
+}
+
 // G, beta, N and M of every chunk.
 void carve_prep(Carver& w, DeltaArgs& a, const fpscan_delta* p, bool keeps_state) {
   const size_t n = (size_t)(a.heads_total * a.chunks);
   a.gb = w.take(n * kChunk * 16);
   a.n = w.take(n * terms_state(p, keeps_state) * kTriBytes);
   a.m = w.take(n * terms_out(p) * kTriBytes);
+  carve_segments(w, a, p);
 }
 
 // What a forward keeps for the gradients; the states and E, of 16 value columns a block.
@@ -1484,6 +1626,7 @@ void carve_bwd(Carver& w, DeltaArgs& a, const fpscan_delta* p) {
   a.dss = reinterpret_cast<float*>(w.take(blocks * 4));
   a.ys = reinterpret_cast<float*>(w.take(blocks * 4));
   a.gs = reinterpret_cast<float*>(w.take(blocks * 4));
+  carve_segments(w, a, p);
 }
 
 template <class F>
@@ -1508,58 +1651,80 @@ int allow_lds(K kernel, int bytes) {
              ? FPSCAN_OK : FPSCAN_ERR_LAUNCH;
 }
 
-// A walk's grid, `waves` times 16 value columns a workgroup: groups of eight heads.
-unsigned walk_grid(DeltaArgs& a, int waves) {
-  a.vblocks = (a.Dv + 16 * waves - 1) / (16 * waves);
-  return (unsigned)((a.heads_total + 7) / 8 * 8 * a.vblocks);
-}
-
 // Waves of a walk's workgroup: two that compute and four that bring while that fills no more than the
 // CUs, four and four beyond (8 heads of 8 sequences, width 128, bf16: 117 us for 2048 steps against
 // 122; 80 heads, fp16, 777 steps: 88 us against 139). fp32 has LDS for two and registers for two more.
-bool walk_narrow(const DeltaArgs& a) { return a.heads_total * ((a.Dv + 63) / 64) <= 128; }
+bool walk_narrow(const DeltaArgs& a) { return a.heads_total * a.segs * ((a.Dv + 63) / 64) <= 128; }
 
-template <class E, int KD, int kTerms, bool kSave, int kWaves, int kBring>
+
+// A walk's grid: segments (all but the last for a map) of groups of eight heads.
+template <int KD, int kWaves, bool kMap>
+unsigned walk_grid(DeltaArgs& a) {
+  a.vblocks = (a.Dv + 16 * kWaves - 1) / (16 * kWaves);
+  return (unsigned)((a.heads_total + 7) / 8 * 8 * (a.vblocks + (kMap ? KD / (16 * kWaves) : 0)) *
+                    (kMap ? a.segs - 1 : a.segs));
+}
+
+template <class E, int KD, int kTerms, bool kSave, bool kMap, int kWaves, int kBring>
 int launch_forward(DeltaArgs& a, hipStream_t stream) {
   using C = ChunkLds<E, KD, kTerms, out_terms<E>(), kWaves>;
-  const auto walk = delta_chunks<E, KD, kTerms, kSave, kWaves, kBring>;
+  const auto walk = delta_chunks<E, KD, kTerms, kSave, kMap, kWaves, kBring>;
   const int st = allow_lds(walk, C::total);
   if (st != FPSCAN_OK) return st;
-  const unsigned grid = walk_grid(a, kWaves);
+  const unsigned grid = walk_grid<KD, kWaves, kMap>(a);
   walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
+  return launched();
+}
+
+template <class E, int KD, bool kMap, int kWaves, int kBring>
+int launch_backward(DeltaArgs& a, hipStream_t stream) {
+  using C = ChunkLds<E, KD, out_terms<E>(), out_terms<E>(), kWaves>;
+  const auto walk = delta_chunks_bwd<E, KD, kMap, kWaves, kBring>;
+  const int st = allow_lds(walk, C::total);
+  if (st != FPSCAN_OK) return st;
+  const unsigned grid = walk_grid<KD, kWaves, kMap>(a);
+  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
+  return launched();
+}
+
+template <int KD>
+int join(DeltaArgs& a, hipStream_t stream) {
+  delta_join<KD><<<(unsigned)(a.heads_total * ((a.Dv + 31) / 32 * 2)), 256, 0, stream>>>(a);
   return launched();
 }
 
 template <class E, int KD, int kTerms, bool kSave>
 int walk_forward(DeltaArgs& a, hipStream_t stream) {
   delta_prep<E, KD, kTerms, out_terms<E>()><<<(unsigned)(a.heads_total * a.chunks), 256, 0, stream>>>(a);
-  const int st = launched();
+  int st = launched();
+  constexpr bool kWide = InputPlanes<E>::n < 3;
+  if (a.segs > 1) {
+    if (st == FPSCAN_OK) st = launch_forward<E, KD, kTerms, false, true, kWide ? 4 : 2, kWide ? 4 : 2>(a, stream);
+    if (st == FPSCAN_OK) st = join<KD>(a, stream);
+  }
   if (st != FPSCAN_OK) return st;
-  if constexpr (InputPlanes<E>::n == 3)
-    return launch_forward<E, KD, kTerms, kSave, 2, 2>(a, stream);
-  else
-    return walk_narrow(a) ? launch_forward<E, KD, kTerms, kSave, 2, 4>(a, stream)
-                          : launch_forward<E, KD, kTerms, kSave, 4, 4>(a, stream);
+  if constexpr (kWide)
+    if (!walk_narrow(a)) return launch_forward<E, KD, kTerms, kSave, false, 4, 4>(a, stream);
+  return launch_forward<E, KD, kTerms, kSave, false, 2, kWide ? 4 : 2>(a, stream);
 }
 
-template <class E, int KD, int kWaves, int kBring>
-int launch_backward(DeltaArgs& a, hipStream_t stream) {
-  using C = ChunkLds<E, KD, out_terms<E>(), out_terms<E>(), kWaves>;
-  const auto walk = delta_chunks_bwd<E, KD, kWaves, kBring>;
-  const int st = allow_lds(walk, C::total);
+template <class E, int KD>
+int walk_backward(DeltaArgs& a, hipStream_t stream) {
+  int st = FPSCAN_OK;
+  constexpr bool kWide = InputPlanes<E>::n < 3;
+  if (a.segs > 1) {
+    st = launch_backward<E, KD, true, kWide ? 4 : 2, kWide ? 4 : 2>(a, stream);
+    if (st == FPSCAN_OK) st = join<KD>(a, stream);
+  }
   if (st != FPSCAN_OK) return st;
-  const unsigned grid = walk_grid(a, kWaves);
-  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
-  return launched();
+  if constexpr (kWide)
+    if (!walk_narrow(a)) return launch_backward<E, KD, false, 4, 4>(a, stream);
+  return launch_backward<E, KD, false, 2, kWide ? 4 : 2>(a, stream);
 }
 
 template <class E, int KD>
 int backward(DeltaArgs& a, hipStream_t stream) {
-  int st;
-  if constexpr (InputPlanes<E>::n == 3)
-    st = launch_backward<E, KD, 2, 2>(a, stream);
-  else
-    st = walk_narrow(a) ? launch_backward<E, KD, 2, 4>(a, stream) : launch_backward<E, KD, 4, 4>(a, stream);
+  int st = walk_backward<E, KD>(a, stream);
   if (st != FPSCAN_OK) return st;
   constexpr int lds = GradLds<E, KD>::size;
   const auto kernel = a.R > 1 ? delta_grads<E, KD, true> : delta_grads<E, KD, false>;

@@ -111,6 +111,31 @@ def test_continued_state(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1300, 1, 2, 64, 40), (2, 2049, 1, 1, 128, 72)])
+def test_long_sequences_of_few_heads(shape, dtype):
+    """Long enough, and few enough heads, that segments of the sequence are walked side by side."""
+    B, L, Hk, H, Dk, Dv = shape
+    t = inputs(*shape, dtype, seed=21, decay=0.02)
+    t["log_decay"][:, 700] = -math.inf
+    leaves = {n: x.double().requires_grad_() for n, x in t.items()}
+    want, _ = rule(leaves)
+    go = torch.randn(want.shape, generator=torch.Generator().manual_seed(9), dtype=torch.float64).to(dtype)
+    grads = torch.autograd.grad(want, [leaves[n] for n in NAMES], go.double())
+    on = [x.requires_grad_() for x in gpu(t)]
+    out = fpscan_amd.gated_delta(*on)
+    check(out, want, OUT_TOL[dtype], "out")
+    for n, x, y in zip(NAMES, torch.autograd.grad(out, on, go.to(DEVICE)), grads):
+        y = torch.where(t[n] == -math.inf, 0, y) if n == "log_decay" else y
+        check(x, y, DECAY_TOL[dtype] if n == "log_decay" else GRAD_TOL[dtype], "grad_" + n)
+    s0 = torch.randn(B, H, Dk, Dv, generator=torch.Generator().manual_seed(22))
+    want, last = rule(t, s0)
+    state = s0.to(DEVICE)
+    check(fpscan_amd.gated_delta_forward(*(x.detach() for x in on), state=state), want, OUT_TOL[dtype],
+          "continued")
+    check(state, last, STATE_TOL, "state")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_parts_of_a_prompt_and_tokens_make_the_whole(dtype):
     """A prompt in two parts, then token by token, is the whole sequence at once."""
     t = inputs(2, 150, 2, 4, 64, 64, dtype, seed=5)
