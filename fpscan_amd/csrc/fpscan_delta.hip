@@ -38,7 +38,7 @@ struct DeltaArgs {
   Heads q, k, v, g, beta, go;
   char* out;          // contiguous (batch, seqlen, heads, value_dim)
   float* state;       // contiguous (batch, heads, key_dim, value_dim), or null
-  char *gb, *n, *m;   // per chunk: (G, beta), N, M
+  char *gb, *n, *m;   // per chunk: (G / ln 2 as two floats, beta), N, M
   char *s, *e;        // saved per chunk: S before it, E
   float *ss, *es;     // and their scales
   char *ds, *y;       // the same of dS' and Y
@@ -72,6 +72,12 @@ __device__ __forceinline__ float element(const Heads& x, int64_t b, int64_t t, i
     return E::widen16(static_cast<const unsigned short*>(x.p)[at]);
 }
 
+// 2^x to an ulp, and 2^(hi + lo) of a sum of two floats; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float exp2_of(float hi, float lo) {
+  return exp2_of(hi) * fmaf(lo, 0.69314718f, 1.0f);
+}
+
 // The wave's index in its workgroup, in a scalar register: what follows from it is uniform.
 __device__ __forceinline__ int wave_index() {
   return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -83,15 +89,15 @@ __device__ __forceinline__ int rows_left(int64_t L, int64_t t0) {
 
 // ------------------------------------------------------------------------------- preparation
 // One workgroup of four waves per (sequence, head, chunk). Wave w makes rows 16 w.. of K K^T and
-// Q K^T; then N = A - A beta N by blocks of 16: the inverses D of the diagonal blocks of
-// I + A beta by substitution, one wave each, and the blocks below them column by column, one wave
-// each, N_IK = D_I (A_IK - sum_{K <= J < I} (A beta)_IJ N_JK), with the fp32 matrix instruction.
+// Q K^T; the latter as its transpose, so that a lane holds a row of M's blocks and stores them as
+// frags. Then N = A - A beta N by blocks of 16: the inverses D of the diagonal blocks of I + A beta by
+// substitution, one wave each, and the blocks below them column by column, one wave each, N_IK =
+// D_I (A_IK - sum_{K <= J < I} (A beta)_IJ N_JK), with the fp32 matrix instruction.
 constexpr int kPrepStride = 68;
 
 template <class E, int KD, int kTerms, int kOut>
-__global__ __launch_bounds__(256) void delta_prep(DeltaArgs a) {
+__global__ __launch_bounds__(256, 4) void delta_prep(DeltaArgs a) {
   __shared__ __attribute__((aligned(16))) float A[kChunk][kPrepStride];
-  __shared__ __attribute__((aligned(16))) float M[kChunk][kPrepStride];
   __shared__ __attribute__((aligned(16))) float D[4][16][20];
   __shared__ __attribute__((aligned(16))) float ghi[kChunk], glo[kChunk], beta[kChunk];
   constexpr int NI = InputPlanes<E>::n;
@@ -110,7 +116,7 @@ __global__ __launch_bounds__(256) void delta_prep(DeltaArgs a) {
     g = g < kLeastLog ? kLeastLog : g;  // NaN stays
     // differences of the running sum have to keep their precision after a decay of zero, whose
     // -104 all later sums hold: summed in 64 bits, kept as two floats
-    double G = g;
+    double G = (double)g * 1.4426950408889634;  // in powers of two: each exponential is one instruction
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const double o = __shfl_up(G, d);
@@ -123,11 +129,12 @@ __global__ __launch_bounds__(256) void delta_prep(DeltaArgs a) {
     reinterpret_cast<f32x4*>(a.gb)[ch * kChunk + lane] = f32x4{hi, lo, bt, 0.0f};
   }
 
-  f32x4 kk[4] = {}, qk[4] = {};
+  f32x4 kk[4] = {}, qk[4] = {};  // kk: row i by lane group, column j by lane; qk: the other way round
   {
     const Rsrc rk = head_rsrc(a.k, b, hk, t0, rows, a.Dk, E::kSize);
     const Rsrc rq = head_rsrc(a.q, b, hk, t0, rows, a.Dk, E::kSize);
     const int kst = (int)a.k.t * E::kSize, qst = (int)a.q.t * E::kSize;
+#pragma unroll
     for (int s = 0; s < KD / 32; ++s) {
       const int d = 32 * s + 8 * lg;
       const bool in = d < a.Dk;
@@ -140,36 +147,65 @@ __global__ __launch_bounds__(256) void delta_prep(DeltaArgs a) {
           bf16x8 kb[NI];
           load8<E>(rk, in ? (16 * nt + li) * kst + d * E::kSize : kNoOffset, kb);
           kk[nt] = mma<3>(ka, kb, kk[nt]);
-          qk[nt] = mma<3>(qa, kb, qk[nt]);
+          qk[nt] = mma<3>(kb, qa, qk[nt]);
         }
     }
   }
   __syncthreads();
+  {
+    const int i0 = 16 * w + 4 * lg, i = 16 * w + li;
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(&ghi[i0]), lo = *reinterpret_cast<const f32x4*>(&glo[i0]);
 #pragma unroll
-  for (int nt = 0; nt < 4; ++nt)
-    if (nt <= (w | 1)) {  // the blocks of 32 columns that reach the diagonal, zeros above it
+    for (int nt = 0; nt < 4; ++nt) {
+      const int j = 16 * nt + li, j0 = 16 * nt + 4 * lg;
+      // the blocks of 32 columns that reach the diagonal, zeros above it
+      if (nt <= (w | 1)) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * w + 4 * lg + r, j = 16 * nt + li;
-        const float gam = j <= i ? expf((ghi[i] - ghi[j]) + (glo[i] - glo[j])) : 0.0f;
-        A[i][j] = j < i ? gam * kk[nt][r] : 0.0f;
-        M[i][j] = j <= i ? a.scale * (gam * qk[nt][r]) : 0.0f;
+        for (int r = 0; r < 4; ++r)
+          A[i0 + r][j] = j < i0 + r ? exp2_of((hi[r] - ghi[j]) + (lo[r] - glo[j])) * kk[nt][r] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          qk[nt][r] = j0 + r <= i ? a.scale * (exp2_of((ghi[i] - ghi[j0 + r]) + (glo[i] - glo[j0 + r])) * qk[nt][r])
+                                  : 0.0f;
       }
     }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s <= w / 2) {
+        bf16x8 pm[kOut];
+        split(join(qk[2 * s], qk[2 * s + 1]), pm);
+        const int at = (w < 2 ? w : 2 * w - 2 + s) * 1024 + frag_lane(li, lg);
+#pragma unroll
+        for (int p = 0; p < kOut; ++p)
+          *reinterpret_cast<bf16x8*>(a.m + (ch * kOut + p) * kTriBytes + at) = pm[p];
+      }
+  }
   __syncthreads();
 
   {  // D[w] = the inverse of I + (A beta)[w][w], lane by column
-    float x[16];
+    f32x4 x[4], bt[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bt[j] = *reinterpret_cast<const f32x4*>(&beta[16 * w + 4 * j]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = i == li ? 1.0f : 0.0f;
+      float v = i == li ? 1.0f : 0.0f, u = 0.0f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) v = fmaf(-(A[16 * w + i][16 * w + j] * beta[16 * w + j]), x[j], v);
-      x[i] = v;
+      for (int j = 0; j < (i + 3) / 4; ++j) {
+        const f32x4 m = *reinterpret_cast<const f32x4*>(&A[16 * w + i][16 * w + 4 * j]) * bt[j];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (4 * j + r < i) {
+            if (r & 1)
+              u = fmaf(-m[r], x[j][r], u);
+            else
+              v = fmaf(-m[r], x[j][r], v);
+          }
+      }
+      x[i / 4][i % 4] = v + u;
     }
     if (lg == 0)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) D[w][i][li] = x[i];
+      for (int i = 0; i < 16; ++i) D[w][i][li] = x[i / 4][i % 4];
   }
   __syncthreads();
   f32x4 n[4];
@@ -201,21 +237,16 @@ __global__ __launch_bounds__(256) void delta_prep(DeltaArgs a) {
       for (int r = 0; r < 4; ++r) A[16 * I + 4 * lg + r][16 * w + li] = n[I][r];
   __syncthreads();
 
-  // out in 16-byte pieces, a block of 16 x 32 per wave and turn
+  // N out in 16-byte pieces, a block of 16 x 32 per wave and turn
   for (int f = w; f < 6; f += 4) {
     const int mt = f < 2 ? f : 1 + f / 2, s = f < 2 ? 0 : f & 1;
     const int i = 16 * mt + li, j = 32 * s + 4 * lg, at = f * 1024 + frag_lane(li, lg);
-    bf16x8 pn[kTerms], pm[kOut];
+    bf16x8 pn[kTerms];
     split(join(*reinterpret_cast<const f32x4*>(&A[i][j]),
                *reinterpret_cast<const f32x4*>(&A[i][j + 16])), pn);
-    split(join(*reinterpret_cast<const f32x4*>(&M[i][j]),
-               *reinterpret_cast<const f32x4*>(&M[i][j + 16])), pm);
 #pragma unroll
     for (int p = 0; p < kTerms; ++p)
       *reinterpret_cast<bf16x8*>(a.n + (ch * kTerms + p) * kTriBytes + at) = pn[p];
-#pragma unroll
-    for (int p = 0; p < kOut; ++p)
-      *reinterpret_cast<bf16x8*>(a.m + (ch * kOut + p) * kTriBytes + at) = pm[p];
   }
 }
 
@@ -380,8 +411,8 @@ struct Brought {
     }
     if (w == 0) {
       const float hi = readlane(gb[0], 63), lo = readlane(gb[1], 63);
-      reinterpret_cast<float*>(lds + C::gam)[lane] = expf(gb[0]) * (1.0f + gb[1]);
-      reinterpret_cast<float*>(lds + C::end)[lane] = expf((hi - gb[0]) + (lo - gb[1]));
+      reinterpret_cast<float*>(lds + C::gam)[lane] = exp2_of(gb[0], gb[1]);
+      reinterpret_cast<float*>(lds + C::end)[lane] = exp2_of((hi - gb[0]) + (lo - gb[1]));
       reinterpret_cast<float*>(lds + C::beta)[lane] = gb[2];
     }
   }
@@ -1120,8 +1151,8 @@ __global__ __launch_bounds__(256, InputPlanes<E>::n == 1 && !kShared ? 2 : 1) vo
       row_hi[lane] = x[0];
       row_lo[lane] = x[1];
       row_beta[lane] = x[2];
-      row_gam[lane] = expf(x[0]) * (1.0f + x[1]);
-      row_end[lane] = expf((l[0] - x[0]) + (l[1] - x[1]));
+      row_gam[lane] = exp2_of(x[0], x[1]);
+      row_end[lane] = exp2_of((l[0] - x[0]) + (l[1] - x[1]));
     }
     if constexpr (kHalf) {
       auto common = [&](int which, const float* from) {
@@ -1251,7 +1282,7 @@ __global__ __launch_bounds__(256, InputPlanes<E>::n == 1 && !kShared ? 2 : 1) vo
         for (int r = 0; r < 4; ++r) {
           const int i = i0 + r;
           const float gam =
-              jj <= i ? expf((row_hi[i] - row_hi[jj]) + (row_lo[i] - row_lo[jj])) : 0.0f;
+              jj <= i ? exp2_of((row_hi[i] - row_hi[jj]) + (row_lo[i] - row_lo[jj])) : 0.0f;
           p[r] = jj <= i ? a.scale * (gam * (ou[nt][r] * fo * fe)) : 0.0f;
           f[r] = jj < i ? -(gam * (vu[nt][r] * fy * fe)) : 0.0f;
         }
@@ -1390,12 +1421,14 @@ __global__ __launch_bounds__(256) void delta_steps(DeltaArgs a) {
   if (a.slots) slot = a.slots[b];
   const bool live = slot >= 0 && slot < a.nslots;
   float* st = a.state + ((slot * a.H + h) * a.Dk + rg * NR) * a.Dv + col;
+  // (read and written once a call: nontemporal)
 
   f32x4 S[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i)
-    S[i] = live && in && rg * NR + i < a.Dk ? *reinterpret_cast<const f32x4*>(st + i * a.Dv)
-                                            : f32x4{};
+    S[i] = live && in && rg * NR + i < a.Dk
+               ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(st + i * a.Dv))
+               : f32x4{};
   for (int64_t t = 0; t < a.L; ++t) {
     const Rsrc rk = head_rsrc(a.k, b, hk, t, 1, a.Dk, E::kSize);
     const Rsrc rq = head_rsrc(a.q, b, hk, t, 1, a.Dk, E::kSize);
@@ -1456,7 +1489,8 @@ __global__ __launch_bounds__(256) void delta_steps(DeltaArgs a) {
   if (live && in)
 #pragma unroll
     for (int i = 0; i < NR; ++i)
-      if (rg * NR + i < a.Dk) *reinterpret_cast<f32x4*>(st + i * a.Dv) = S[i];
+      if (rg * NR + i < a.Dk)
+        __builtin_nontemporal_store(S[i], reinterpret_cast<f32x4*>(st + i * a.Dv));
 }
 
 // ------------------------------------------------------------------------------------ host side
