@@ -586,6 +586,209 @@ __global__ __launch_bounds__(1024) void norm_apply_bwd(NormArgs a) {
   });
 }
 
+// ------------------------------------------------------------------------------ a group at a time
+// Small sequences: one workgroup per (sequence, group), in one launch where the passes above are three
+// (forward) or four (backward). Threads own 16-byte vectors that the group's channels reach into, the
+// first and the last of a row perhaps in part. kKept vectors a thread stay in registers from the sum
+// to the output.
+struct GroupPlace {
+  int64_t at;      // byte offset of the thread's first vector
+  int64_t step;    // bytes to its next one
+  int rows, row, c, lo, hi;  // rows a turn, its first row; first channel of the vector, which of it count
+  int count;       // vectors of the thread
+  bool in;
+};
+template <class E>
+__device__ __forceinline__ GroupPlace group_place(const NormArgs& a, int64_t b, int g) {
+  constexpr int V = E::V;
+  const int c0 = g * a.width, c1 = c0 + a.width, v0 = c0 / V, vecs = (c1 + V - 1) / V - v0;
+  GroupPlace p;
+  p.rows = (int)blockDim.x / vecs;
+  p.row = (int)threadIdx.x / vecs;
+  p.c = (v0 + (int)threadIdx.x - p.row * vecs) * V;
+  p.in = p.row < p.rows;
+  p.lo = c0 > p.c ? c0 - p.c : 0;
+  p.hi = c1 < p.c + V ? c1 - p.c : V;
+  p.count = p.in && p.row < a.seqlen ? (int)((a.seqlen - p.row + p.rows - 1) / p.rows) : 0;
+  p.at = ((b * a.seqlen + p.row) * a.dim + p.c) * E::kSize;
+  p.step = (int64_t)p.rows * a.dim * E::kSize;
+  return p;
+}
+
+// The workgroup's sum of x, in every thread.
+__device__ __forceinline__ float block_sum(float x, float* lds) {
+  x = wave_sum(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+  float s = lds[0];
+  for (int i = 1; i < (int)blockDim.x / 64; ++i) s += lds[i];
+  return s;
+}
+
+// x's channels of the group to memory, the others left as they are.
+template <class E>
+__device__ __forceinline__ void store_part(char* to, const GroupPlace& p, const float (&x)[E::V]) {
+  if (p.lo == 0 && p.hi == E::V) {
+    store_vec<E>(to, x);
+  } else {
+    const u32x4 v = E::pack(x);
+#pragma unroll
+    for (int i = 0; i < E::V; ++i)
+      if (i >= p.lo && i < p.hi) {
+        if constexpr (E::kSize == 4)
+          reinterpret_cast<unsigned*>(to)[i] = v[i];
+        else
+          reinterpret_cast<unsigned short*>(to)[i] = (unsigned short)(v[i / 2] >> (16 * (i & 1)));
+      }
+  }
+}
+
+// Parameters of the vector's channels, 1 and 0 beside the group (and so for the means: nothing).
+template <int V>
+__device__ __forceinline__ void group_params(const NormArgs& a, const GroupPlace& p, float (&w)[V], float (&b)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const bool in = p.in && i >= p.lo && i < p.hi;
+    w[i] = a.weight && in ? a.weight[p.c + i] : 1.0f;
+    b[i] = a.bias && in ? a.bias[p.c + i] : 0.0f;
+  }
+}
+
+constexpr int kKept = 4;
+
+template <class E, bool kAct, bool kGate>
+__global__ __launch_bounds__(1024) void norm_groups(NormArgs a) {
+  constexpr int V = E::V;
+  __shared__ float lds[16];
+  const int64_t b = blockIdx.x / a.groups;
+  const int g = (int)(blockIdx.x - b * a.groups);
+  const GroupPlace p = group_place<E>(a, b, g);
+  u32x4 raw[kKept];
+#pragma unroll
+  for (int j = 0; j < kKept; ++j) raw[j] = j < p.count ? raw_vec(a.x + p.at + j * p.step) : u32x4{};
+  float w[V], bias[V];
+  group_params(a, p, w, bias);
+  // the means are taken from the group's first value, so that sums of values far from 0 lose nothing
+  float first[V];
+  E::unpack(raw[0], first);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i == p.lo) lds[0] = first[i];
+  }
+  __syncthreads();
+  const float base = lds[0], inv = 1.0f / ((float)a.seqlen * (float)a.width);
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kKept; ++j) {
+    float x[V];
+    E::unpack(raw[j], x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += j < p.count && i >= p.lo && i < p.hi ? x[i] - base : 0.0f;
+  }
+  const float mean = fmaf(block_sum(s, lds), inv, base);
+  s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kKept; ++j) {
+    float x[V];
+    E::unpack(raw[j], x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float d = j < p.count && i >= p.lo && i < p.hi ? x[i] - mean : 0.0f;
+      s = fmaf(d, d, s);
+    }
+  }
+  const float rstd = __builtin_amdgcn_rsqf(fmaf(block_sum(s, lds), inv, a.eps));
+  if (a.mean && threadIdx.x == 0) {
+    a.mean[blockIdx.x] = mean;
+    a.rstd[blockIdx.x] = rstd;
+  }
+#pragma unroll
+  for (int j = 0; j < kKept; ++j)
+    if (j < p.count) {
+      const int64_t at = p.at + j * p.step;
+      float x[V], z[V] = {};
+      E::unpack(raw[j], x);
+      if (kGate) load_vec<E>(a.gate + at, z);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        x[i] = activate<E, kAct, kGate>(fmaf((x[i] - mean) * rstd, w[i], bias[i]), z[i]);
+      store_part<E>(a.out + at, p, x);
+    }
+}
+
+// Backward in two passes over the group, the second one out of the caches; the parameters' sums of the
+// sequence to `channels`.
+template <class E, bool kAct, bool kGate>
+__global__ __launch_bounds__(1024) void norm_groups_bwd(NormArgs a) {
+  constexpr int V = E::V;
+  extern __shared__ float lds[];  // a row of the workgroup's vectors: dy, then dy h
+  __shared__ float sums[16];
+  const int64_t b = blockIdx.x / a.groups;
+  const int g = (int)(blockIdx.x - b * a.groups);
+  const GroupPlace p = group_place<E>(a, b, g);
+  float w[V], bias[V], gw[V] = {}, gb[V] = {};
+  group_params(a, p, w, bias);
+  const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
+  auto gradient = [&](int64_t at, float (&h)[V], float (&dy)[V], float (&z)[V]) {
+    load_vec<E>(a.x + at, h);
+    load_vec<E>(a.go + at, dy);
+    if (kGate) load_vec<E>(a.gate + at, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      h[i] = (h[i] - mean) * rstd;
+      dy[i] = slope<E, kAct, kGate>(fmaf(h[i], w[i], bias[i]), z[i], dy[i], z[i]);
+    }
+  };
+#pragma unroll 2
+  for (int j = 0; j < p.count; ++j) {
+    float h[V], dy[V], z[V] = {};
+    gradient(p.at + j * p.step, h, dy, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      gb[i] += dy[i];
+      gw[i] = fmaf(dy[i], h[i], gw[i]);
+    }
+  }
+  float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i >= p.lo && i < p.hi) {
+      m1 = fmaf(w[i], gb[i], m1);
+      m2 = fmaf(w[i], gw[i], m2);
+    }
+  const float inv = rstd / ((float)a.seqlen * (float)a.width);
+  m1 = block_sum(m1, sums) * inv;
+  m2 = block_sum(m2, sums) * inv;
+#pragma unroll 2
+  for (int j = 0; j < p.count; ++j) {
+    const int64_t at = p.at + j * p.step;
+    float h[V], dy[V], z[V] = {};
+    gradient(at, h, dy, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = fmaf(rstd * w[i], dy[i], -fmaf(h[i], m2, m1));
+    store_part<E>(a.gx + at, p, h);
+    if (kGate) store_part<E>(a.ggate + at, p, z);
+  }
+  // per channel over the workgroup's rows
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[threadIdx.x * V + i] = turn ? gw[i] : gb[i];
+    __syncthreads();
+    const int c0 = g * a.width, lead = c0 % V;
+    const int per_row = ((c0 + a.width + V - 1) / V - c0 / V) * V;
+    for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+      float s = 0.0f;
+      for (int r = 0; r < p.rows; ++r) s += lds[r * per_row + lead + c];
+      a.channels[(b * 2 + turn) * a.dim + c0 + c] = s;
+    }
+  }
+}
+
 // Sums over the rows of slabs of a (slabs, rows, cols) array: 16 columns a workgroup, 64 threads each
 // (a row's 64 bytes at a time; 64 columns by 16 threads left most CUs without work: 38 instead of 9 us
 // for 2048 rows of 2048). The first `split` columns go to `to_a`, the others to `to_b` (either may be
@@ -624,6 +827,7 @@ struct Launch {
   int threads, blocks;  // blocks: of the token kernel backward
   int turns;            // and forward
   bool tokens, aligned;
+  int group_threads;  // a group at a time: threads; 0: not
   size_t lds;
 };
 
@@ -662,6 +866,17 @@ Launch launch_of(const fpscan_norm* p) {
   l.threads = a.vecs <= 256 ? 256 : a.vecs <= 512 ? 512 : 1024;
   a.rows = l.threads / a.vecs;
   l.tokens = p->seqlen == 1;
+  // A group at a time: up to kKept vectors a thread, tensors that stay in the L2 caches (their lines
+  // are read by several groups). 2 sequences of 256 steps, 256 channels in 32 groups, fp32: 5.0 us
+  // against 14.5 of the three launches below; but at 14 vectors a thread (3 sequences of 1000 steps,
+  // 776 channels in 8 groups, fp16), on 24 of the CUs, 50 and 44 us forward and backward against 18 and
+  // 27.
+  const int64_t group_vecs = (a.width + V - 1) / V + (a.width % V != 0);
+  if (!l.tokens && group_vecs <= 1024 && a.batch * a.groups < (int64_t)1 << 31 &&
+      a.batch * a.seqlen * a.dim * size <= (int64_t)8 << 20) {
+    l.group_threads = a.seqlen * group_vecs <= 1024 ? 256 : 1024;
+    if (l.group_threads / group_vecs * kKept < a.seqlen) l.group_threads = 0;
+  }
   const int gv = a.width / V;
   l.aligned = l.tokens && a.width % V == 0 && gv <= 64 && (gv & (gv - 1)) == 0;
   a.lanes = l.aligned ? gv : power_of_two_below(l.threads / a.groups < 1 ? 1 : l.threads / a.groups);
@@ -694,10 +909,10 @@ size_t carve(char* base, Launch& l, bool backward, bool own_stats) {
   char* at = base;
   NormArgs& a = l.a;
   if (backward) {
-    const int64_t parts = l.tokens ? l.blocks : a.batch * a.chunks;
+    const int64_t parts = l.tokens ? l.blocks : l.group_threads ? 0 : a.batch * a.chunks;
     a.part = reinterpret_cast<float*>(take(at, (size_t)parts * 2 * a.dim * 4));
     if (!l.tokens) a.channels = reinterpret_cast<float*>(take(at, (size_t)a.batch * 2 * a.dim * 4));
-  } else if (!l.tokens) {
+  } else if (!l.tokens && !l.group_threads) {
     a.part = reinterpret_cast<float*>(take(at, (size_t)a.batch * a.chunks * 2 * a.groups * 4));
     if (own_stats) {
       a.mean = reinterpret_cast<float*>(take(at, (size_t)a.batch * a.groups * 4));
@@ -784,6 +999,10 @@ int fpscan_norm_fwd(const fpscan_norm* p, const void* x, const float* weight, co
     if (l.tokens)
       return l.aligned ? launch(norm_tokens<E, act.value, gated.value, true>, l, l.turns, s)
                        : launch(norm_tokens<E, act.value, gated.value, false>, l, l.turns, s);
+    if (l.group_threads) {
+      norm_groups<E, act.value, gated.value><<<(unsigned)(a.batch * a.groups), l.group_threads, 0, s>>>(a);
+      return launched();
+    }
     int st = launch(norm_stats<E>, l, a.batch * a.chunks, s);
     if (st != FPSCAN_OK) return st;
     norm_join<<<(unsigned)((a.batch * a.groups + 3) / 4), 256, 0, s>>>(a);
@@ -825,6 +1044,11 @@ int fpscan_norm_bwd(const fpscan_norm* p, const void* x, const float* weight, co
     if (l.tokens)
       return l.aligned ? launch(norm_tokens_bwd<E, act.value, gated.value, true>, l, l.blocks, s)
                        : launch(norm_tokens_bwd<E, act.value, gated.value, false>, l, l.blocks, s);
+    if (l.group_threads) {
+      norm_groups_bwd<E, act.value, gated.value>
+          <<<(unsigned)(a.batch * a.groups), l.group_threads, l.group_threads * 16 / E::kSize * 4, s>>>(a);
+      return launched();
+    }
     int st = launch(norm_sums_bwd<E, act.value, gated.value>, l, a.batch * a.chunks, s);
     if (st != FPSCAN_OK) return st;
     if ((st = columns(a.part, a.batch, a.chunks, a.dim, a.channels, nullptr, 2 * a.dim, s)) != FPSCAN_OK)

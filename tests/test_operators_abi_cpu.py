@@ -132,7 +132,7 @@ def test_norm_refuses(lib, d, change, error):
 
 def test_norm_refuses_pointers_and_short_workspaces(lib, d):
     null, align, short = (d["FPSCAN_ERR_" + n] for n in ("NULL", "ALIGN", "WORKSPACE"))
-    for p in (norm(), norm(seqlen=1)):
+    for p in (norm(seqlen=5000), norm(seqlen=1)):
         fwd = lambda x=FAKE, w=None, out=FAKE, n=BIG: lib.fpscan_norm_fwd(  # noqa: E731
             p, x, w, None, None, out, None, FAKE, n, None)
         bwd = lambda stats=FAKE, gate=None, gx=FAKE, n=BIG: lib.fpscan_norm_bwd(  # noqa: E731
@@ -141,8 +141,9 @@ def test_norm_refuses_pointers_and_short_workspaces(lib, d):
         assert bwd(gate=FAKE) == null  # no place for the gate's gradient
         assert fwd(x=FAKE + 8) == align and fwd(w=FAKE + 2) == align and bwd(gx=FAKE + 4) == align
         assert bwd(n=lib.fpscan_norm_workspace_bytes(p, 1) - 1) == short
-    assert lib.fpscan_norm_fwd(norm(), FAKE, None, None, None, FAKE, None, FAKE,
-                               lib.fpscan_norm_workspace_bytes(norm(), 0) - 1, None) == short
+    p = norm(seqlen=5000)
+    assert lib.fpscan_norm_fwd(p, FAKE, None, None, None, FAKE, None, FAKE,
+                               lib.fpscan_norm_workspace_bytes(p, 0) - 1, None) == short
     for p in (norm(batch=0), norm(seqlen=0), norm(dim=0)):
         assert lib.fpscan_norm_workspace_bytes(p, 0) == lib.fpscan_norm_workspace_bytes(p, 1) == 0
         assert lib.fpscan_norm_fwd(p, None, None, None, None, None, None, None, 0, None) == 0
