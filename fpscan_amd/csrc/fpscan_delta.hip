@@ -258,10 +258,13 @@ __global__ __launch_bounds__(256, 4) void delta_prep(DeltaArgs a) {
 template <class E>
 constexpr int kept_size() { return InputPlanes<E>::n == 1 ? 2 : 4; }
 
-__device__ __forceinline__ float block_scale(float most) {
+struct BlockScale {
+  float up, down;  // 2^e and 2^-e
+};
+__device__ __forceinline__ BlockScale block_scale(float most) {
   const int e = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^e
-  const int up = 15 - e > 126 ? 126 : 15 - e;
-  return __uint_as_float((unsigned)(up + 127) << 23);
+  const int up = 15 - e > 126 ? 126 : 15 - e;              // >= -114
+  return {__uint_as_float((unsigned)(127 + up) << 23), __uint_as_float((unsigned)(127 - up) << 23)};
 }
 
 // `live`: whether the block exists (its stores are dropped otherwise, without a branch).
@@ -276,12 +279,12 @@ __device__ __forceinline__ void keep(char* base, float* scales, int64_t block, b
     for (int i = 0; i < 2 * kPairs; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[i][j]));
-    const float up = block_scale(wave_max(most));
+    const BlockScale scale = block_scale(wave_max(most));
 #pragma unroll
     for (int i = 0; i < kPairs; ++i)
       bst16<0>(r, (i * 64 + lane) * 16,
-               __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * i], x[2 * i + 1]) * up, f16x8)));
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(1.0f / up),
+               __builtin_bit_cast(u32x4, __builtin_convertvector(join(x[2 * i], x[2 * i + 1]) * scale.up, f16x8)));
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(scale.down),
                                           row_rsrc(scales, block, 4, live ? 4 : 0), lane * 4, 0, 0);
   } else {
 #pragma unroll
@@ -627,40 +630,56 @@ __device__ __forceinline__ void write_map(const DeltaArgs& a, const Place& p, in
   }
 }
 
-// States from segment to segment, 16 value columns a workgroup: ts of each, from `state` or zero.
+// States from segment to segment, 16 value columns a workgroup: ts of each, from `state` or zero. A step
+// is a product by the segment's KD x KD map in fp32, its rows and quarters of its columns spread over
+// the threads so that a thread's loads are all out at once (one thread a row, 128 loads in turn: 6.5 us a
+// step against 4).
+constexpr int kJoinThreads = 1024;
 template <int KD>
-__global__ __launch_bounds__(256) void delta_join(DeltaArgs a) {
-  __shared__ __attribute__((aligned(16))) float S[2][KD][16];
-  constexpr int kParts = 256 / KD, kCols = 16 / kParts;  // threads and columns a row
+__global__ __launch_bounds__(kJoinThreads) void delta_join(DeltaArgs a) {
+  constexpr int kQuarters = 4, kCols = 16 * KD * kQuarters / kJoinThreads, kEach = 16 * KD / kJoinThreads;
+  __shared__ __attribute__((aligned(16))) float S[KD][16];
+  __shared__ __attribute__((aligned(16))) float part[kQuarters][KD][17];
   const int stride = (a.Dv + 31) / 32 * 32, blocks = stride / 16;
   const int64_t bh = blockIdx.x / blocks;
-  const int col0 = (int)(blockIdx.x - bh * blocks) * 16, row = threadIdx.x % KD,
-            c0 = threadIdx.x / KD * kCols;
-  float x[kCols];
+  const int col0 = (int)(blockIdx.x - bh * blocks) * 16;
+  const int row = threadIdx.x % KD, rest = threadIdx.x / KD, quarter = rest % kQuarters,
+            c0 = rest / kQuarters * kCols;
+  // the elements that this thread joins: kEach of row er from column ec
+  const int er = threadIdx.x * kEach / 16, ec = threadIdx.x * kEach % 16;
+  float x[kEach];
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    const int col = col0 + c0 + i;
-    x[i] = a.state && row < a.Dk && col < a.Dv ? a.state[(bh * a.Dk + row) * a.Dv + col] : 0.0f;
+  for (int i = 0; i < kEach; ++i) {
+    const int col = col0 + ec + i;
+    x[i] = a.state && er < a.Dk && col < a.Dv ? a.state[(bh * a.Dk + er) * a.Dv + col] : 0.0f;
   }
   for (int p = 0;; ++p) {
     const int64_t at = bh * a.segs + p;
-    float* const to = a.ts + (at * KD + row) * stride + col0 + c0;
+    const int64_t here = (at * KD + er) * stride + col0 + ec;
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) {
-      to[i] = x[i];
-      S[p & 1][row][c0 + i] = x[i];
+    for (int i = 0; i < kEach; ++i) {
+      a.ts[here + i] = x[i];
+      S[er][ec + i] = x[i];
     }
     if (p + 1 == a.segs) break;
+    const float* const m = a.tm + (at * KD + quarter * (KD / kQuarters)) * KD + row;
+    float f[KD / kQuarters], y[kCols] = {};
+#pragma unroll
+    for (int k = 0; k < KD / kQuarters; ++k) f[k] = m[k * KD];
     __syncthreads();
-    const float* const n = a.tn + (at * KD + row) * stride + col0 + c0;
-    const float* const m = a.tm + at * KD * KD + row;
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) x[i] = n[i];
-#pragma unroll 16
-    for (int k = 0; k < KD; ++k) {
-      const float f = m[k * KD];
+    for (int k = 0; k < KD / kQuarters; ++k)
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) x[i] = fmaf(f, S[p & 1][k][c0 + i], x[i]);
+      for (int i = 0; i < kCols; ++i)
+        y[i] = fmaf(f[k], S[quarter * (KD / kQuarters) + k][c0 + i], y[i]);
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) part[quarter][row][c0 + i] = y[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      x[i] = a.tn[here + i];
+#pragma unroll
+      for (int q = 0; q < kQuarters; ++q) x[i] += part[q][er][ec + i];
     }
   }
 }
@@ -926,7 +945,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
 #pragma unroll
         for (int r = 0; r < 8; ++r) most = fmaxf(most, fabsf(v[r]));
       }
-      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(1.0f / block_scale(wave_max(most))),
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(block_scale(wave_max(most)).down),
                                             row_rsrc(a.gs, ch * tiles + tile, 4, tile < tiles ? 4 : 0),
                                             lane * 4, 0, 0);
     }
@@ -1177,7 +1196,7 @@ __global__ __launch_bounds__(256, InputPlanes<E>::n == 1 && !kShared ? 2 : 1) vo
     if constexpr (kHalf) {
       // |beta| up to a power of two: U and dV keep to fp16's range
       const float most = wave_max(fabsf(row_beta[lane]));
-      if (most > 1.0f) beta_scale = 0x1p-15f * block_scale(most);
+      if (most > 1.0f) beta_scale = 0x1p-15f * block_scale(most).up;
     }
     for (int vb = 0; vb < vblocks; ++vb) {
       if (vb > 0) lds_barrier();  // the block before is read
@@ -1723,7 +1742,7 @@ int launch_backward(DeltaArgs& a, hipStream_t stream) {
 
 template <int KD>
 int join(DeltaArgs& a, hipStream_t stream) {
-  delta_join<KD><<<(unsigned)(a.heads_total * ((a.Dv + 31) / 32 * 2)), 256, 0, stream>>>(a);
+  delta_join<KD><<<(unsigned)(a.heads_total * ((a.Dv + 31) / 32 * 2)), kJoinThreads, 0, stream>>>(a);
   return launched();
 }
 
