@@ -300,7 +300,9 @@ __device__ __forceinline__ void keep(char* base, float* scales, int64_t block, b
 // left operands are shared in LDS. Of a pair of waves, columns interleave as key_col says.
 //
 // In LDS, of a chunk: K, Q and V (dO) as frags, N and M, and per step exp(G), exp(G_end - G), beta.
-template <class E, int KD, int kTerms, int kOut, int kWaves>
+// `kTile`: bytes of each computing wave beside, at `own`: to turn columns of results into rows (half
+// types), or what a pair of waves exchanges.
+template <class E, int KD, int kTerms, int kOut, int kWaves, int kTile>
 struct ChunkLds {
   static constexpr int NI = InputPlanes<E>::n;
   static constexpr int kBlocks = KD / 32, kCols = 16 * kWaves, kColBlocks = kCols / 32;
@@ -308,13 +310,39 @@ struct ChunkLds {
   static constexpr int k = 0, q = k + NI * kPlane, v = q + NI * kPlane, n = v + NI * kColPlane,
                        m = n + kTerms * kTriBytes, gam = m + kOut * kTriBytes, end = gam + 4 * kChunk,
                        beta = end + 4 * kChunk, size = beta + 4 * kChunk;
-  // per wave, to turn 16 columns of results into rows (half types)
-  static constexpr int kTurn = E::kSize == 2 ? 2048 : 0;
   // two buffers where they fit: a chunk is then stored while the one before is still read
-  static constexpr int kBuffers = 2 * size + kWaves * kTurn <= 160 * 1024 ? 2 : 1;
-  static constexpr int turn = kBuffers * size, total = turn + kWaves * kTurn;
+  static constexpr int kBuffers = 2 * size + kWaves * kTile <= 160 * 1024 ? 2 : 1;
+  static constexpr int own = kBuffers * size, total = own + kWaves * kTile;
   static_assert(total <= 160 * 1024, "a chunk fits LDS");
 };
+
+template <class E>
+constexpr int turn_bytes() { return E::kSize == 2 ? 2048 : 0; }
+
+// Backward, half types, two computing waves: each has a second one on another SIMD (which would else
+// idle) that makes what does not hang on dS', M^T dO and the planes of scale exp(G) dO, and keeps dS'
+// from the planes that the first has made of it: 908 -> 775 us for 16384 steps of 8 heads of 8
+// sequences (width 128, bf16), 114 -> 102 us for 2048. (The same split forward, with the output as the
+// second wave's, gives 815 -> 797 us and 98 -> 93 us, but costs 423 -> 436 us where no states are kept.)
+// What one of a pair writes the other waits for at a flag, not at a barrier, which would hold up the
+// waves that bring (a tenth slower): the chunk that it holds for, counted from one. Within a chunk each
+// flag is raised once, and the barrier between chunks is passed by both, so the wait is for that value.
+__device__ __forceinline__ void raise(char* flag, int64_t chunk) {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __hip_atomic_store(reinterpret_cast<uint32_t*>(flag), (uint32_t)(chunk + 1), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ void await(char* flag, int64_t chunk) {
+  while (__hip_atomic_load(reinterpret_cast<uint32_t*>(flag), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_WORKGROUP) != (uint32_t)(chunk + 1))
+    __builtin_amdgcn_s_sleep(1);
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+constexpr int kFlags = 16;  // bytes of a pair's flags, at the end of its tile
+template <class E, int KD, bool kPair>
+constexpr int backward_tile() {
+  return kPair ? 4096 + out_terms<E>() * (KD / 32 + 2) * 1024 + kFlags : turn_bytes<E>();
+}
 
 // kCols columns of a chunk's 64 rows, in blocks of 16 x 32 shared among kWaves waves: on the way from
 // memory, and in LDS as planes.
@@ -381,9 +409,8 @@ struct Copies {
 
 // A chunk on its way from memory to LDS, in the registers of kBring waves. `value` is V or dO.
 // kReads: also Q and M, which a walk that only hands a state on does not read.
-template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring, bool kReads>
+template <class E, int KD, class C, int kTerms, int kOut, int kBring, bool kReads>
 struct Brought {
-  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
   RowBlocks<E, KD, kBring> k, q;
   RowBlocks<E, C::kCols, kBring> v;
   Copies<6 * kTerms, kBring> n;
@@ -424,12 +451,11 @@ struct Brought {
 // The waves that bring chunks first, first + step .. (`count` of them) to LDS: a chunk's loads are under
 // way while the one before is waited for and stored (past the last, it is loaded again and dropped).
 // Of `value` the columns col0 .. below `dim`, zeros beyond.
-template <class E, int KD, int kTerms, int kOut, int kWaves, int kBring, bool kReads>
+template <class E, int KD, class C, int kTerms, int kOut, int kBring, bool kReads>
 __device__ __forceinline__ void bring(char* buffers, const DeltaArgs& a, const Heads& value, int64_t bh,
                                       int64_t b, int64_t h, int64_t hk, int col0, int dim, int w,
                                       int64_t first, int64_t step, int64_t count) {
-  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
-  Brought<E, KD, kTerms, kOut, kWaves, kBring, kReads> even, odd;
+  Brought<E, KD, C, kTerms, kOut, kBring, kReads> even, odd;
   auto chunk = [&](int64_t i) { return first + step * (i < count ? i : count - 1); };
   auto pass = [&](const auto& x, int64_t i) {
     if (C::kBuffers == 1 && i > 0) lds_barrier();  // the chunk before is read
@@ -687,14 +713,14 @@ __global__ __launch_bounds__(kJoinThreads) void delta_join(DeltaArgs a) {
 template <class E, int KD, int kTerms, bool kSave, bool kMap, int kWaves, int kBring>
 __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs a) {
   constexpr int kOut = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
-  using C = ChunkLds<E, KD, kTerms, kOut, kWaves>;
+  using C = ChunkLds<E, KD, kTerms, kOut, kWaves, turn_bytes<E>()>;
   extern __shared__ __attribute__((aligned(16))) char buffers[];
   const Place p = place_of<kWaves, kMap>(a, KD);
   if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), li = lane & 15, lg = lane >> 4;
   if (w >= kWaves) {
-    bring<E, KD, kTerms, kOut, kWaves, kBring, !kMap>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, p.dim,
-                                                      w - kWaves, p.first, 1, p.count);
+    bring<E, KD, C, kTerms, kOut, kBring, !kMap>(buffers, a, a.v, p.bh, p.b, p.h, p.hk, p.col0, p.dim,
+                                                 w - kWaves, p.first, 1, p.count);
     return;
   }
   const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2, col = p.col0 + key_col(w, li);
@@ -743,7 +769,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
     constexpr bool kRoom = NI == 1 && kTerms == 2;
     f32x4 ks[4] = {}, o[4] = {}, x[4], u[4], y[4] = {};
     bf16x8 ring[2][4][NI], sp[C::kBlocks][kTerms];
-    char* const turn = buffers + C::turn + w * C::kTurn;
+    char* const turn = buffers + C::own + w * turn_bytes<E>();
     // K S, with the planes of the state a step ahead
     keys_at(0, ring[0]);
     split(join(S[0], S[1]), sp[0]);
@@ -869,21 +895,100 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs
       }
 }
 
+// The scale at which dO's 16 columns are fp16, as keep's.
+template <class E, int NI>
+__device__ __forceinline__ void keep_scale(const DeltaArgs& a, int64_t block, bool live,
+                                           const bf16x8 (&vp)[2][NI], int lane) {
+  if constexpr (kept_size<E>() == 2) {
+    float most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const f32x8 v = whole(vp[s]);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) most = fmaxf(most, fabsf(v[r]));
+    }
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(block_scale(wave_max(most)).down),
+                                          row_rsrc(a.gs, block, 4, live ? 4 : 0), lane * 4, 0, 0);
+  }
+}
+
+// The second wave of a backward pair, for tile w: M^T dO and the planes of scale exp(G) dO for the
+// first, dS' and dO's scale for the gradients of q and k.
+template <class E, int KD, class C>
+__device__ __forceinline__ void first_terms_of(const char* buffers, char* own, const DeltaArgs& a,
+                                               const Place& p, int w) {
+  constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n;
+  const int lane = threadIdx.x & 63, lg = lane >> 4;
+  const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2;
+  char* const flags = own + backward_tile<E, KD, true>() - kFlags;
+  lds_barrier();
+  for (int64_t i = 0; i < p.count; ++i) {
+    const int64_t c = a.chunks - 1 - p.first - i, ch = p.bh * a.chunks + c;
+    const char* const lds = buffers + (C::kBuffers == 2 && (i & 1) ? C::size : 0);
+    bf16x8 vp[2][NI], mf[6][kT], xp[2][kT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
+      cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+    }
+    triangle_t(lds + C::m, lane, mf);
+    f32x4 y[4] = {};
+    mma_triangle_t<kT>(mf, vp, y);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const f32x8 gam = join(*reinterpret_cast<const f32x4*>(lds + C::gam + (32 * s + 4 * lg) * 4),
+                             *reinterpret_cast<const f32x4*>(lds + C::gam + (32 * s + 16 + 4 * lg) * 4));
+      split(whole(vp[s]) * (gam * a.scale), xp[s]);
+#pragma unroll
+      for (int j = 0; j < kT; ++j)
+        reinterpret_cast<bf16x8*>(own + 4096 + (j * 2 + s) * 1024)[lane] = xp[s][j];
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) reinterpret_cast<f32x4*>(own + mt * 1024)[lane] = y[mt];
+    raise(flags, i);
+    await(flags + 4, i);  // the planes of dS' are there
+    f32x4 dS[KD / 16];
+#pragma unroll
+    for (int s = 0; s < C::kBlocks; ++s) {
+      bf16x8 sp[kT];
+#pragma unroll
+      for (int j = 0; j < kT; ++j)
+        sp[j] = reinterpret_cast<const bf16x8*>(own + 4096 + kT * 2048 + (j * C::kBlocks + s) * 1024)[lane];
+      const f32x8 x = whole(sp);
+      dS[2 * s] = __builtin_shufflevector(x, x, 0, 1, 2, 3);
+      dS[2 * s + 1] = __builtin_shufflevector(x, x, 4, 5, 6, 7);
+    }
+    keep<E, KD / 32>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
+    keep_scale<E>(a, ch * tiles + tile, tile < tiles, vp, lane);
+    if (i + 1 < p.count) {
+      if (C::kBuffers == 1) lds_barrier();
+      lds_barrier();
+    }
+  }
+}
+
 // Backward walk, the same way: a wave owns 16 columns of dS' and gives dV, and for the gradients of q
 // and k the dS' and Y of every chunk.
-template <class E, int KD, bool kMap, int kWaves, int kBring>
-__global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(DeltaArgs a) {
+template <class E, int KD, bool kMap, bool kPair, int kWaves, int kBring>
+__global__ __launch_bounds__(64 * (kWaves * (kPair ? 2 : 1) + kBring)) void delta_chunks_bwd(DeltaArgs a) {
   constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
-  using C = ChunkLds<E, KD, kT, kT, kWaves>;
+  using C = ChunkLds<E, KD, kT, kT, kWaves, backward_tile<E, KD, kPair>()>;
   extern __shared__ __attribute__((aligned(16))) char buffers[];
   const Place p = place_of<kWaves, kMap>(a, KD);
   if (p.bh >= a.heads_total) return;
   const int lane = threadIdx.x & 63, w = wave_index(), lg = lane >> 4;
-  if (w >= kWaves) {
-    bring<E, KD, kT, kT, kWaves, kBring, true>(buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, p.dim,
-                                               w - kWaves, a.chunks - 1 - p.first, -1, p.count);
+  if (w >= kWaves * (kPair ? 2 : 1)) {
+    bring<E, KD, C, kT, kT, kBring, true>(
+        buffers, a, a.go, p.bh, p.b, p.h, p.hk, p.col0, p.dim, w - kWaves * (kPair ? 2 : 1),
+        a.chunks - 1 - p.first, -1, p.count);
     return;
   }
+  if constexpr (kPair)
+    if (w >= kWaves) {
+      char* const own = buffers + C::own + (w - kWaves) * backward_tile<E, KD, true>();
+      first_terms_of<E, KD, C>(buffers, own, a, p, w - kWaves);
+      return;
+    }
   const int tile = p.col0 / 16 + w, tiles = (a.Dv + 31) / 32 * 2, col = p.col0 + key_col(w, lane & 15);
 
   f32x4 dS[KT] = {};
@@ -898,6 +1003,10 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
         else
           dS[t][r] = col < tiles * 16 ? segment_state<KD>(a.ts, a, p)[row * (tiles * 16) + col] : 0.0f;
       }
+  // of a pair: M^T dO, the planes of scale exp(G) dO, those of dS'; then the place to turn dV's columns
+  char* const own = buffers + C::own + w * backward_tile<E, KD, kPair>();
+  char* const flags = own + backward_tile<E, KD, kPair>() - kFlags;
+  if (kPair && lane < 2) reinterpret_cast<uint32_t*>(flags)[lane] = 0;
   lds_barrier();
   for (int64_t i = 0; i < p.count; ++i) {
     const int64_t c = a.chunks - 1 - p.first - i, ch = p.bh * a.chunks + c, t0 = c * kChunk;
@@ -921,13 +1030,14 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
     constexpr int kS = 4 * products(NI, kT, kT);
     f32x4 u[4] = {}, y[4] = {};
     bf16x8 ring[2][4][NI], mf[6][kT], nf[6][kT], vp[2][NI], sp[2][kT];
+    if (!kPair) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
-      cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+      for (int s = 0; s < 2; ++s) {
+        const char* at = lds + C::v + (2 * s * C::kColBlocks + w / 2) * 1024;
+        cols_of(at, at + C::kColBlocks * 1024, C::kColPlane, w, lane, vp[s]);
+      }
+      triangle_t(lds + C::m, lane, mf);
     }
-    triangle_t(lds + C::m, lane, mf);
-    char* const turn = buffers + C::turn + w * C::kTurn;
     f32x4 gam[4], beta[4], end[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -936,25 +1046,21 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
     }
     in_order();
     // M^T dO, meanwhile dS' is kept
-    if constexpr (kept_size<E>() == 2 && !kMap) {
-      // the scale at which dO's 16 columns are fp16, as keep's
-      float most = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const f32x8 v = whole(vp[s]);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) most = fmaxf(most, fabsf(v[r]));
-      }
-      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(block_scale(wave_max(most)).down),
-                                            row_rsrc(a.gs, ch * tiles + tile, 4, tile < tiles ? 4 : 0),
-                                            lane * 4, 0, 0);
-    }
+    if (!kMap && !kPair) keep_scale<E>(a, ch * tiles + tile, tile < tiles, vp, lane);
     keys_at(0, ring[0]);
     split(join(dS[0], dS[1]), sp[0]);
     settle(sp[0]);
-    if (!kMap) keep<E, KT / 2>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
-    mma_triangle_t<kT>(mf, vp, y);
-    interleave<6 * products(kT, NI, kT), 5>();
+    if (!kMap && !kPair) keep<E, KT / 2>(a.ds, a.dss, ch * tiles + tile, tile < tiles, dS, lane);
+    if (!kPair) {
+      mma_triangle_t<kT>(mf, vp, y);
+      interleave<6 * products(kT, NI, kT), 5>();
+    }
+    auto hand = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+        reinterpret_cast<bf16x8*>(own + 4096 + kT * 2048 + (i * C::kBlocks + j) * 1024)[lane] = sp[j & 1][i];
+    };
+    if (kPair) hand(0);
     // K dS', meanwhile the planes of scale exp(G) dO
     bf16x8 up[2][kT], xp[2][kT];
 #pragma unroll
@@ -963,10 +1069,11 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
         keys_at(j + 1, ring[(j + 1) & 1]);
         split(join(dS[2 * j + 2], dS[2 * j + 3]), sp[(j + 1) & 1]);
         settle(sp[(j + 1) & 1]);
+        if (kPair) hand(j + 1);
       } else {
         steps_at(0, ring[(j + 1) & 1]);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < (kPair ? 0 : 2); ++s) {
           split(whole(vp[s]) * (join(gam[2 * s], gam[2 * s + 1]) * a.scale), xp[s]);
           settle(xp[s]);
         }
@@ -980,6 +1087,16 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
 #pragma unroll
     for (int t = 0; t < KT; ++t) dS[t] *= last;
     in_order();
+    if (kPair) {
+      raise(flags + 4, i);
+      await(flags, i);  // the second wave's are there
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < kT; ++i) xp[s][i] = reinterpret_cast<const bf16x8*>(own + 4096 + (i * 2 + s) * 1024)[lane];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) y[mt] = reinterpret_cast<const f32x4*>(own + mt * 1024)[lane];
+    }
     // Q^T (scale exp(G) dO), meanwhile dU (u) and the planes of beta dU
 #pragma unroll
     for (int j = 0; j < KT / 2; ++j) {
@@ -1022,7 +1139,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
         f32x4 v[4];
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
-        turn_in<E>(turn, v, lane);
+        turn_in<E>(own, v, lane);
       }
       if (!kMap && j + 1 == KT / 4 * 3) keep<E, 2>(a.y, a.ys, ch * tiles + tile, tile < tiles, u, lane);
       if (!kMap && j + 1 == KT) {
@@ -1030,7 +1147,7 @@ __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks_bwd(Delta
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) v[mt] = u[mt] * beta[mt];
         turn_out<E>(rows_rsrc<E>(a.out, p.b, a.L, t0, a.H, p.h, a.Dv), a.H * a.Dv * E::kSize, a.Dv, p.col0, w,
-                    turn, v, lane);
+                    own, v, lane);
       }
       mma_tiles<kT>(ring[(C::kBlocks + j) & 1], up[j & 1], &dS[4 * (j / 2 % (KT / 4))]);
       interleave<kS, 4>();
@@ -1704,11 +1821,11 @@ int allow_lds(K kernel, int bytes) {
              ? FPSCAN_OK : FPSCAN_ERR_LAUNCH;
 }
 
-// Waves of a walk's workgroup: two that compute and four that bring while that fills no more than the
-// CUs, four and four beyond (8 heads of 8 sequences, width 128, bf16: 117 us for 2048 steps against
-// 122; 80 heads, fp16, 777 steps: 88 us against 139). fp32 has LDS for two and registers for two more.
+// Waves of a walk's workgroup: two columns' tiles and four waves that bring while that fills no more than
+// the CUs, four and four beyond (8 heads of 8 sequences, width 128, bf16, 2048 steps: forward 98 us
+// against 111, backward 101 against 131; 80 heads, fp16, 777 steps: 136 against 79). fp32 has LDS for two
+// and registers for two more.
 bool walk_narrow(const DeltaArgs& a) { return a.heads_total * a.segs * ((a.Dv + 63) / 64) <= 128; }
-
 
 // A walk's grid: segments (all but the last for a map) of groups of eight heads.
 template <int KD, int kWaves, bool kMap>
@@ -1720,7 +1837,7 @@ unsigned walk_grid(DeltaArgs& a) {
 
 template <class E, int KD, int kTerms, bool kSave, bool kMap, int kWaves, int kBring>
 int launch_forward(DeltaArgs& a, hipStream_t stream) {
-  using C = ChunkLds<E, KD, kTerms, out_terms<E>(), kWaves>;
+  using C = ChunkLds<E, KD, kTerms, out_terms<E>(), kWaves, turn_bytes<E>()>;
   const auto walk = delta_chunks<E, KD, kTerms, kSave, kMap, kWaves, kBring>;
   const int st = allow_lds(walk, C::total);
   if (st != FPSCAN_OK) return st;
@@ -1729,14 +1846,14 @@ int launch_forward(DeltaArgs& a, hipStream_t stream) {
   return launched();
 }
 
-template <class E, int KD, bool kMap, int kWaves, int kBring>
+template <class E, int KD, bool kMap, bool kPair, int kWaves, int kBring>
 int launch_backward(DeltaArgs& a, hipStream_t stream) {
-  using C = ChunkLds<E, KD, out_terms<E>(), out_terms<E>(), kWaves>;
-  const auto walk = delta_chunks_bwd<E, KD, kMap, kWaves, kBring>;
+  using C = ChunkLds<E, KD, out_terms<E>(), out_terms<E>(), kWaves, backward_tile<E, KD, kPair>()>;
+  const auto walk = delta_chunks_bwd<E, KD, kMap, kPair, kWaves, kBring>;
   const int st = allow_lds(walk, C::total);
   if (st != FPSCAN_OK) return st;
   const unsigned grid = walk_grid<KD, kWaves, kMap>(a);
-  walk<<<grid, 64 * (kWaves + kBring), C::total, stream>>>(a);
+  walk<<<grid, 64 * (kWaves * (kPair ? 2 : 1) + kBring), C::total, stream>>>(a);
   return launched();
 }
 
@@ -1766,13 +1883,13 @@ int walk_backward(DeltaArgs& a, hipStream_t stream) {
   int st = FPSCAN_OK;
   constexpr bool kWide = InputPlanes<E>::n < 3;
   if (a.segs > 1) {
-    st = launch_backward<E, KD, true, kWide ? 4 : 2, kWide ? 4 : 2>(a, stream);
+    st = launch_backward<E, KD, true, false, kWide ? 4 : 2, kWide ? 4 : 2>(a, stream);
     if (st == FPSCAN_OK) st = join<KD>(a, stream);
   }
   if (st != FPSCAN_OK) return st;
   if constexpr (kWide)
-    if (!walk_narrow(a)) return launch_backward<E, KD, false, 4, 4>(a, stream);
-  return launch_backward<E, KD, false, 2, kWide ? 4 : 2>(a, stream);
+    if (!walk_narrow(a)) return launch_backward<E, KD, false, false, 4, 4>(a, stream);
+  return launch_backward<E, KD, false, kWide, 2, kWide ? 4 : 2>(a, stream);
 }
 
 template <class E, int KD>
