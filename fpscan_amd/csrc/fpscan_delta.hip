@@ -92,7 +92,9 @@ __device__ __forceinline__ int rows_left(int64_t L, int64_t t0) {
 // Q K^T; the latter as its transpose, so that a lane holds a row of M's blocks and stores them as
 // frags. Then N = A - A beta N by blocks of 16: the inverses D of the diagonal blocks of I + A beta by
 // substitution, one wave each, and the blocks below them column by column, one wave each, N_IK =
-// D_I (A_IK - sum_{K <= J < I} (A beta)_IJ N_JK), with the fp32 matrix instruction.
+// D_I (A_IK - sum_{K <= J < I} (A beta)_IJ N_JK), with the fp32 matrix instruction. 16384 steps of 8
+// heads of 8 sequences, width 128, bf16: 292 us, of which reading k and q and writing N and M would take
+// 153 at 6 TB/s; the rest is the solve, dependent steps that four workgroups a CU take at once.
 constexpr int kPrepStride = 68;
 
 template <class E, int KD, int kTerms, int kOut>
@@ -710,6 +712,12 @@ __global__ __launch_bounds__(kJoinThreads) void delta_join(DeltaArgs a) {
   }
 }
 
+// The walk: a wave owns 16 value columns of a state, in registers for the whole walk, and every product of
+// a chunk is made of them or of what its wave made, so that computing waves wait for nothing but the
+// chunk, which other waves bring to LDS. Bound by the chain from state to state (five products and the
+// planes between them, about 6300 clocks of a wave a chunk) and by what a chunk's 61 KB take on their way
+// through LDS: 16384 steps of 8 heads of 8 sequences, width 128, bf16, states kept: 790 us, 2.8 TB/s (no
+// bringing in a copy of the kernel: a fifth less; half of the matrix instructions: 3 %).
 template <class E, int KD, int kTerms, bool kSave, bool kMap, int kWaves, int kBring>
 __global__ __launch_bounds__(64 * (kWaves + kBring)) void delta_chunks(DeltaArgs a) {
   constexpr int kOut = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
@@ -968,7 +976,8 @@ __device__ __forceinline__ void first_terms_of(const char* buffers, char* own, c
 }
 
 // Backward walk, the same way: a wave owns 16 columns of dS' and gives dV, and for the gradients of q
-// and k the dS' and Y of every chunk.
+// and k the dS' and Y of every chunk. Bound as the forward: 16384 steps of 8 heads of 8 sequences, width
+// 128, bf16: 760 us, 2.9 TB/s.
 template <class E, int KD, bool kMap, bool kPair, int kWaves, int kBring>
 __global__ __launch_bounds__(64 * (kWaves * (kPair ? 2 : 1) + kBring)) void delta_chunks_bwd(DeltaArgs a) {
   constexpr int kT = out_terms<E>(), NI = InputPlanes<E>::n, KT = KD / 16;
@@ -1231,6 +1240,10 @@ __device__ __forceinline__ f32x4 mma_first(const bf16x8 (&a)[NA], const bf16x8 (
     return mma<kTerms>(a, b, c);
 }
 
+// A workgroup a chunk and key head, its value heads in turn (kShared), 16 rows of the gradients a wave;
+// value columns in blocks, so that a state's LDS is a block's. Bound by memory, with what two workgroups a
+// CU hide of it: 16384 steps of 8 heads of 8 sequences, width 128, bf16: 829 us, 480 of them what its 2.9
+// GB (the kept states mostly) take at 6 TB/s.
 template <class E, int KD, bool kShared>
 __global__ __launch_bounds__(256, InputPlanes<E>::n == 1 && !kShared ? 2 : 1) void delta_grads(DeltaArgs a) {
   using C = GradLds<E, KD>;
@@ -1543,7 +1556,8 @@ __global__ __launch_bounds__(256, InputPlanes<E>::n == 1 && !kShared ? 2 : 1) vo
 // ------------------------------------------------------------------------------ token by token
 // The recurrence itself in fp32, for one to a few tokens: a wave holds 32 columns of a state (lane:
 // four columns, KD / 8 consecutive rows), and one reduction over the eight row groups gives k^T S',
-// q^T S' and q.k; then out = scale (q^T S' + (q.k) u). Bound by reading and writing the state.
+// q^T S' and q.k; then out = scale (q^T S' + (q.k) u). Bound by reading and writing the state: one token
+// of 32 heads of 256 sequences, width 128: 182 us, 5.9 TB/s; of 8 heads of one: the launch (7 us).
 template <class E, int KD>
 __global__ __launch_bounds__(256) void delta_steps(DeltaArgs a) {
   constexpr int NR = KD / 8, NI = InputPlanes<E>::n;

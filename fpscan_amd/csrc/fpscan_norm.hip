@@ -225,6 +225,8 @@ struct TokenRows {
   }
 };
 
+// Token by token. Bound by memory: 16384 rows of 1024, 8 groups, gated, bf16: 20 us forward (5.0 TB/s of
+// each tensor once), 31 backward (5.4).
 template <class E, bool kAct, bool kGate, bool kAligned>
 __global__ __launch_bounds__(1024) void norm_tokens(NormArgs a) {
   constexpr int V = E::V;
@@ -377,6 +379,9 @@ __device__ __forceinline__ void by_two(const NormArgs& a, const Place& p, const 
   }
 }
 
+// Whole sequences, each tensor read twice, as a sequence's statistics come first: 16384 steps of 8
+// sequences, 1024 channels in 32 groups, bf16: norm_stats 60 us (4.5 TB/s), norm_join 6, norm_apply 85
+// (6.3); backward norm_sums_bwd 123 (4.4), norm_apply_bwd 154 (5.2), norm_columns 14.
 template <class E>
 __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
   constexpr int V = E::V;
@@ -790,8 +795,8 @@ __global__ __launch_bounds__(1024) void norm_groups_bwd(NormArgs a) {
 }
 
 // Sums over the rows of slabs of a (slabs, rows, cols) array: 16 columns a workgroup, 64 threads each
-// (a row's 64 bytes at a time; 64 columns by 16 threads left most CUs without work: 38 instead of 9 us
-// for 2048 rows of 2048). The first `split` columns go to `to_a`, the others to `to_b` (either may be
+// (a row's 64 bytes at a time; 64 columns by 16 threads left most CUs without work: 38 us against 9, now
+// 4.9, for 2048 rows of 2048). The first `split` columns go to `to_a`, the others to `to_b` (either may be
 // null), slab after slab.
 __global__ __launch_bounds__(1024) void norm_columns(const float* from, int64_t rows, int cols, int split,
                                                      float* to_a, float* to_b, int blocks) {
@@ -867,7 +872,7 @@ Launch launch_of(const fpscan_norm* p) {
   a.rows = l.threads / a.vecs;
   l.tokens = p->seqlen == 1;
   // A group at a time: up to kKept vectors a thread, tensors that stay in the L2 caches (their lines
-  // are read by several groups). 2 sequences of 256 steps, 256 channels in 32 groups, fp32: 5.0 us
+  // are read by several groups). 2 sequences of 256 steps, 256 channels in 32 groups, fp32: 5.1 us
   // against 14.5 of the three launches below; but at 14 vectors a thread (3 sequences of 1000 steps,
   // 776 channels in 8 groups, fp16), on 24 of the CUs, 50 and 44 us forward and backward against 18 and
   // 27.
@@ -884,7 +889,8 @@ Launch launch_of(const fpscan_norm* p) {
   l.lds = ((size_t)a.rows * (a.dim + a.groups) + a.groups) * sizeof(float);
   if (a.rows == 1) l.lds = 2 * (size_t)(a.dim + a.groups) * sizeof(float);
   // token by token: workgroups take rows in turn, so that parameters are loaded and their gradients
-  // summed in registers (forward with a workgroup a turn: 65 instead of 24 us for 16384 rows of 1024)
+  // summed in registers (forward with a workgroup a turn: 65 us against 24, now 20, for 16384
+  // rows of 1024)
   const int64_t turns = (a.batch + a.rows - 1) / a.rows;
   l.turns = turns < 2048 ? turns : 2048;
   l.blocks = (int)(turns < 1024 ? turns : 1024);
