@@ -8,18 +8,23 @@ reference module's contraction scan, csrc/main.cpp:10) with ``dimwise_groups``, 
 fused gate producer ``pscan_softplus`` (gates exp(-softplus(z) * rate) computed in the
 kernels), and ``lookback_overruns`` / ``check_lookback`` (the tiled paths' count of look-back
 waits that gave up, whose outputs are NaN).
+
+For layers whose recurrence has a matrix as its state: ``gated_delta`` (the gated delta rule,
+differentiable), ``gated_delta_forward`` (with states continued in place: prompts) and
+``gated_delta_step`` (token by token, from a pool of states: decoding); and for what follows or
+precedes it ``group_norm_channel_last`` (group norm with an activation or an activated gate,
+differentiable). None of the four has a reference counterpart.
 """
 from .ops import (PScan, PScanChannelLast, PScanSoftplus, check_lookback, dimwise_forward,
                   dimwise_groups, gated_delta, gated_delta_forward, gated_delta_step,
-                  group_norm_channel_last, lookback_overruns, pscan, pscan_channel_last, pscan_softplus,
-                  scan_backward,
-                  scan_backward_channel_last, scan_backward_softplus, scan_forward,
-                  scan_forward_channel_last, scan_forward_softplus)
+                  group_norm_channel_last, lookback_overruns, pscan, pscan_channel_last,
+                  pscan_softplus, scan_backward, scan_backward_channel_last,
+                  scan_backward_softplus, scan_forward, scan_forward_channel_last,
+                  scan_forward_softplus)
 
 __all__ = ["pscan", "scan_forward", "scan_backward", "PScan", "pscan_channel_last",
            "scan_forward_channel_last", "scan_backward_channel_last", "PScanChannelLast",
            "dimwise_forward", "dimwise_groups", "pscan_softplus", "scan_forward_softplus",
-           "scan_backward_softplus", "PScanSoftplus", "gated_delta", "gated_delta_forward", "gated_delta_step",
-           "group_norm_channel_last",
-           "lookback_overruns", "check_lookback"]
+           "scan_backward_softplus", "PScanSoftplus", "gated_delta", "gated_delta_forward",
+           "gated_delta_step", "group_norm_channel_last", "lookback_overruns", "check_lookback"]
 __version__ = "0.2.0"

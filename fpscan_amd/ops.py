@@ -29,7 +29,8 @@ import torch
 
 __all__ = ["pscan", "scan_forward", "scan_backward", "PScan", "pscan_channel_last",
            "scan_forward_channel_last", "scan_backward_channel_last", "PScanChannelLast",
-           "pscan_softplus", "scan_forward_softplus", "scan_backward_softplus", "PScanSoftplus"]
+           "pscan_softplus", "scan_forward_softplus", "scan_backward_softplus", "PScanSoftplus",
+           "gated_delta", "gated_delta_forward", "gated_delta_step", "group_norm_channel_last"]
 
 _EXT_CANDIDATES = ("fpscan_amd._C",)
 _ext = None
