@@ -653,14 +653,17 @@ at::Tensor gated_delta_forward(const at::Tensor& q, const at::Tensor& k, const a
   return out;
 }
 
+bool starts_vector(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
 // grad_out as the kernels take it: its own strides where they are whole vectors and its steps apart
-// (a gradient of a sum is one value for all), else a copy.
+// (a gradient of a sum is one value for all), else a copy (a gradient of one of several tensors joined
+// may start anywhere).
 at::Tensor readable(const at::Tensor& t) {
   const int64_t vec = 16 / (int64_t)t.element_size();
-  bool ok = (t.size(3) <= 1 || t.stride(3) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  bool ok = (t.size(3) <= 1 || t.stride(3) == 1) && starts_vector(t);
   for (int64_t d = 0; d < 3; ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) % vec == 0);
   ok = ok && (t.size(1) <= 1 || t.stride(1) >= t.size(3));
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 // The gated delta rule as an autograd function in C++ (see PScanFunction). What the backward needs of
@@ -826,7 +829,9 @@ struct GroupNormFunction : public torch::autograd::Function<GroupNormFunction> {
     };
     at::Tensor gx = at::empty_like(x), gw = like(weight), gb = like(bias), gg = like(gate);
     if (!empty) {
-      const at::Tensor go = grads[0].contiguous();
+      const at::Tensor go = grads[0].is_contiguous() && starts_vector(grads[0])
+                                ? grads[0]
+                                : grads[0].clone(at::MemoryFormat::Contiguous);
       check_like(go, x, "grad_out", "x");
       c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
       void* stream = launch_stream(x);
