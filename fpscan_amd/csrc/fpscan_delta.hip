@@ -2017,7 +2017,9 @@ int fpscan_delta_step(const fpscan_delta* p, void* out, float* state, const int3
   a.slots = slots;
   a.nslots = nslots;
   a.vblocks = (a.Dv + 31) / 32;
-  const unsigned grid = (unsigned)((a.heads_total * a.vblocks + 3) / 4);
+  const int64_t groups = (a.heads_total * a.vblocks + 3) / 4;
+  if (groups >= (int64_t)1 << 24) return FPSCAN_ERR_SHAPE;  // a launch has fewer than 2^32 threads
+  const unsigned grid = (unsigned)groups;
   return by_type(p->dtype, padded_key_dim(p), [&](auto e, auto kd) {
     delta_steps<decltype(e), kd.value><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     return launched();

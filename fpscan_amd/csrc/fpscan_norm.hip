@@ -455,28 +455,29 @@ __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
 
 // The chunks of a sequence joined: a wave per (sequence, group), lanes over chunks.
 __global__ __launch_bounds__(256) void norm_join(NormArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  if (i >= a.batch * a.groups) return;
-  const int64_t b = i / a.groups;
-  const float* const part = a.part + (b * a.chunks * 2) * a.groups + (i - b * a.groups);
   const float full = (float)a.chunk_rows * (float)a.width;
   const float last = (float)(a.seqlen - (a.chunks - 1) * a.chunk_rows) * (float)a.width;
   const float inv = 1.0f / ((float)a.seqlen * (float)a.width);
-  const float base = part[0];  // as in norm_stats
-  float s = 0.0f;
-  for (int64_t k = lane; k < a.chunks; k += 64)
-    s = fmaf(k + 1 < a.chunks ? full : last, part[k * 2 * a.groups] - base, s);
-  const float mean = fmaf(wave_sum(s), inv, base);
-  float q = 0.0f;
-  for (int64_t k = lane; k < a.chunks; k += 64) {
-    const float d = part[k * 2 * a.groups] - mean;
-    q += fmaf((k + 1 < a.chunks ? full : last) * d, d, part[(k * 2 + 1) * a.groups]);
-  }
-  q = wave_sum(q);
-  if (lane == 0) {
-    a.mean[i] = mean;
-    a.rstd[i] = __builtin_amdgcn_rsqf(fmaf(q, inv, a.eps));
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.batch * a.groups;
+       i += (int64_t)gridDim.x * 4) {
+    const int64_t b = i / a.groups;
+    const float* const part = a.part + (b * a.chunks * 2) * a.groups + (i - b * a.groups);
+    const float base = part[0];  // as in norm_stats
+    float s = 0.0f;
+    for (int64_t k = lane; k < a.chunks; k += 64)
+      s = fmaf(k + 1 < a.chunks ? full : last, part[k * 2 * a.groups] - base, s);
+    const float mean = fmaf(wave_sum(s), inv, base);
+    float q = 0.0f;
+    for (int64_t k = lane; k < a.chunks; k += 64) {
+      const float d = part[k * 2 * a.groups] - mean;
+      q += fmaf((k + 1 < a.chunks ? full : last) * d, d, part[(k * 2 + 1) * a.groups]);
+    }
+    q = wave_sum(q);
+    if (lane == 0) {
+      a.mean[i] = mean;
+      a.rstd[i] = __builtin_amdgcn_rsqf(fmaf(q, inv, a.eps));
+    }
   }
 }
 
@@ -798,30 +799,34 @@ __global__ __launch_bounds__(1024) void norm_groups_bwd(NormArgs a) {
 // (a row's 64 bytes at a time; 64 columns by 16 threads left most CUs without work: 38 us against 9, now
 // 4.9, for 2048 rows of 2048). The first `split` columns go to `to_a`, the others to `to_b` (either may be
 // null), slab after slab.
-__global__ __launch_bounds__(1024) void norm_columns(const float* from, int64_t rows, int cols, int split,
-                                                     float* to_a, float* to_b, int blocks) {
+__global__ __launch_bounds__(1024) void norm_columns(const float* from, int64_t slabs, int64_t rows,
+                                                     int cols, int split, float* to_a, float* to_b,
+                                                     int blocks) {
   __shared__ float lds[64][17];
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-  const int64_t slab = blockIdx.x / blocks;
-  const int c = (int)(blockIdx.x - slab * blocks) * 16 + x;
-  float s = 0.0f;
-  if (c < cols) {
-    const float* p = from + (slab * rows + y) * cols + c;
+  for (int64_t i = blockIdx.x; i < slabs * blocks; i += gridDim.x) {
+    const int64_t slab = i / blocks;
+    const int c = (int)(i - slab * blocks) * 16 + x;
+    float s = 0.0f;
+    if (c < cols) {
+      const float* p = from + (slab * rows + y) * cols + c;
 #pragma unroll 8
-    for (int64_t r = y; r < rows; r += 64, p += (int64_t)64 * cols) s += *p;
-  }
-  lds[y][x] = s;
-  __syncthreads();
-  for (int n = 32; n > 0; n >>= 1) {
-    if (y < n) lds[y][x] += lds[y + n][x];
+      for (int64_t r = y; r < rows; r += 64, p += (int64_t)64 * cols) s += *p;
+    }
+    __syncthreads();  // the sums before are read
+    lds[y][x] = s;
     __syncthreads();
-  }
-  if (y == 0 && c < cols) {
-    s = lds[0][x];
-    if (c < split) {
-      if (to_a) to_a[slab * split + c] = s;
-    } else if (to_b) {
-      to_b[slab * (cols - split) + c - split] = s;
+    for (int n = 32; n > 0; n >>= 1) {
+      if (y < n) lds[y][x] += lds[y + n][x];
+      __syncthreads();
+    }
+    if (y == 0 && c < cols) {
+      s = lds[0][x];
+      if (c < split) {
+        if (to_a) to_a[slab * split + c] = s;
+      } else if (to_b) {
+        to_b[slab * (cols - split) + c - split] = s;
+      }
     }
   }
 }
@@ -905,6 +910,13 @@ Launch launch_of(const fpscan_norm* p) {
   return l;
 }
 
+// A launch has fewer than 2^32 threads: joins and column sums of more workgroups go in turns, more chunks
+// of rows are refused.
+constexpr int64_t kMostGroups = (int64_t)1 << 21;
+bool too_many(const Launch& l) {
+  return !l.tokens && !l.group_threads && (__int128)l.a.batch * l.a.chunks * l.threads >= (__int128)1 << 32;
+}
+
 char* take(char*& at, size_t bytes) {
   char* p = at;
   at += (bytes + 255) & ~(size_t)255;
@@ -955,8 +967,9 @@ int launch(K kernel, const Launch& l, int64_t blocks, hipStream_t stream) {
 int columns(const float* from, int64_t slabs, int64_t rows, int dim, float* to_a, float* to_b, int split,
             hipStream_t stream) {
   const int blocks = (2 * dim + 15) / 16;
-  norm_columns<<<(unsigned)(slabs * blocks), 1024, 0, stream>>>(from, rows, 2 * dim, split, to_a, to_b,
-                                                               blocks);
+  const int64_t all = slabs * blocks;
+  norm_columns<<<(unsigned)(all < kMostGroups ? all : kMostGroups), 1024, 0, stream>>>(
+      from, slabs, rows, 2 * dim, split, to_a, to_b, blocks);
   return launched();
 }
 
@@ -985,7 +998,7 @@ int fpscan_norm_fwd(const fpscan_norm* p, const void* x, const float* weight, co
   if (!aligned16({x, gate, out, workspace}) || ((uintptr_t)weight | (uintptr_t)bias | (uintptr_t)stats) % 4)
     return FPSCAN_ERR_ALIGN;
   Launch l = launch_of(p);
-  if ((!l.tokens && l.a.batch * l.a.chunks >= (int64_t)1 << 31)) return FPSCAN_ERR_SHAPE;
+  if (too_many(l)) return FPSCAN_ERR_SHAPE;
   if (workspace_bytes < fpscan_norm_workspace_bytes(p, FPSCAN_OP_FWD)) return FPSCAN_ERR_WORKSPACE;
   carve(static_cast<char*>(workspace), l, false, stats == nullptr);
   NormArgs& a = l.a;
@@ -1011,7 +1024,8 @@ int fpscan_norm_fwd(const fpscan_norm* p, const void* x, const float* weight, co
     }
     int st = launch(norm_stats<E>, l, a.batch * a.chunks, s);
     if (st != FPSCAN_OK) return st;
-    norm_join<<<(unsigned)((a.batch * a.groups + 3) / 4), 256, 0, s>>>(a);
+    const int64_t joins = (a.batch * a.groups + 3) / 4;
+    norm_join<<<(unsigned)(joins < kMostGroups ? joins : kMostGroups), 256, 0, s>>>(a);
     if ((st = launched()) != FPSCAN_OK) return st;
     return launch(norm_apply<E, act.value, gated.value>, l, a.batch * a.chunks, s);
   });
@@ -1031,7 +1045,7 @@ int fpscan_norm_bwd(const fpscan_norm* p, const void* x, const float* weight, co
        (uintptr_t)grad_bias) % 4)
     return FPSCAN_ERR_ALIGN;
   Launch l = launch_of(p);
-  if ((!l.tokens && l.a.batch * l.a.chunks >= (int64_t)1 << 31)) return FPSCAN_ERR_SHAPE;
+  if (too_many(l)) return FPSCAN_ERR_SHAPE;
   if (workspace_bytes < fpscan_norm_workspace_bytes(p, FPSCAN_OP_BWD)) return FPSCAN_ERR_WORKSPACE;
   carve(static_cast<char*>(workspace), l, true, false);
   NormArgs& a = l.a;
