@@ -382,7 +382,7 @@ __device__ __forceinline__ void by_two(const NormArgs& a, const Place& p, const 
 
 // Whole sequences, each tensor read twice, as a sequence's statistics come first: 16384 steps of 8
 // sequences, 1024 channels in 32 groups, bf16: norm_stats 60 us (4.5 TB/s), norm_join 6, norm_apply 85
-// (6.3); backward norm_sums_bwd 123 (4.4), norm_apply_bwd 154 (5.2), norm_columns 14.
+// (6.3); backward norm_sums_bwd 123 (4.4), norm_apply_bwd 155 (5.2), norm_columns 9.
 template <class E>
 __global__ __launch_bounds__(1024) void norm_stats(NormArgs a) {
   constexpr int V = E::V;
